@@ -171,6 +171,11 @@ def prepare(case, seed):
     s["k_lengths"] = lengths
     index = torch.arange(tk, device="cuda").expand(b, tk)
     document = None
+    # where the queries stand among the keys: the whole sequence, or the newest of what is stored
+    newest = torch.arange(tk, device="cuda").expand(b, tk)
+    if tq < tk:
+        last = torch.full((b,), tk, device="cuda") if lengths is None else lengths.long()
+        newest = (last[:, None] - tq + torch.arange(tq, device="cuda")).clamp(min=0)
     if case["documents"]:
         # borders anywhere; in packed sequences the last twentieth is left empty
         edge = torch.rand(b, case["documents"] - 1, generator=g, device="cuda").mul_(0.95 * tk).long().sort(1)[0]
@@ -180,13 +185,13 @@ def prepare(case, seed):
         empty = torch.arange(tk, device="cuda") >= (max(1, int(0.95 * tk)) if tq == tk else tk)
         document = document.masked_fill(empty, -1).to(torch.int32)
     s["k_documents"] = document
-    s["q_documents"] = None if document is None else document[:, tk - tq:].contiguous()
+    s["q_documents"] = None if document is None else document.gather(1, newest)
     s["k_positions"] = s["q_positions"] = s["slopes"] = s["prefix"] = None
     if case["bias"] != "none":
         s["slopes"] = (2.0 ** -(1 + 7 * torch.rand(h, generator=g, device="cuda"))).requires_grad_(case["train"])
     if case["bias"] == "grid":
         s["k_positions"] = _grid_positions(index)
-        s["q_positions"] = s["k_positions"][:, tk - tq:].contiguous()
+        s["q_positions"] = _grid_positions(index.gather(1, newest))
     if case["mask"] == "prefix":
         s["prefix"] = torch.randint(tk // 8, tk // 4 + 1, (b,), generator=g, device="cuda", dtype=torch.int32)
     if case["train"]:
