@@ -272,6 +272,108 @@ int wst_probe_fma(float* d_scratch, int64_t nthreads, int iters, void* stream);
 /* Thread-local message of the last failed wst_noise_* / wst_advanced_stats call. */
 const char* wst_aux_last_error(void);
 
+/* ------------------------------------------------------------------------------------------
+ * Token operators (csrc/wst_tokens.hip, csrc/wst_attention.hip): what a network behind the transform does with its
+ * maps.  A map's points are tokens, its coefficients (of all channels) their values.  No kymatio counterpart; the
+ * reference's fixed read-out of the same maps is the mean | std of train_and_save_model.py:371-375.
+ *
+ * Strides are in elements.  Workspaces are the caller's; a call keeps nothing and two calls may run at once when each
+ * has its own.  All calls are asynchronous on `stream`, capturable into a graph, and repeat bit for bit.
+ * ------------------------------------------------------------------------------------------ */
+
+enum wst_dtype { WST_F32 = 0, WST_BF16 = 1, WST_F16 = 2 };
+
+#define WST_MAX_AXES 4
+#define WST_MAX_HEAD_DIM 256
+
+/* Thread-local message of the last failed wst_layer_norm_* / wst_rotary / wst_attention_* call. */
+const char* wst_tokens_last_error(void);
+
+/*
+ * Layer norm over the n values of each of batch x points tokens: y = (x - mean) / sqrt(var + eps) * weight + bias
+ * (population variance).  The values of a token are adjacent (x_stride_n == 1), or its points are
+ * (x_stride_point == 1: the transform's maps, read where they lie).  y and dy are contiguous (batch, points, n).
+ * weight, bias and their gradients have type w_dtype; weight == NULL is 1, bias == NULL is 0.
+ */
+typedef struct wst_norm_desc {
+    int64_t batch, points, n;
+    int64_t x_stride_batch, x_stride_point, x_stride_n;
+    int64_t dx_stride_batch, dx_stride_point, dx_stride_n;   /* backward: must lie as x does */
+    int32_t x_dtype, y_dtype, w_dtype;
+    float eps;
+} wst_norm_desc;
+
+/* mean, rstd: float32 (batch, points), for the backward pass; both may be NULL. */
+int wst_layer_norm_forward(const wst_norm_desc* d, const void* x, const void* weight, const void* bias, void* y,
+                           float* mean, float* rstd, void* stream);
+int wst_layer_norm_workspace(const wst_norm_desc* d, size_t* bytes);
+/* dx, dweight, dbias: each may be NULL when not wanted. */
+int wst_layer_norm_backward(const wst_norm_desc* d, const void* x, const void* weight, const void* dy,
+                            const float* mean, const float* rstd, void* dx, void* dweight, void* dbias,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Rotary positions with several axes: of a head's dim values, the first 2 * sum(sections) are turned in pairs, the
+ * rest copied.  Axis a has sections[a] pairs, the i-th turned by position[a] * base^(-i / sections[a]).  With P pairs
+ * in all, pair p is (p, p + P), or (2p, 2p + 1) when interleaved.  inverse != 0 turns back: the gradient.  q and k are
+ * (batch, tokens, heads, dim) with adjacent dim; strides are batch, token, head; either may have no heads.  q_out may
+ * be q, k_out may be k.  positions: int32 (batch, tokens, axes), or (tokens, axes) when positions_shared.
+ */
+typedef struct wst_rotary_desc {
+    int64_t batch, tokens;
+    int64_t q_strides[3], k_strides[3], q_out_strides[3], k_out_strides[3];
+    double base;
+    int32_t q_heads, k_heads, dim, dtype;
+    int32_t axes, sections[WST_MAX_AXES];
+    int32_t interleaved, inverse, positions_shared;
+} wst_rotary_desc;
+
+int wst_rotary(const wst_rotary_desc* d, const void* q, void* q_out, const void* k, void* k_out,
+               const int32_t* positions, void* stream);
+
+/*
+ * Attention.  q, o: (batch, q_len, q_heads, dim); k, v: (batch, k_len, k_heads, dim), dim adjacent, strides batch,
+ * token, head; q head h reads k head h / (q_heads / k_heads).  For query i and key j of batch entry b, with
+ * L = k_lengths ? k_lengths[b] (clamped to 0..k_len) : k_len and place(i) = i + L - q_len:
+ *   z = scale * q_i . k_j;  z = cap * tanh(z / cap) if cap > 0;  s = z - slopes[h] * distance(i, j)
+ *   distance = sum over axes of |q_pos[i] - k_pos[j]|, or |place(i) - j| without positions
+ *   key j is seen iff j < L, and (causal) j <= place(i) or j < prefix[b], and (documents) q_doc[i] == k_doc[j] >= 0
+ *   o_i = sum_j softmax(s_i)_j v_j over the keys seen; a query that sees none gets 0 (and lse = -inf, no gradient).
+ * What is not seen has no influence, infinities and NaN included.  Scores, softmax and sums are float32; the weights
+ * that multiply v, and the score gradients that multiply q and k, are rounded to the inputs' type.
+ * Coordinates lie in [-2^29, 2^29).
+ */
+typedef struct wst_attention_desc {
+    int64_t batch, q_len, k_len;
+    int64_t q_strides[3], k_strides[3], v_strides[3], o_strides[3];
+    int64_t q_pos_stride, k_pos_stride, q_doc_stride, k_doc_stride;   /* of a batch entry; 0 when shared */
+    const void *q, *k, *v;
+    const float* slopes;                       /* (q_heads) or NULL: no distance bias */
+    const int32_t *q_pos, *k_pos;              /* (q_len, axes), (k_len, axes) or both NULL */
+    const int32_t *q_doc, *k_doc;              /* (q_len), (k_len) or both NULL; negative: belongs to none */
+    const int32_t* k_lengths;                  /* (batch) or NULL */
+    const int32_t* prefix;                     /* (batch) or NULL; needs causal */
+    float scale, cap;
+    int32_t q_heads, k_heads, dim, dtype, axes, causal;
+} wst_attention_desc;
+
+/* Bytes of workspace of a forward (backward == 0) or backward call. */
+int wst_attention_workspace(const wst_attention_desc* d, int backward, size_t* bytes);
+/* lse: float32 (batch, q_heads, q_len), log of the softmax's sum, for the backward pass; may be NULL. */
+int wst_attention_forward(const wst_attention_desc* d, void* o, float* lse, void* workspace, size_t workspace_bytes,
+                          void* stream);
+/* o, lse: of the forward call.  grads: do, dq, dk, dv with the strides given; dq, dk, dv, dslopes (float32 (q_heads))
+ * may each be NULL when not wanted. */
+typedef struct wst_attention_grads {
+    const void *o, *d_o;
+    const float* lse;
+    void *dq, *dk, *dv;
+    float* dslopes;
+    int64_t do_strides[3], dq_strides[3], dk_strides[3], dv_strides[3];
+} wst_attention_grads;
+int wst_attention_backward(const wst_attention_desc* d, const wst_attention_grads* g, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -31,6 +31,9 @@ EXPORTS = (
     "wst_patch_generate", "wst_u8_to_chw", "wst_probe_copy", "wst_probe_fma",
     "wst_aux_last_error", "wst_plan_variants", "wst_describe_variants", "wst_plan_trace",
     "wst_plan_read_trace",
+    "wst_tokens_last_error", "wst_layer_norm_forward", "wst_layer_norm_workspace",
+    "wst_layer_norm_backward", "wst_rotary", "wst_attention_workspace", "wst_attention_forward",
+    "wst_attention_backward",
 )
 
 _lib = None
@@ -68,6 +71,45 @@ def _conv_ptr(convention):
         rot32 = getattr(convention, "rot_dtype", _np.float64) == _np.float32
         convention = Convention(convention.norm_pi, convention.periodize_half, rot_f32=rot32)
     return ctypes.byref(convention)
+
+
+_I64, _I32, _PTR = ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p
+_STRIDES = _I64 * 3
+MAX_AXES, MAX_HEAD_DIM = 4, 256
+
+
+class NormDesc(ctypes.Structure):
+    """``wst_norm_desc`` (include/wst_hip.h)."""
+    _fields_ = [(n, _I64) for n in ("batch", "points", "n", "x_stride_batch", "x_stride_point", "x_stride_n",
+                                    "dx_stride_batch", "dx_stride_point", "dx_stride_n")] + \
+               [("x_dtype", _I32), ("y_dtype", _I32), ("w_dtype", _I32), ("eps", ctypes.c_float)]
+
+
+class RotaryDesc(ctypes.Structure):
+    """``wst_rotary_desc``."""
+    _fields_ = [("batch", _I64), ("tokens", _I64), ("q_strides", _STRIDES), ("k_strides", _STRIDES),
+                ("q_out_strides", _STRIDES), ("k_out_strides", _STRIDES), ("base", ctypes.c_double),
+                ("q_heads", _I32), ("k_heads", _I32), ("dim", _I32), ("dtype", _I32), ("axes", _I32),
+                ("sections", _I32 * MAX_AXES), ("interleaved", _I32), ("inverse", _I32),
+                ("positions_shared", _I32)]
+
+
+class AttentionDesc(ctypes.Structure):
+    """``wst_attention_desc``."""
+    _fields_ = [("batch", _I64), ("q_len", _I64), ("k_len", _I64), ("q_strides", _STRIDES),
+                ("k_strides", _STRIDES), ("v_strides", _STRIDES), ("o_strides", _STRIDES),
+                ("q_pos_stride", _I64), ("k_pos_stride", _I64), ("q_doc_stride", _I64),
+                ("k_doc_stride", _I64)] + \
+               [(n, _PTR) for n in ("q", "k", "v", "slopes", "q_pos", "k_pos", "q_doc", "k_doc", "k_lengths",
+                                    "prefix")] + \
+               [("scale", ctypes.c_float), ("cap", ctypes.c_float), ("q_heads", _I32), ("k_heads", _I32),
+                ("dim", _I32), ("dtype", _I32), ("axes", _I32), ("causal", _I32)]
+
+
+class AttentionGrads(ctypes.Structure):
+    """``wst_attention_grads``."""
+    _fields_ = [(n, _PTR) for n in ("o", "d_o", "lse", "dq", "dk", "dv", "dslopes")] + \
+               [(n, _STRIDES) for n in ("do_strides", "dq_strides", "dk_strides", "dv_strides")]
 
 
 class WSTError(RuntimeError):
@@ -187,6 +229,20 @@ def _open(path, name) -> ctypes.CDLL:
         lib.wst_plan_trace.argtypes = [c_vp, c_int]
         lib.wst_plan_read_trace.restype = c_int
         lib.wst_plan_read_trace.argtypes = [c_vp, c_vp, c_i64, i64p]
+    if hasattr(lib, "wst_tokens_last_error"):
+        norm_p, rot_p = ctypes.POINTER(NormDesc), ctypes.POINTER(RotaryDesc)
+        attn_p, grad_p = ctypes.POINTER(AttentionDesc), ctypes.POINTER(AttentionGrads)
+        lib.wst_tokens_last_error.restype = ctypes.c_char_p
+        lib.wst_tokens_last_error.argtypes = []
+        for fn, types in (("wst_layer_norm_forward", [norm_p] + [c_vp] * 7),
+                          ("wst_layer_norm_workspace", [norm_p, ctypes.POINTER(c_sz)]),
+                          ("wst_layer_norm_backward", [norm_p] + [c_vp] * 9 + [c_sz, c_vp]),
+                          ("wst_rotary", [rot_p] + [c_vp] * 6),
+                          ("wst_attention_workspace", [attn_p, c_int, ctypes.POINTER(c_sz)]),
+                          ("wst_attention_forward", [attn_p] + [c_vp] * 3 + [c_sz, c_vp]),
+                          ("wst_attention_backward", [attn_p, grad_p, c_vp, c_sz, c_vp])):
+            getattr(lib, fn).restype = c_int
+            getattr(lib, fn).argtypes = types
     v = lib.wst_abi_version()
     if v != ABI_VERSION:
         raise RuntimeError(f"{name} ABI version {v} != expected {ABI_VERSION}; rebuild it")
@@ -205,6 +261,12 @@ def check_aux(code: int) -> None:
     """Status check of the wst_noise_* / wst_advanced_stats entry points."""
     if code != WST_OK:
         raise WSTError(code, aux_last_error() or f"wst status {code}")
+
+
+def check_tokens(code: int) -> None:
+    """Status check of the wst_layer_norm_* / wst_rotary / wst_attention_* entry points."""
+    if code != WST_OK:
+        raise WSTError(code, (load().wst_tokens_last_error() or b"").decode() or f"wst status {code}")
 
 
 def check(code: int) -> None:

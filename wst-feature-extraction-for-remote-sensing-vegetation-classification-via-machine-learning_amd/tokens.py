@@ -1,0 +1,410 @@
+"""Operators on coefficient tokens: what a network behind the transform does with its maps.
+
+A scattering map of (C, K, Mo, No) is a sequence of Mo * No tokens of C * K values each.  The reference reads such maps
+out by the mean and standard deviation of each coefficient (train_and_save_model.py:371-375); these operators are the
+learned counterpart, for training and inference:
+
+* ``layer_norm``  -- over a token's values; reads tokens, or maps where the transform wrote them;
+* ``rotary``      -- positions with several axes (time, row, column) turned into queries and keys;
+* ``attention``   -- scores capped by tanh, a bias that depends on distance, documents, order and a prefix.
+
+All run in the HIP library on the tensors' device and current stream, have gradients (torch autograd, first order), and
+can be captured into a graph.  float32, bfloat16 and float16; sums and statistics are held in float32.  There is no CPU
+execution: tensors must live on a ROCm GPU.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .frontend import require_gpu
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _dtype_id(t, name):
+    try:
+        return DTYPES[t.dtype]
+    except KeyError:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, not {t.dtype}") from None
+
+
+def _check_tensor(t, name, like=None):
+    if not torch.is_tensor(t):
+        raise TypeError(f"{name} must be a PyTorch Tensor.")
+    if not t.is_cuda:
+        require_gpu()
+        raise RuntimeError(f"{name} must be on a ROCm GPU, not on {t.device}")
+    if like is not None and t.device != like.device:
+        raise RuntimeError(f"{name} is on {t.device}, expected {like.device}")
+
+
+def _check_ints(t, name, like):
+    _check_tensor(t, name, like)
+    if t.dtype != torch.int32:
+        raise TypeError(f"{name} must be int32, not {t.dtype}")
+
+
+def _call(device, fn, *args):
+    """Run a library call on the tensors' device and its current stream, and check the status."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if device.index == torch.cuda.current_device():
+        _lib.check_tokens(fn(*args, stream))
+    else:
+        with torch.cuda.device(device):
+            _lib.check_tokens(fn(*args, stream))
+
+
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+# ------------------------------------------------------------------------------------------ layer norm
+def _token_view(x):
+    """x (..., n) as (batch, points, n) strides the library reads, copied only when it has none."""
+    n = x.shape[-1]
+    lead = []                                   # (size, stride) of the leading dimensions, merged where adjacent
+    for size, stride in zip(x.shape[:-1], x.stride()[:-1]):
+        if size == 1:
+            continue
+        if lead and lead[-1][1] == size * stride:
+            lead[-1] = (lead[-1][0] * size, stride)
+        else:
+            lead.append((size, stride))
+    sn = x.stride(-1)
+    batch, sb = lead[0] if len(lead) == 2 else (1, 0)
+    points, sp = lead[-1] if lead else (1, n)
+    if len(lead) > 2 or not (sn == 1 or n == 1 or sp == 1 or points == 1):
+        x, rows = x.contiguous(), x.numel() // n
+        return x, (1, rows, n, 0, n, 1)
+    return x, (batch, points, n, sb, sp, sn)
+
+
+def _norm_desc(view, dview, x, out_dtype, weight, bias, eps):
+    w = weight if weight is not None else bias
+    return _lib.NormDesc(*view, *dview, DTYPES[x.dtype], DTYPES[out_dtype], 0 if w is None else DTYPES[w.dtype], eps)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _norm_forward(x, weight, bias, eps, out_dtype, stats):
+    xs, view = _token_view(x)
+    y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    mean = rstd = None
+    if stats:
+        mean, rstd = torch.empty((2, view[0] * view[1]), dtype=torch.float32, device=x.device).unbind(0)
+    if x.numel():
+        d = _norm_desc(view, (0, 0, 0), x, out_dtype, weight, bias, eps)
+        _call(x.device, _lib.load().wst_layer_norm_forward, d, xs.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(),
+              _ptr(mean), _ptr(rstd))
+    return y, xs, mean, rstd
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, out_dtype):
+        y, xs, mean, rstd = _norm_forward(x, weight, bias, eps, out_dtype, True)
+        ctx.save_for_backward(xs, weight, mean, rstd)
+        ctx.bias_like = None if bias is None else (bias.shape, bias.dtype)
+        ctx.eps, ctx.x_shape = eps, x.shape
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        xs, weight, mean, rstd = ctx.saved_tensors
+        want_x, want_w, want_b = ctx.needs_input_grad[:3]
+        dx = dw = db = None
+        dev = xs.device
+        if want_w:
+            dw = torch.empty_like(weight)
+        if want_b:
+            db = torch.empty(ctx.bias_like[0], dtype=ctx.bias_like[1], device=dev)
+        if not xs.numel():
+            return (torch.empty(ctx.x_shape, dtype=xs.dtype, device=dev) if want_x else None,
+                    dw.zero_() if want_w else None, db.zero_() if want_b else None, None, None)
+        _, view = _token_view(xs)
+        batch, points, n = view[:3]
+        dview = (points * n, n, 1)
+        if want_x:
+            if view[5] != 1 and n > 1:          # maps: the gradient lies as they do
+                dx = torch.empty((batch, n, points), dtype=xs.dtype, device=dev).transpose(1, 2)
+                dview = (points * n, 1, points)
+                dx = dx.view(ctx.x_shape)
+            else:
+                dx = torch.empty(ctx.x_shape, dtype=xs.dtype, device=dev)
+        dy = dy.contiguous()
+        d = _lib.NormDesc(*view, *dview, DTYPES[xs.dtype], DTYPES[dy.dtype],
+                          DTYPES[weight.dtype] if weight is not None else DTYPES[db.dtype] if want_b else 0, ctx.eps)
+        lib, need = _lib.load(), ctypes.c_size_t()
+        _lib.check_tokens(lib.wst_layer_norm_workspace(d, ctypes.byref(need)))
+        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        _call(dev, lib.wst_layer_norm_backward, d, xs.data_ptr(), _ptr(weight), dy.data_ptr(), mean.data_ptr(),
+              rstd.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), ws.data_ptr(), need.value)
+        return dx, dw, db, None, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, out_dtype=None):
+    """Layer norm over the last axis: ``(x - mean) / sqrt(var + eps) * weight + bias`` (population variance).
+
+    x (..., n) may lie with its values adjacent, or with its tokens adjacent: ``maps.flatten(-2).transpose(-1, -2)`` of
+    the transform's maps is read in place.  The result is contiguous, of ``out_dtype`` (default x's).  weight and bias
+    (n,) may have a type of their own, the same for both; either may be None."""
+    _check_tensor(x, "x")
+    _dtype_id(x, "x")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise RuntimeError("x must have a last axis of at least one value")
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype not in DTYPES:
+        raise TypeError(f"out_dtype must be float32, bfloat16 or float16, not {out_dtype}")
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is not None:
+            _check_tensor(t, name, x)
+            _dtype_id(t, name)
+            if t.shape != x.shape[-1:]:
+                raise RuntimeError(f"{name} must be of shape ({x.shape[-1]},), not {tuple(t.shape)}")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TypeError("weight and bias must have the same type")
+    eps = float(eps)
+    if not eps >= 0.0:
+        raise RuntimeError("eps must not be negative")
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    if _wants_grad(x, weight, bias):
+        return _LayerNorm.apply(x, weight, bias, eps, out_dtype)
+    return _norm_forward(x, weight, bias, eps, out_dtype, False)[0]
+
+
+# ------------------------------------------------------------------------------------------ rotary
+def grid_positions(frames, rows, cols, device=None):
+    """(frames * rows * cols, 3) int32 positions (time, row, column) of a series of maps, in the maps' order."""
+    axes = [torch.arange(n, dtype=torch.int32, device=device) for n in (frames, rows, cols)]
+    return torch.stack(torch.meshgrid(*axes, indexing="ij"), -1).reshape(-1, 3)
+
+
+def _rows_of(t):
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _strides(t):
+    return t.stride()[:3]
+
+
+def _rotate(q, k, positions, sections, base, interleaved, inverse):
+    q = _rows_of(q)
+    B, T, H, D = q.shape
+    qo = torch.empty((B, T, H, D), dtype=q.dtype, device=q.device)
+    ko, ks, kos, Hk = None, (0, 0, 0), (0, 0, 0), 0
+    if k is not None:
+        k = _rows_of(k)
+        ko, Hk = torch.empty(k.shape, dtype=k.dtype, device=k.device), k.shape[2]
+        ks, kos = _strides(k), _strides(ko)
+    d = _lib.RotaryDesc(B, T, _strides(q), ks, _strides(qo), kos, base, H, Hk, D, DTYPES[q.dtype], len(sections),
+                        sections, interleaved, inverse, positions.dim() == 2)
+    _call(q.device, _lib.load().wst_rotary, d, q.data_ptr(), qo.data_ptr(), _ptr(k), _ptr(ko), positions.data_ptr())
+    return qo, ko
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, sections, base, interleaved):
+        ctx.save_for_backward(positions)
+        ctx.how = (sections, base, interleaved)
+        qo, ko = _rotate(q, k, positions, sections, base, interleaved, 0)
+        return qo if k is None else (qo, ko)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk=None):
+        positions, = ctx.saved_tensors
+        gq, gk = _rotate(dq, dk, positions, *ctx.how, 1)
+        return gq, gk, None, None, None, None
+
+
+def rotary(q, positions, sections, base=10000.0, interleaved=False, k=None):
+    """Rotary positions with several axes.
+
+    q (B, T, H, D) and, in the same call, k (B, T, Hk, D); positions int32 (T, A) or (B, T, A), 1 <= A <= 4, such as
+    ``grid_positions``; sections: the pairs that each of the A axes turns.  The first 2 * sum(sections) values of a head
+    are turned, the rest copied.  Pair i of an axis with s pairs turns by ``position * base**(-i / s)``.  With P pairs in
+    all, pair p is the values (p, p + P), or (2p, 2p + 1) when ``interleaved``.  Returns q turned, or (q, k)."""
+    _check_tensor(q, "q")
+    _dtype_id(q, "q")
+    if q.dim() != 4:
+        raise RuntimeError("q must be (batch, tokens, heads, dim)")
+    B, T, _, D = q.shape
+    if k is not None:
+        _check_tensor(k, "k", q)
+        if k.dtype != q.dtype:
+            raise TypeError("q and k must have the same type")
+        if k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != D:
+            raise RuntimeError(f"k must be ({B}, {T}, heads, {D}), not {tuple(k.shape)}")
+    sections = tuple(int(s) for s in sections)
+    if not 1 <= len(sections) <= _lib.MAX_AXES or min(sections) < 0:
+        raise RuntimeError(f"sections must be 1 to {_lib.MAX_AXES} numbers of pairs")
+    if 2 * sum(sections) > D:
+        raise RuntimeError(f"{sum(sections)} pairs do not fit heads of {D} values")
+    _check_ints(positions, "positions", q)
+    A = len(sections)
+    if tuple(positions.shape) not in ((T, A), (B, T, A)):
+        raise RuntimeError(f"positions must be ({T}, {A}) or ({B}, {T}, {A}), not {tuple(positions.shape)}")
+    base = float(base)
+    if not 0.0 < base < float("inf"):
+        raise RuntimeError("base must be positive")
+    positions = positions.contiguous()
+    if _wants_grad(q, k):
+        return _Rotary.apply(q, k, positions, sections, base, bool(interleaved))
+    qo, ko = _rotate(q, k, positions, sections, base, bool(interleaved), 0)
+    return qo if k is None else (qo, ko)
+
+
+# ------------------------------------------------------------------------------------------ attention
+class _Side:
+    """The arguments of a call that have no gradient."""
+    __slots__ = ("scale", "cap", "q_pos", "k_pos", "q_doc", "k_doc", "k_lengths", "prefix", "causal")
+
+    def tensors(self):
+        return (self.q_pos, self.k_pos, self.q_doc, self.k_doc, self.k_lengths, self.prefix)
+
+
+def _attention_desc(q, k, v, slopes, side, o):
+    B, Tq, H, D = q.shape
+
+    def per_batch(t, dims):
+        return 0 if t is None or t.dim() < dims else t.stride(0)
+
+    return _lib.AttentionDesc(
+        B, Tq, k.shape[1], _strides(q), _strides(k), _strides(v), _strides(o), per_batch(side.q_pos, 3),
+        per_batch(side.k_pos, 3), per_batch(side.q_doc, 2), per_batch(side.k_doc, 2), q.data_ptr(), k.data_ptr(),
+        v.data_ptr(), _ptr(slopes), _ptr(side.q_pos), _ptr(side.k_pos), _ptr(side.q_doc), _ptr(side.k_doc),
+        _ptr(side.k_lengths), _ptr(side.prefix), side.scale, side.cap, H, k.shape[2], D, DTYPES[q.dtype],
+        0 if side.q_pos is None else side.q_pos.shape[-1], side.causal)
+
+
+def _workspace(d, backward, device):
+    lib, need = _lib.load(), ctypes.c_size_t()
+    _lib.check_tokens(lib.wst_attention_workspace(d, backward, ctypes.byref(need)))
+    return torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None, need.value
+
+
+def _attend(q, k, v, slopes, side, want_lse):
+    B, Tq, H, _ = q.shape
+    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, H, Tq), dtype=torch.float32, device=q.device) if want_lse else None
+    d = _attention_desc(q, k, v, slopes, side, o)
+    ws, size = _workspace(d, 0, q.device)
+    _call(q.device, _lib.load().wst_attention_forward, d, o.data_ptr(), _ptr(lse), _ptr(ws), size)
+    return o, lse
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, slopes, side):
+        o, lse = _attend(q, k, v, slopes, side, True)
+        ctx.save_for_backward(q, k, v, slopes, o, lse, *side.tensors())
+        ctx.side = side
+        ctx.mark_non_differentiable(lse)
+        return o, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do, _):
+        q, k, v, slopes, o, lse = ctx.saved_tensors[:6]
+        want = ctx.needs_input_grad
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if w else None
+                      for t, w in zip((q, k, v), want))
+        dslopes = torch.empty_like(slopes) if want[3] else None
+        if not q.numel() or not k.numel():
+            return tuple(None if t is None else t.zero_() for t in (dq, dk, dv, dslopes)) + (None,)
+        do = _rows_of(do)
+        d = _attention_desc(q, k, v, slopes, ctx.side, o)
+        none = (0, 0, 0)
+        g = _lib.AttentionGrads(o.data_ptr(), do.data_ptr(), lse.data_ptr(), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dslopes),
+                                _strides(do), *(none if t is None else _strides(t) for t in (dq, dk, dv)))
+        ws, size = _workspace(d, 1, q.device)
+        _call(q.device, _lib.load().wst_attention_backward, d, g, _ptr(ws), size)
+        return dq, dk, dv, dslopes, None
+
+
+def _check_side(t, name, like, shapes):
+    if t is None:
+        return None
+    _check_ints(t, name, like)
+    if tuple(t.shape) not in shapes:
+        raise RuntimeError(f"{name} must be of shape {' or '.join(str(s) for s in shapes)}, not {tuple(t.shape)}")
+    return t.contiguous()
+
+
+def attention(q, k, v, *, scale=None, cap=0.0, slopes=None, q_positions=None, k_positions=None, q_documents=None,
+              k_documents=None, causal=False, prefix=None, k_lengths=None, return_lse=False):
+    """Softmax attention of q (B, Tq, H, D) over k, v (B, Tk, Hk, D); H a multiple of Hk, D <= 256.
+
+    With ``L = k_lengths[b]`` (default Tk) and ``place(i) = i + L - Tq``, query i scores key j as
+    ``z = scale * q_i.k_j`` (scale defaults to ``D ** -0.5``), ``z = cap * tanh(z / cap)`` where ``cap > 0``, and
+    ``z - slopes[h] * distance``: slopes float32 (H,); the distance is the sum over axes of
+    ``|q_positions[i] - k_positions[j]|`` (int32 (T, A) or (B, T, A), A <= 4, within +-2**29), or ``|place(i) - j|``
+    without positions.  Key j is seen iff
+
+    * ``j < L`` (k_lengths int32 (B,): keys behind are not read into any result), and
+    * ``j <= place(i)`` where ``causal`` or a prefix is given, or ``j < prefix[b]`` (int32 (B,)), and
+    * ``q_documents[i] == k_documents[j] >= 0`` where given (int32 (T,) or (B, T); negative belongs to none).
+
+    What is not seen has no influence, not even infinities or NaN.  A query that sees nothing gets 0, and no gradient.
+    Gradients reach q, k, v and slopes.  Returns o (B, Tq, H, D), and with ``return_lse`` the float32 (B, H, Tq)
+    log-sum-exp of the scores (-inf where nothing is seen; it has no gradient)."""
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        _check_tensor(t, name, q if t is not q else None)
+        _dtype_id(t, name)
+        if t.dim() != 4:
+            raise RuntimeError(f"{name} must be (batch, tokens, heads, dim)")
+        if t.dtype != q.dtype:
+            raise TypeError("q, k and v must have the same type")
+    B, Tq, H, D = q.shape
+    Tk, Hk = k.shape[1:3]
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+        raise RuntimeError(f"k and v must be ({B}, tokens, heads, {D}), not {tuple(k.shape)} and {tuple(v.shape)}")
+    if Hk < 1 or H < 1 or H % Hk:
+        raise RuntimeError(f"{H} query heads do not share {Hk} key heads evenly")
+    if not 1 <= D <= _lib.MAX_HEAD_DIM:
+        raise RuntimeError(f"heads must have 1 to {_lib.MAX_HEAD_DIM} values, not {D}")
+    if slopes is not None:
+        _check_tensor(slopes, "slopes", q)
+        if slopes.dtype != torch.float32:
+            raise TypeError(f"slopes must be float32, not {slopes.dtype}")
+        if slopes.shape != (H,):
+            raise RuntimeError(f"slopes must be of shape ({H},), not {tuple(slopes.shape)}")
+        slopes = slopes.contiguous()
+    if (q_positions is None) != (k_positions is None) or (q_documents is None) != (k_documents is None):
+        raise RuntimeError("positions and documents are given for queries and keys alike")
+    if q_positions is not None and slopes is None:
+        raise RuntimeError("positions are of use with slopes only")
+    s = _Side()
+    A = 0
+    if q_positions is not None and torch.is_tensor(q_positions):
+        A = q_positions.shape[-1] if q_positions.dim() else 0
+        if not 1 <= A <= _lib.MAX_AXES:
+            raise RuntimeError(f"positions must have 1 to {_lib.MAX_AXES} axes")
+    s.q_pos = _check_side(q_positions, "q_positions", q, ((Tq, A), (B, Tq, A)))
+    s.k_pos = _check_side(k_positions, "k_positions", q, ((Tk, A), (B, Tk, A)))
+    s.q_doc = _check_side(q_documents, "q_documents", q, ((Tq,), (B, Tq)))
+    s.k_doc = _check_side(k_documents, "k_documents", q, ((Tk,), (B, Tk)))
+    s.k_lengths = _check_side(k_lengths, "k_lengths", q, ((B,),))
+    s.prefix = _check_side(prefix, "prefix", q, ((B,),))
+    s.causal = bool(causal) or prefix is not None
+    s.scale = D ** -0.5 if scale is None else float(scale)
+    s.cap = float(cap)
+    if not 0.0 <= s.cap < float("inf"):
+        raise RuntimeError("cap must be finite and not negative")
+    if not abs(s.scale) < float("inf"):
+        raise RuntimeError("scale must be finite")
+    q, k, v = _rows_of(q), _rows_of(k), _rows_of(v)
+    if _wants_grad(q, k, v, slopes):
+        o, lse = _Attention.apply(q, k, v, slopes, s)
+    else:
+        o, lse = _attend(q, k, v, slopes, s, return_lse)
+    return (o, lse) if return_lse else o
