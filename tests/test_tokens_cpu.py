@@ -189,3 +189,11 @@ def test_token_view_copies_what_it_cannot_read():
     x = torch.zeros(2, 3, 4, 5)[:, ::2, :, ::2]
     t, got = tokens._token_view(x)
     assert t.is_contiguous() and tuple(got) == (1, 16, 3, 0, 3, 1)
+
+
+@pytest.mark.parametrize("sizes", [dict(batch=0), dict(q_len=0), dict(k_len=0), dict(q_len=0, k_len=0), dict()])
+@pytest.mark.parametrize("dim", [8, 5, 128])
+def test_attention_workspace_of_empty_sizes(sizes, dim):
+    lib, need = _lib.load(), ctypes.c_size_t(1)
+    for backward in (0, 1):
+        assert lib.wst_attention_workspace(_attn(dim=dim, slopes=256, **sizes), backward, ctypes.byref(need)) == 0
