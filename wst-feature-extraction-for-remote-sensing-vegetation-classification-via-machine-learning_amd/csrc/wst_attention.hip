@@ -443,6 +443,31 @@ struct Stage {
     }
 };
 
+// N rows of a tensor straight into LDS, past the registers: each lane names the 16 bytes it wants, the sixteen-byte units
+// of a wave land one after the other. Swizzling is done by choosing the source. What does not exist, or belongs to no
+// document, is fetched from a line of zeros. The compiler does not know of these loads: arrived() waits for them.
+__device__ const u32x4 g_zero = {0, 0, 0, 0};
+
+template <typename T, int DP, int N, int TH>
+struct Fetch {
+    using L = Tile<T, DP>;
+    static_assert(N * L::kUnits % TH == 0, "whole waves");
+    static __device__ __forceinline__ void issue(const T* base, int64_t stride, int64_t row0, int64_t rows, const int32_t* doc, int dim,
+                                                 const char* tile, int t) {
+        const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((WST_LDS const char*)tile)) + (t & ~63) * 16;
+#pragma unroll
+        for (int i = 0; i < N * L::kUnits / TH; ++i) {
+            const int id = t + i * TH, row = id / L::kUnits, unit = (id % L::kUnits) ^ L::swizzle(row);
+            bool ok = row0 + row < rows && unit * L::kElems < dim;
+            if (doc) ok = ok && doc[row0 + row < rows ? row0 + row : row0] >= 0;
+            const void* src = ok ? static_cast<const void*>(base + (row0 + row) * stride + unit * L::kElems) : static_cast<const void*>(&g_zero);
+            const uint32_t dst = __builtin_amdgcn_readfirstlane(lds + i * TH * 16);
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(dst), "v"(src) : "memory", "m0");
+        }
+    }
+};
+__device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+
 // Eight values of a row as an operand fragment, from memory; zero beyond the head or where the row is not to be read.
 template <typename T, int DP>
 __device__ __forceinline__ void row_frags(const T* row, bool ok, int dim, Frag<T> (&f)[DP / 16]) {
@@ -691,8 +716,8 @@ constexpr int kBQ = 128, kBK = 64;
 template <typename T, int DP>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(AttnArgs a) {
     using L = Tile<T, DP>;
-    __shared__ __attribute__((aligned(256))) char kt[kBK * L::kRowBytes], vt[kBK * L::kRowBytes];
-    __shared__ Along al;
+    __shared__ __attribute__((aligned(256))) char kt[2][kBK * L::kRowBytes], vt[2][kBK * L::kRowBytes];
+    __shared__ Along al[2];
     __shared__ Marks marks;
     __shared__ float scratch[4][DP];
     const wst_attention_desc& d = a.d;
@@ -731,39 +756,36 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(AttnAr
     float m = -INFINITY, l = 0.f;
 
     const T *kb = at<T>(d.k, d.k_strides, b, 0, kvh), *vb = at<T>(d.v, d.v_strides, b, 0, kvh);
-    Stage<T, DP, kBK, 256> ks, vs;
     AlongStage as;
+    auto fetch = [&](int64_t n, int buf) {
+        Fetch<T, DP, kBK, 256>::issue(kb, d.k_strides[1], n * kBK, sc.length, sc.k_doc, d.dim, kt[buf], t);
+        Fetch<T, DP, kBK, 256>::issue(vb, d.v_strides[1], n * kBK, sc.length, sc.k_doc, d.dim, vt[buf], t);
+        as.load(sc.k_pos, sc.k_doc, sc.axes, n * kBK, sc.length, t);
+    };
     int64_t tile = next_tile(marks, marked, -1, 0, tiles);
+    int buf = 0;
     if (tile < tiles) {
-        ks.load(kb, d.k_strides[1], tile * kBK, sc.length, sc.k_doc, d.dim, t);
-        vs.load(vb, d.v_strides[1], tile * kBK, sc.length, sc.k_doc, d.dim, t);
-        as.load(sc.k_pos, sc.k_doc, sc.axes, tile * kBK, sc.length, t);
+        fetch(tile, 0);
+        as.store(al[0], t);
     }
     while (tile < tiles) {
-        const int64_t key0 = tile * kBK;
-        __syncthreads();
-        ks.store(kt, t);
-        vs.store(vt, t);
-        as.store(al, t);
-        __syncthreads();
-        const int64_t next = next_tile(marks, marked, tile, 0, tiles);
-        if (next < tiles) {
-            ks.load(kb, d.k_strides[1], next * kBK, sc.length, sc.k_doc, d.dim, t);
-            vs.load(vb, d.v_strides[1], next * kBK, sc.length, sc.k_doc, d.dim, t);
-            as.load(sc.k_pos, sc.k_doc, sc.axes, next * kBK, sc.length, t);
-        }
+        const int64_t key0 = tile * kBK, next = next_tile(marks, marked, tile, 0, tiles);
+        arrived();
+        __syncthreads();                          // the tile is there, and nobody reads the other buffer any more
+        if (next < tiles) fetch(next, buf ^ 1);
         const bool masked = key0 + kBK > open || (marked && !full_tile(marks, tile));
+        const char *kc = kt[buf], *vc = vt[buf];
         f32x16 s[2], unused;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             s[n] = zero16();
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) s[n] = Mma<T>::mul(L::row_frag(kt, 32 * n, c), qf[c], s[n]);
+            for (int c = 0; c < DP / 16; ++c) s[n] = Mma<T>::mul(L::row_frag(kc, 32 * n, c), qf[c], s[n]);
         }
         float top = -INFINITY;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            scores<T, false>(s[n], sh, slope2, d.slopes != nullptr, sc, q, al, key0, n, masked, unused, unused);
+            scores<T, false>(s[n], sh, slope2, d.slopes != nullptr, sc, q, al[buf], key0, n, masked, unused, unused);
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = fmaxf(top, s[n][r]);
         }
@@ -790,9 +812,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(AttnAr
 #pragma unroll
             for (int k = 0; k < 2; ++k)
 #pragma unroll
-                for (int db = 0; db < DP / 32; ++db) o[db] = Mma<T>::mul(L::col_frag(vt, 32 * n + 16 * k, db), p[k], o[db]);
+                for (int db = 0; db < DP / 32; ++db) o[db] = Mma<T>::mul(L::col_frag(vc, 32 * n + 16 * k, db), p[k], o[db]);
         }
+        if (next < tiles) as.store(al[buf ^ 1], t);
         tile = next;
+        buf ^= 1;
     }
     l = halves_sum(l);
     const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -1045,8 +1069,8 @@ constexpr float kUp<f16> = 64.f;
 template <typename T, int DP>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(AttnArgs a) {
     using L = Tile<T, DP>;
-    __shared__ __attribute__((aligned(256))) char kt[kBK * L::kRowBytes], vt[kBK * L::kRowBytes];
-    __shared__ Along al;
+    __shared__ __attribute__((aligned(256))) char kt[2][kBK * L::kRowBytes], vt[2][kBK * L::kRowBytes];
+    __shared__ Along al[2];
     __shared__ Marks marks;
     __shared__ float scratch[4][2][DP];
     const wst_attention_desc& d = a.d;
@@ -1096,52 +1120,54 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(AttnArg
     f32x16 dq[DP / 32];
 #pragma unroll
     for (int k = 0; k < DP / 32; ++k) dq[k] = zero16();
-    float share = 0.f;
+    // -sum ds far = -(sum p dp far - (sum p dp) (sum p far)): from delta as the row itself gives it, in 32 bits, since
+    // delta out of the rounded output would be multiplied by a mean distance
+    float pdf = 0.f, pd = 0.f, pf = 0.f;
 
     const T *kb = at<T>(d.k, d.k_strides, b, 0, kvh), *vb = at<T>(d.v, d.v_strides, b, 0, kvh);
-    Stage<T, DP, kBK, 256> ks, vs;
     AlongStage as;
+    auto fetch = [&](int64_t n, int buf) {
+        Fetch<T, DP, kBK, 256>::issue(kb, d.k_strides[1], n * kBK, sc.length, sc.k_doc, d.dim, kt[buf], t);
+        Fetch<T, DP, kBK, 256>::issue(vb, d.v_strides[1], n * kBK, sc.length, sc.k_doc, d.dim, vt[buf], t);
+        as.load(sc.k_pos, sc.k_doc, sc.axes, n * kBK, sc.length, t);
+    };
     int64_t tile = next_tile(marks, marked, -1, 0, tiles);
+    int buf = 0;
     if (tile < tiles) {
-        ks.load(kb, d.k_strides[1], tile * kBK, sc.length, sc.k_doc, d.dim, t);
-        vs.load(vb, d.v_strides[1], tile * kBK, sc.length, sc.k_doc, d.dim, t);
-        as.load(sc.k_pos, sc.k_doc, sc.axes, tile * kBK, sc.length, t);
+        fetch(tile, 0);
+        as.store(al[0], t);
     }
     while (tile < tiles) {
-        const int64_t key0 = tile * kBK;
+        const int64_t key0 = tile * kBK, next = next_tile(marks, marked, tile, 0, tiles);
+        arrived();
         __syncthreads();
-        ks.store(kt, t);
-        vs.store(vt, t);
-        as.store(al, t);
-        __syncthreads();
-        const int64_t next = next_tile(marks, marked, tile, 0, tiles);
-        if (next < tiles) {
-            ks.load(kb, d.k_strides[1], next * kBK, sc.length, sc.k_doc, d.dim, t);
-            vs.load(vb, d.v_strides[1], next * kBK, sc.length, sc.k_doc, d.dim, t);
-            as.load(sc.k_pos, sc.k_doc, sc.axes, next * kBK, sc.length, t);
-        }
+        if (next < tiles) fetch(next, buf ^ 1);
         const bool masked = key0 + kBK > open || (marked && !full_tile(marks, tile));
+        const char *kc = kt[buf], *vc = vt[buf];
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             f32x16 s = zero16(), dp = zero16(), grad, far;
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) s = Mma<T>::mul(L::row_frag(kt, 32 * n, c), qf[c], s);
+            for (int c = 0; c < DP / 16; ++c) s = Mma<T>::mul(L::row_frag(kc, 32 * n, c), qf[c], s);
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) dp = Mma<T>::mul(L::row_frag(vt, 32 * n, c), df[c], dp);
-            scores<T, true>(s, sh, slope2, d.slopes != nullptr, sc, q, al, key0, n, masked, grad, far);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float p = __builtin_amdgcn_exp2f(s[r] - lse2);
-                dp[r] = p * (dp[r] - delta);
-            }
-            if (masked) {     // a weight of 0 may have met a value that is not finite
+            for (int c = 0; c < DP / 16; ++c) dp = Mma<T>::mul(L::row_frag(vc, 32 * n, c), df[c], dp);
+            scores<T, true>(s, sh, slope2, d.slopes != nullptr, sc, q, al[buf], key0, n, masked, grad, far);
+            if (masked) {     // a weight of 0 may meet a value that is not finite
 #pragma unroll
                 for (int r = 0; r < 16; ++r) dp[r] = s[r] == -INFINITY ? 0.f : dp[r];
             }
-            if (d.slopes) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) share -= dp[r] * far[r];
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] - lse2);
+            if (a.slope_part) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    pf += s[r] * far[r];
+                    pd += s[r] * dp[r];
+                    pdf += s[r] * dp[r] * far[r];
+                }
             }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dp[r] = s[r] * (dp[r] - delta);
             if (sh.cap) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) dp[r] *= grad[r];
@@ -1155,9 +1181,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(AttnArg
 #pragma unroll
             for (int k = 0; k < 2; ++k)
 #pragma unroll
-                for (int db = 0; db < DP / 32; ++db) dq[db] = Mma<T>::mul(L::col_frag(kt, 32 * n + 16 * k, db), z[k], dq[db]);
+                for (int db = 0; db < DP / 32; ++db) dq[db] = Mma<T>::mul(L::col_frag(kc, 32 * n + 16 * k, db), z[k], dq[db]);
         }
+        if (next < tiles) as.store(al[buf ^ 1], t);
         tile = next;
+        buf ^= 1;
     }
     const float mul = d.scale / kUp<T>;
     if (ok && a.g.dq) {
@@ -1172,7 +1200,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(AttnArg
             }
     }
     if (a.slope_part) {
-        const float sum = wave_sum(share);
+        const float share = halves_sum(pd) * halves_sum(pf) - halves_sum(pdf), sum = wave_sum(hl ? 0.f : share);
         if (lane == 0) a.slope_part[(static_cast<int64_t>(h) * d.batch + b) * a.slots + qt * 4 + w] = sum;
     }
     uint64_t bad = __ballot(ok && not_finite<T, DP>(dq));      // see k_attn_fwd
@@ -1197,8 +1225,8 @@ template <typename T, int DP>
 __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64) ? 2 : 1) void k_attn_dkv(AttnArgs a) {
     using L = Tile<T, DP>;
     constexpr int kRows = 64;
-    __shared__ __attribute__((aligned(256))) char qt[kRows * L::kRowBytes], dt[kRows * L::kRowBytes];
-    __shared__ Rows rw;
+    __shared__ __attribute__((aligned(256))) char qt[2][kRows * L::kRowBytes], dt[2][kRows * L::kRowBytes];
+    __shared__ Rows rows[2];
     __shared__ Marks marks;
     __shared__ float scratch[4][2][DP];
     const wst_attention_desc& d = a.d;
@@ -1232,15 +1260,14 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64) ? 2 : 1) void k_a
         scan_documents(marks, sc.k_doc, j0, kBQ, sc.length, sc.q_doc, tile0, tiles, d.q_len);
         __syncthreads();
     }
-    Stage<T, DP, kRows, 256> qs, ds;
     float r_lse = 0.f, r_delta = 0.f, r_place = 0.f;
     int r_limit = 0, r_doc = -1;
     uint32_t r_pos = 0;
     int g = 0;
-    auto fetch = [&](int64_t tile) {
+    auto fetch = [&](int64_t tile, int buf) {
         const int h = kvh * group + g;
-        qs.load(at<T>(d.q, d.q_strides, b, 0, h), d.q_strides[1], tile * kRows, d.q_len, sc.q_doc, d.dim, t);
-        ds.load(at<T>(a.g.d_o, a.g.do_strides, b, 0, h), a.g.do_strides[1], tile * kRows, d.q_len, sc.q_doc, d.dim, t);
+        Fetch<T, DP, kRows, 256>::issue(at<T>(d.q, d.q_strides, b, 0, h), d.q_strides[1], tile * kRows, d.q_len, sc.q_doc, d.dim, qt[buf], t);
+        Fetch<T, DP, kRows, 256>::issue(at<T>(a.g.d_o, a.g.do_strides, b, 0, h), a.g.do_strides[1], tile * kRows, d.q_len, sc.q_doc, d.dim, dt[buf], t);
         const int64_t i = tile * kRows + (t & 63), row = (b * d.q_heads + h) * d.q_len + i;
         const bool in = i < d.q_len;
         if (t < 64) {
@@ -1273,13 +1300,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64) ? 2 : 1) void k_a
     } else {
         tile = tiles;
     }
-    if (tile < tiles) fetch(tile);
-    while (tile < tiles) {
-        const int64_t row0 = tile * kRows;
-        const float slope2 = d.slopes ? d.slopes[kvh * group + g] * kLog2e : 0.f;
-        __syncthreads();
-        qs.store(qt, t);
-        ds.store(dt, t);
+    auto put = [&](Rows& rw) {
         if (t < 64) {
             rw.lse2[t] = r_lse;
             rw.delta[t] = r_delta;
@@ -1288,6 +1309,18 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64) ? 2 : 1) void k_a
             rw.place[t] = r_place;
         }
         rw.pos[t >> 6][t & 63] = r_pos;
+    };
+    int buf = 0;
+    if (tile < tiles) {
+        fetch(tile, 0);
+        put(rows[0]);
+    }
+    while (tile < tiles) {
+        const int64_t row0 = tile * kRows;
+        const float slope2 = d.slopes ? d.slopes[kvh * group + g] * kLog2e : 0.f;
+        const Rows& rw = rows[buf];
+        const char *qc = qt[buf], *dc = dt[buf];
+        arrived();
         __syncthreads();
         // in order for every pair: the tile's first query sees the block's last key, and all rows and keys exist
         bool masked = row0 + kRows > d.q_len || keys < kBQ || (marked && !full_tile(marks, tile - tile0));
@@ -1296,14 +1329,14 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64) ? 2 : 1) void k_a
             masked = masked || lim < j0 + kBQ;
         }
         skip(a.parts);
-        if (tile < tiles) fetch(tile);
+        if (tile < tiles) fetch(tile, buf ^ 1);
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             f32x16 s = zero16(), dp = zero16(), grad;
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) s = Mma<T>::mul(L::row_frag(qt, 32 * n, c), kf[c], s);
+            for (int c = 0; c < DP / 16; ++c) s = Mma<T>::mul(L::row_frag(qc, 32 * n, c), kf[c], s);
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) dp = Mma<T>::mul(L::row_frag(dt, 32 * n, c), vf[c], dp);
+            for (int c = 0; c < DP / 16; ++c) dp = Mma<T>::mul(L::row_frag(dc, 32 * n, c), vf[c], dp);
             if (sh.cap) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
@@ -1370,10 +1403,12 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64) ? 2 : 1) void k_a
             for (int k = 0; k < 2; ++k)
 #pragma unroll
                 for (int db = 0; db < DP / 32; ++db) {
-                    dv[db] = Mma<T>::mul(L::col_frag(dt, 32 * n + 16 * k, db), p[k], dv[db]);
-                    dk[db] = Mma<T>::mul(L::col_frag(qt, 32 * n + 16 * k, db), z[k], dk[db]);
+                    dv[db] = Mma<T>::mul(L::col_frag(dc, 32 * n + 16 * k, db), p[k], dv[db]);
+                    dk[db] = Mma<T>::mul(L::col_frag(qc, 32 * n + 16 * k, db), z[k], dk[db]);
                 }
         }
+        if (tile < tiles) put(rows[buf ^ 1]);
+        buf ^= 1;
     }
     const float up = 1.f / kUp<T>, mul = d.scale * up;
     if (a.parts > 1) {
@@ -1492,15 +1527,25 @@ size_t rows_of(const wst_attention_desc& d) { return static_cast<size_t>(d.batch
 
 // How a call runs.
 struct Plan {
-    bool tiles;                 // matrix instructions; else a row at a time (heads of other widths)
+    bool tiles;                 // matrix instructions; else a row at a time (heads of other widths, rows not lined up to 16 bytes)
     int splits;                 // forward: 0 = k_attn_fwd, else blocks along the keys of k_attn_split
     int parts, slots;           // backward: parts of dk and dv; partial slope sums of a head and sequence
     size_t forward, backward;   // workspace, in floats
 };
 
-Plan plan_of(const wst_attention_desc& d) {
+// Rows that can be fetched 16 bytes at a time.
+bool lined_up(const wst_attention_desc& d, const void* p, const int64_t (&s)[3]) {
+    const int64_t size = d.dtype == WST_F32 ? 4 : 2;
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && s[0] * size % 16 == 0 && s[1] * size % 16 == 0 && s[2] * size % 16 == 0;
+}
+
+bool can_tile(const wst_attention_desc& d) {
+    return d.dim % 8 == 0 && d.dim <= 128 && lined_up(d, d.q, d.q_strides) && lined_up(d, d.k, d.k_strides) && lined_up(d, d.v, d.v_strides);
+}
+
+Plan plan_of(const wst_attention_desc& d, bool tiles) {
     Plan p{};
-    p.tiles = d.dim % 8 == 0 && d.dim <= 128;
+    p.tiles = tiles;
     const int64_t rows = static_cast<int64_t>(rows_of(d)), group = d.q_heads / d.k_heads;
     p.slots = static_cast<int>(d.q_len);
     p.parts = 1;
@@ -1526,8 +1571,10 @@ Plan plan_of(const wst_attention_desc& d) {
 }
 
 size_t bytes_of(const wst_attention_desc& d, int backward) {
-    const Plan p = plan_of(d);
-    return sizeof(float) * (backward ? p.backward : p.forward);
+    // either way of running: the gradient of the output, which decides with the rest, is not known here
+    const Plan p = plan_of(d, true), q = plan_of(d, false);
+    const size_t b = p.backward > q.backward ? p.backward : q.backward;
+    return sizeof(float) * (backward ? b : p.forward);
 }
 
 template <typename F>
@@ -1557,7 +1604,7 @@ int wst_attention_forward(const wst_attention_desc* d, void* o, float* lse, void
     const size_t need = bytes_of(*d, 0);
     if (need && (!workspace || workspace_bytes < need)) return fail(WST_ERR_INVALID, "attention: workspace too small");
     AttnArgs a{};
-    const Plan p = plan_of(*d);
+    const Plan p = plan_of(*d, can_tile(*d));
     a.d = *d;
     a.o = o;
     a.lse = lse;
@@ -1598,7 +1645,7 @@ int wst_attention_backward(const wst_attention_desc* d, const wst_attention_grad
     AttnArgs a{};
     a.d = *d;
     a.g = *g;
-    const Plan p = plan_of(*d);
+    const Plan p = plan_of(*d, can_tile(*d) && lined_up(*d, g->d_o, g->do_strides));
     a.delta = static_cast<float*>(workspace);
     a.slots = p.slots;
     a.parts = p.parts;

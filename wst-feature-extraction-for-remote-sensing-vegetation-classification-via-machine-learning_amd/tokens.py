@@ -195,6 +195,21 @@ def _strides(t):
     return t.stride()[:3]
 
 
+def _lined_up(t):
+    """t with rows the library can fetch 16 bytes at a time (heads of other widths go value by value anyway)."""
+    t = _rows_of(t)
+    if t.shape[-1] % 8 == 0:
+        size = t.element_size()
+        if t.data_ptr() % 16 or any(s * size % 16 for s, n in zip(t.stride()[:3], t.shape) if n > 1):
+            return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _call_strides(t):
+    """The strides of t for a call; of an axis of one entry, which is never stepped along, 0."""
+    return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape))
+
+
 def _rotate(q, k, positions, sections, base, interleaved, inverse):
     q = _rows_of(q)
     B, T, H, D = q.shape
@@ -279,7 +294,7 @@ def _attention_desc(q, k, v, slopes, side, o):
         return 0 if t is None or t.dim() < dims else t.stride(0)
 
     return _lib.AttentionDesc(
-        B, Tq, k.shape[1], _strides(q), _strides(k), _strides(v), _strides(o), per_batch(side.q_pos, 3),
+        B, Tq, k.shape[1], _call_strides(q), _call_strides(k), _call_strides(v), _call_strides(o), per_batch(side.q_pos, 3),
         per_batch(side.k_pos, 3), per_batch(side.q_doc, 2), per_batch(side.k_doc, 2), q.data_ptr(), k.data_ptr(),
         v.data_ptr(), _ptr(slopes), _ptr(side.q_pos), _ptr(side.k_pos), _ptr(side.q_doc), _ptr(side.k_doc),
         _ptr(side.k_lengths), _ptr(side.prefix), side.scale, side.cap, H, k.shape[2], D, DTYPES[q.dtype],
@@ -321,11 +336,11 @@ class _Attention(torch.autograd.Function):
         dslopes = torch.empty_like(slopes) if want[3] else None
         if not q.numel() or not k.numel():
             return tuple(None if t is None else t.zero_() for t in (dq, dk, dv, dslopes)) + (None,)
-        do = _rows_of(do)
+        do = _lined_up(do)
         d = _attention_desc(q, k, v, slopes, ctx.side, o)
         none = (0, 0, 0)
         g = _lib.AttentionGrads(o.data_ptr(), do.data_ptr(), lse.data_ptr(), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dslopes),
-                                _strides(do), *(none if t is None else _strides(t) for t in (dq, dk, dv)))
+                                _call_strides(do), *(none if t is None else _strides(t) for t in (dq, dk, dv)))
         ws, size = _workspace(d, 1, q.device)
         _call(q.device, _lib.load().wst_attention_backward, d, g, _ptr(ws), size)
         return dq, dk, dv, dslopes, None
@@ -402,7 +417,7 @@ def attention(q, k, v, *, scale=None, cap=0.0, slopes=None, q_positions=None, k_
         raise RuntimeError("cap must be finite and not negative")
     if not abs(s.scale) < float("inf"):
         raise RuntimeError("scale must be finite")
-    q, k, v = _rows_of(q), _rows_of(k), _rows_of(v)
+    q, k, v = _lined_up(q), _lined_up(k), _lined_up(v)
     if _wants_grad(q, k, v, slopes):
         o, lse = _Attention.apply(q, k, v, slopes, s)
     else:
