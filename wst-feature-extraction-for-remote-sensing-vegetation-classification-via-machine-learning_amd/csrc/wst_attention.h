@@ -1,0 +1,1610 @@
+// Attention on coefficient tokens, with scores capped by tanh, a bias that depends on distance, documents, order and a
+// prefix (C ABI and formulas: include/wst_hip.h, "Token operators").
+//
+//   z = scale q.k;  z = cap tanh(z / cap);  s = z - slope * distance;  p = softmax(s over the keys seen);  o = p v
+//   backward, with delta_i = sum_d do_id o_id:  dv = p^T do;  dp = do v^T;  ds = p (dp - delta);
+//   dslope = -sum ds distance;  dz = ds (1 - (z / cap)^2) scale;  dq = dz k;  dk = dz^T q
+//
+// Kernels as templates over the element type; wst_attention_t.hip instantiates one type, wst_attention.hip checks the
+// arguments and chooses.
+#ifndef WST_ATTENTION_H
+#define WST_ATTENTION_H
+
+#include <type_traits>
+
+#include "wst_tokens.h"
+
+namespace wst_tok {
+
+// How a call runs.
+struct AttnPlan {
+    bool tiles;                 // matrix instructions; else a row at a time (other widths, rows not lined up to 16 bytes)
+    int splits;                 // forward: 0 = k_attn_fwd, else blocks along the keys of k_attn_split
+    int parts, slots;           // backward: parts of dk and dv; partial slope sums of a head and sequence
+    size_t forward, backward;   // workspace, in floats
+};
+
+struct AttnArgs {
+    wst_attention_desc d;
+    wst_attention_grads g;
+    void* o;
+    float* lse;
+    float* delta;        // (batch, heads, q_len)
+    float* slope_part;   // (heads, batch, slots)
+    float *part, *part_ml;   // forward: (splits, rows, dim) and (splits, rows, 2); backward: (parts, keys, 2, dim)
+    int slots, splits, parts;
+};
+
+// What one batch entry's keys and queries may see.
+struct Scope {
+    int length, shift, prefix;   // keys that exist; place(i) = i + shift; keys below prefix are seen out of order
+    const int32_t *q_doc, *k_doc, *q_pos, *k_pos;
+    bool causal;
+    int axes;
+
+    __device__ __forceinline__ Scope(const wst_attention_desc& d, int64_t b) {
+        length = static_cast<int>(d.k_len);
+        if (d.k_lengths) {
+            const int l = d.k_lengths[b];
+            length = l < 0 ? 0 : l < length ? l : length;
+        }
+        shift = length - static_cast<int>(d.q_len);
+        prefix = d.prefix ? d.prefix[b] : 0;
+        prefix = prefix < 0 ? 0 : prefix < length ? prefix : length;
+        causal = d.causal != 0;
+        axes = d.axes;
+        q_doc = d.q_doc ? d.q_doc + b * d.q_doc_stride : nullptr;
+        k_doc = d.k_doc ? d.k_doc + b * d.k_doc_stride : nullptr;
+        q_pos = d.q_pos ? d.q_pos + b * d.q_pos_stride : nullptr;
+        k_pos = d.k_pos ? d.k_pos + b * d.k_pos_stride : nullptr;
+    }
+    __device__ __forceinline__ bool seen(int i, int j) const {
+        if (j >= length) return false;
+        if (causal && j > i + shift && j >= prefix) return false;
+        if (q_doc) {
+            const int32_t x = q_doc[i];
+            return x >= 0 && x == k_doc[j];
+        }
+        return true;
+    }
+    // first key that query i does not see in order
+    __device__ __forceinline__ int limit(int i) const {
+        if (!causal) return length;
+        const int e = i + shift + 1 > prefix ? i + shift + 1 : prefix;
+        return e < length ? e : length;
+    }
+    __device__ __forceinline__ float distance(int i, int j) const {
+        if (!q_pos) return static_cast<float>(i + shift > j ? i + shift - j : j - i - shift);
+        float s = 0.f;
+        for (int a = 0; a < axes; ++a) {
+            const int64_t x = static_cast<int64_t>(q_pos[static_cast<int64_t>(i) * axes + a]) - k_pos[static_cast<int64_t>(j) * axes + a];
+            s += static_cast<float>(x < 0 ? -x : x);
+        }
+        return s;
+    }
+};
+
+constexpr int kD = WST_MAX_HEAD_DIM, kPer = kD / 64;   // values of a row a lane holds: d = lane + 64 c
+
+template <typename T>
+__device__ __forceinline__ const T* at(const void* p, const int64_t (&s)[3], int64_t b, int64_t t, int h) {
+    return static_cast<const T*>(p) + b * s[0] + t * s[1] + h * s[2];
+}
+
+// dot of a row in LDS with a row in memory
+template <typename T>
+__device__ __forceinline__ float dot_row(const float* a, const T* b, int dim) {
+    float s = 0.f;
+    int d = 0;
+    for (; d + 8 <= dim; d += 8) {
+        float v[8];
+        load<8>(b + d, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += a[d + e] * v[e];
+    }
+    for (; d < dim; ++d) s += a[d] * static_cast<float>(b[d]);
+    return s;
+}
+
+// capped score before the bias, and the slope of the cap there
+__device__ __forceinline__ float capped(float z, float cap, float& grad) {
+    grad = 1.f;
+    if (cap > 0.f) {
+        const float t = tanhf(z / cap);
+        grad = 1.f - t * t;
+        z = cap * t;
+    }
+    return z;
+}
+
+// One query by one wave, a key a lane. q: the query's row in LDS (this wave's own).
+template <typename T>
+__device__ void row_forward(const AttnArgs& a, const Scope& sc, int64_t b, int h, int i, float* q) {
+    const wst_attention_desc& d = a.d;
+    const int lane = threadIdx.x & 63, kvh = h / (d.q_heads / d.k_heads);
+    const T* qr = at<T>(d.q, d.q_strides, b, i, h);
+    for (int x = lane; x < d.dim; x += 64) q[x] = static_cast<float>(qr[x]);
+    __builtin_amdgcn_wave_barrier();
+    const float slope = d.slopes ? d.slopes[h] : 0.f;
+    float m = -INFINITY, l = 0.f, acc[kPer] = {};
+    for (int j0 = 0; j0 < sc.length; j0 += 64) {
+        const int j = j0 + lane;
+        const bool see = sc.seen(i, j);
+        float s = -INFINITY, unused;
+        if (see) {
+            s = capped(dot_row(q, at<T>(d.k, d.k_strides, b, j, kvh), d.dim) * d.scale, d.cap, unused);
+            if (d.slopes) s -= slope * sc.distance(i, j);
+        }
+        const uint64_t who = __ballot(see);
+        if (!who) continue;
+        const float mn = fmaxf(m, wave_max(s)), base = mn == -INFINITY ? 0.f : mn;
+        const float p = see ? expf(s - base) : 0.f, f = expf(m - base);
+        l = l * f + wave_sum(p);
+        m = mn;
+#pragma unroll
+        for (int c = 0; c < kPer; ++c) acc[c] *= f;
+        for (uint64_t w = who; w; w &= w - 1) {
+            const int e = __builtin_ctzll(w);
+            const float pe = __shfl(p, e);
+            const T* v = at<T>(d.v, d.v_strides, b, j0 + e, kvh);
+#pragma unroll
+            for (int c = 0; c < kPer; ++c)
+                if (lane + 64 * c < d.dim) acc[c] += pe * static_cast<float>(v[lane + 64 * c]);
+        }
+    }
+    T* o = const_cast<T*>(at<T>(a.o, d.o_strides, b, i, h));
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int c = 0; c < kPer; ++c)
+        if (lane + 64 * c < d.dim) o[lane + 64 * c] = static_cast<T>(acc[c] * inv);
+    if (lane == 0 && a.lse) a.lse[(b * d.q_heads + h) * d.q_len + i] = l == 0.f ? -INFINITY : m + logf(l);
+}
+
+// The gradient of one query, and its share of -sum ds distance. LDS: q and do of the row.
+template <typename T>
+__device__ float row_dq(const AttnArgs& a, const Scope& sc, int64_t b, int h, int i, float* q, float* dout) {
+    const wst_attention_desc& d = a.d;
+    const int lane = threadIdx.x & 63, kvh = h / (d.q_heads / d.k_heads);
+    const T *qr = at<T>(d.q, d.q_strides, b, i, h), *dr = at<T>(a.g.d_o, a.g.do_strides, b, i, h);
+    for (int x = lane; x < d.dim; x += 64) {
+        q[x] = static_cast<float>(qr[x]);
+        dout[x] = static_cast<float>(dr[x]);
+    }
+    __builtin_amdgcn_wave_barrier();
+    const float slope = d.slopes ? d.slopes[h] : 0.f;
+    const int64_t row = (b * d.q_heads + h) * d.q_len + i;
+    const float lse = a.g.lse[row], delta = a.delta[row];
+    float acc[kPer] = {}, share = 0.f;
+    if (lse != -INFINITY)
+        for (int j0 = 0; j0 < sc.length; j0 += 64) {
+            const int j = j0 + lane;
+            const bool see = sc.seen(i, j);
+            float dz = 0.f;
+            if (see) {
+                float grad;
+                float s = capped(dot_row(q, at<T>(d.k, d.k_strides, b, j, kvh), d.dim) * d.scale, d.cap, grad);
+                const float far = d.slopes ? sc.distance(i, j) : 0.f;
+                s -= slope * far;
+                const float ds = expf(s - lse) * (dot_row(dout, at<T>(d.v, d.v_strides, b, j, kvh), d.dim) - delta);
+                share -= ds * far;
+                dz = ds * grad * d.scale;
+            }
+            for (uint64_t w = __ballot(see); w; w &= w - 1) {
+                const int e = __builtin_ctzll(w);
+                const float x = __shfl(dz, e);
+                const T* k = at<T>(d.k, d.k_strides, b, j0 + e, kvh);
+#pragma unroll
+                for (int c = 0; c < kPer; ++c)
+                    if (lane + 64 * c < d.dim) acc[c] += x * static_cast<float>(k[lane + 64 * c]);
+            }
+        }
+    if (a.g.dq) {
+        T* o = const_cast<T*>(at<T>(a.g.dq, a.g.dq_strides, b, i, h));
+#pragma unroll
+        for (int c = 0; c < kPer; ++c)
+            if (lane + 64 * c < d.dim) o[lane + 64 * c] = static_cast<T>(acc[c]);
+    }
+    return wave_sum(share);
+}
+
+// The gradients of one key and value, over all queries of the heads that share it. LDS: k and v of the row.
+template <typename T>
+__device__ void row_dkv(const AttnArgs& a, const Scope& sc, int64_t b, int kvh, int j, float* k, float* v) {
+    const wst_attention_desc& d = a.d;
+    const int lane = threadIdx.x & 63, group = d.q_heads / d.k_heads;
+    const T *kr = at<T>(d.k, d.k_strides, b, j, kvh), *vr = at<T>(d.v, d.v_strides, b, j, kvh);
+    for (int x = lane; x < d.dim; x += 64) {
+        k[x] = static_cast<float>(kr[x]);
+        v[x] = static_cast<float>(vr[x]);
+    }
+    __builtin_amdgcn_wave_barrier();
+    float dk[kPer] = {}, dv[kPer] = {};
+    for (int h = kvh * group; h < (kvh + 1) * group; ++h) {
+        const float slope = d.slopes ? d.slopes[h] : 0.f;
+        for (int i0 = 0; i0 < d.q_len; i0 += 64) {
+            const int i = i0 + lane;
+            const int64_t row = (b * d.q_heads + h) * d.q_len + i;
+            const bool see = i < d.q_len && sc.seen(i, j) && a.g.lse[row] != -INFINITY;
+            float p = 0.f, dz = 0.f;
+            if (see) {
+                float grad;
+                float s = capped(dot_row(k, at<T>(d.q, d.q_strides, b, i, h), d.dim) * d.scale, d.cap, grad);
+                if (d.slopes) s -= slope * sc.distance(i, j);
+                p = expf(s - a.g.lse[row]);
+                dz = p * (dot_row(v, at<T>(a.g.d_o, a.g.do_strides, b, i, h), d.dim) - a.delta[row]) * grad * d.scale;
+            }
+            for (uint64_t w = __ballot(see); w; w &= w - 1) {
+                const int e = __builtin_ctzll(w);
+                const float pe = __shfl(p, e), ze = __shfl(dz, e);
+                const T *q = at<T>(d.q, d.q_strides, b, i0 + e, h), *dr = at<T>(a.g.d_o, a.g.do_strides, b, i0 + e, h);
+#pragma unroll
+                for (int c = 0; c < kPer; ++c)
+                    if (lane + 64 * c < d.dim) {
+                        dk[c] += ze * static_cast<float>(q[lane + 64 * c]);
+                        dv[c] += pe * static_cast<float>(dr[lane + 64 * c]);
+                    }
+            }
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < kPer; ++c)
+        if (lane + 64 * c < d.dim) {
+            if (a.g.dk) const_cast<T*>(at<T>(a.g.dk, a.g.dk_strides, b, j, kvh))[lane + 64 * c] = static_cast<T>(dk[c]);
+            if (a.g.dv) const_cast<T*>(at<T>(a.g.dv, a.g.dv_strides, b, j, kvh))[lane + 64 * c] = static_cast<T>(dv[c]);
+        }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a) {
+    __shared__ float q[4][kD];
+    const int w = threadIdx.x >> 6, h = blockIdx.y;
+    const int i = static_cast<int>(blockIdx.x) * 4 + w;
+    const int64_t b = blockIdx.z;
+    if (i >= a.d.q_len) return;
+    row_forward<T>(a, Scope(a.d, b), b, h, i, q[w]);
+}
+
+// delta_i = sum_d do_id o_id, a wave a row
+template <typename T>
+__global__ __launch_bounds__(256) void k_attn_delta(AttnArgs a) {
+    const wst_attention_desc& d = a.d;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6), b = blockIdx.z;
+    const int h = blockIdx.y, lane = threadIdx.x & 63;
+    if (i >= d.q_len) return;
+    const T *o = at<T>(a.g.o, d.o_strides, b, i, h), *dr = at<T>(a.g.d_o, a.g.do_strides, b, i, h);
+    float s = 0.f;
+    for (int x = lane; x < d.dim; x += 64) s += static_cast<float>(o[x]) * static_cast<float>(dr[x]);
+    s = wave_sum(s);
+    if (lane == 0) a.delta[(b * d.q_heads + h) * d.q_len + i] = s;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_attn_dq_rows(AttnArgs a) {
+    __shared__ float q[4][kD], dout[4][kD];
+    const int w = threadIdx.x >> 6, h = blockIdx.y;
+    const int i = static_cast<int>(blockIdx.x) * 4 + w;
+    const int64_t b = blockIdx.z;
+    if (i >= a.d.q_len) return;
+    const float share = row_dq<T>(a, Scope(a.d, b), b, h, i, q[w], dout[w]);
+    if (a.slope_part && (threadIdx.x & 63) == 0)
+        a.slope_part[(static_cast<int64_t>(h) * a.d.batch + b) * a.slots + i] = share;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_attn_dkv_rows(AttnArgs a) {
+    __shared__ float k[4][kD], v[4][kD];
+    const int w = threadIdx.x >> 6;
+    const int j = static_cast<int>(blockIdx.x) * 4 + w;
+    const int64_t b = blockIdx.z;
+    if (j >= a.d.k_len) return;
+    row_dkv<T>(a, Scope(a.d, b), b, blockIdx.y, j, k[w], v[w]);
+}
+
+// ------------------------------------------------------------------------------------------ matrix instructions
+// Heads of a multiple of 8 values up to 128 go through 32x32 matrix instructions, padded to DP = 32, 64, 96 or 128.
+//
+// Operand layout (16-bit: 32x32x16, eight values a lane; float32: 32x32x2, one value a lane): with h = lane / 32, an
+// operand fragment holds, of row or column lane % 32, the eight inner indices 8 h .. 8 h + 7 of a step of 16. For float32
+// the eight values feed eight instructions, one each; which inner index meets which instruction does not matter as long
+// as both operands agree. The result holds column lane % 32 and rows 8 (r / 4) + 4 h + r % 4 for r = 0 .. 15.
+//
+// So a tile of scores taken as (keys x queries) has one query a lane: the softmax's maximum and sum are in-lane but for
+// one exchange between the halves, and its sixteen registers are, rounded, the next product's operand for the keys
+// 16 s + 8 (e / 4) + 4 h + e % 4 (step s, element e): the other operand reads the same keys in that order, so no score
+// ever moves between lanes.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <typename T>
+struct Mma;
+template <>
+struct Mma<bf16> {
+    typedef bf16 Frag __attribute__((ext_vector_type(8)));
+    typedef bf16 Quad __attribute__((ext_vector_type(4)));
+    static __device__ __forceinline__ f32x16 mul(Frag a, Frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Mma<f16> {
+    typedef f16 Frag __attribute__((ext_vector_type(8)));
+    typedef f16 Quad __attribute__((ext_vector_type(4)));
+    static __device__ __forceinline__ f32x16 mul(Frag a, Frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Mma<float> {
+    typedef float Frag __attribute__((ext_vector_type(8)));
+    typedef float Quad __attribute__((ext_vector_type(4)));
+    static __device__ __forceinline__ f32x16 mul(Frag a, Frag b, f32x16 c) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+        return c;
+    }
+};
+template <typename T>
+using Frag = typename Mma<T>::Frag;
+template <typename T>
+using Quad = typename Mma<T>::Quad;
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+#define WST_LDS __attribute__((address_space(3)))
+
+__device__ __forceinline__ f32x16 zero16() {
+    f32x16 z;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z[r] = 0.f;
+    return z;
+}
+
+// max / sum with the lane 32 away
+__device__ __forceinline__ float halves_max(float x) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float halves_sum(float x) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Rows of DP values in LDS, in units of 16 bytes. Unit u of a row lies at u ^ swizzle(row): reading 16 rows at one unit
+// (row_frag) and 4 rows at 4 units (col_frag) both then touch every bank once. The swizzle depends on row % 16 alone, so
+// a lane's is the same for all its rows.
+template <typename T, int DP>
+struct Tile {
+    static constexpr int kElems = 16 / sizeof(T), kUnits = DP / kElems, kRowBytes = DP * sizeof(T);
+    static __device__ __forceinline__ int swizzle(int row) {
+        if constexpr (kUnits % 16 == 0) return ((row & 3) << 2) | ((row >> 2) & 3);        // a row spans all banks
+        else if constexpr (kUnits % 8 == 0) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);   // two rows do
+        else return (row >> 2) & 3;                                                        // four rows do
+    }
+    static __device__ __forceinline__ int at(int row, int unit) { return row * kRowBytes + ((unit ^ swizzle(row)) << 4); }
+
+    // row row0 + lane % 32, values 16 c + 8 (lane / 32) .. + 7; row0 a multiple of 16
+    static __device__ __forceinline__ Frag<T> row_frag(const char* t, int row0, int c) {
+        const int lane = threadIdx.x & 63, row = lane & 31, h = lane >> 5;
+        Frag<T> f;
+        if constexpr (sizeof(T) == 2) {
+            f = *reinterpret_cast<const Frag<T>*>(t + row0 * kRowBytes + at(row, 2 * c + h));
+        } else {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(t + row0 * kRowBytes + at(row, 4 * c + 2 * h));
+            const f32x4 b = *reinterpret_cast<const f32x4*>(t + row0 * kRowBytes + at(row, 4 * c + 2 * h + 1));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                f[e] = a[e];
+                f[4 + e] = b[e];
+            }
+        }
+        return f;
+    }
+    // value 32 db + lane % 32 of the eight rows row0 + 8 (e / 4) + 4 (lane / 32) + e % 4; row0 a multiple of 16
+    static __device__ __forceinline__ Frag<T> col_frag(const char* t, int row0, int db) {
+        const int lane = threadIdx.x & 63;
+        Frag<T> f;
+        if constexpr (sizeof(T) == 2) {
+            // the transposing read: sixteen lanes hand in four rows of sixteen values and get a column of four each
+            const int g = lane >> 4, x = lane & 15, row = 4 * (g >> 1) + (x >> 2), unit = 4 * db + 2 * (g & 1) + ((x & 3) >> 1);
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            union {
+                s16x4 q[2];
+                Frag<T> f;
+            } u;
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                u.q[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (WST_LDS s16x4*)(t + row0 * kRowBytes + at(8 * k + row, unit) + 8 * (x & 1)));
+            f = u.f;
+        } else {
+            const int d = 32 * db + (lane & 31), h = lane >> 5;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                f[e] = *reinterpret_cast<const float*>(t + row0 * kRowBytes + at(8 * (e >> 2) + 4 * h + (e & 3), d >> 2) + 4 * (d & 3));
+        }
+        return f;
+    }
+};
+
+// N rows of a tensor on their way to LDS: loaded into registers early, stored when the tile is free. A thread of TH takes
+// units t, t + TH, ...; rows that do not exist or belong to no document, and values beyond the head, become zero.
+template <typename T, int DP, int N, int TH>
+struct Stage {
+    using L = Tile<T, DP>;
+    static constexpr int kCount = (N * L::kUnits + TH - 1) / TH;
+    u32x4 v[kCount];
+
+    __device__ __forceinline__ void load(const T* base, int64_t stride, int64_t row0, int64_t rows, const int32_t* doc, int dim, int t) {
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) {
+            const int id = t + i * TH, row = id / L::kUnits, unit = id % L::kUnits;
+            bool ok = (N * L::kUnits % TH == 0 || row < N) && row0 + row < rows && unit * L::kElems < dim;
+            if (doc) ok = ok && doc[row0 + (row0 + row < rows ? row : 0)] >= 0;
+            v[i] = u32x4{0, 0, 0, 0};
+            if (ok) __builtin_memcpy(&v[i], base + (row0 + row) * stride + unit * L::kElems, 16);
+        }
+    }
+    __device__ __forceinline__ void store(char* tile, int t) const {
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) {
+            const int id = t + i * TH, row = id / L::kUnits, unit = id % L::kUnits;
+            if (N * L::kUnits % TH == 0 || row < N) *reinterpret_cast<u32x4*>(tile + L::at(row, unit)) = v[i];
+        }
+    }
+};
+
+// N rows of a tensor straight into LDS, past the registers, by 256 threads: each lane names the 16 bytes it wants, and a
+// wave's land one after the other, so the swizzle is in the choice of the source. A lane's offsets from the tile's first
+// row are the same for every tile; what moves is the scalar base. Lanes whose row does not exist or belongs to no
+// document, and those beyond the head's width, fetch nothing and leave what is there: zeros at first (clear()), later
+// perhaps an earlier tile's row, which the mask keeps out like any other. The compiler does not know of these loads:
+// arrived() waits for them.
+template <typename T, int DP, int N>
+struct Fetch {
+    using L = Tile<T, DP>;
+    static constexpr int kCount = N * L::kUnits / 256;
+    static_assert(N * L::kUnits % 256 == 0, "whole waves");
+    static constexpr int kStep = 256 / L::kUnits;                                     // rows from one count to the next
+    static constexpr bool kSame = 256 % L::kUnits == 0 && kStep % 16 == 0;            // the same unit and swizzle in each
+    static constexpr int kOff = kSame ? 1 : kCount;
+    uint32_t off[kOff], live;
+
+    __device__ __forceinline__ void init(int64_t stride, int dim, int t) {
+        live = 0;
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) {
+            const int id = t + i * 256, row = id / L::kUnits, unit = (id % L::kUnits) ^ L::swizzle(row);
+            if (i < kOff) off[i] = static_cast<uint32_t>(row * stride * sizeof(T)) + unit * 16;
+            live |= static_cast<uint32_t>(unit * L::kElems < dim) << i;
+        }
+    }
+    // base: the tile's first row; left: rows that exist from there on; doc: the rows' documents in LDS, or nullptr
+    __device__ __forceinline__ void issue(const T* base, int64_t stride, int left, const int* doc, int dim, const char* tile, int t) const {
+        const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((WST_LDS const char*)tile)) + (t & ~63) * 16;
+        if (left >= N && !doc && dim == DP) {
+#pragma unroll
+            for (int i = 0; i < kCount; ++i) load(base, stride, i, lds);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kCount; ++i) {
+                const int row = (t + i * 256) / L::kUnits;
+                if ((live >> i & 1) && row < left && (!doc || doc[row] >= 0)) load(base, stride, i, lds);
+            }
+        }
+    }
+    __device__ __forceinline__ void load(const T* base, int64_t stride, int i, uint32_t lds) const {
+        const T* b = kSame ? base + i * kStep * stride : base;
+        const uint32_t dst = __builtin_amdgcn_readfirstlane(lds + i * 4096);
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(dst), "v"(off[kSame ? 0 : i]), "s"(b) : "memory", "m0");
+    }
+};
+__device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+
+template <int BYTES>
+__device__ __forceinline__ void clear(char* p, int t) {
+    for (int i = t * 16; i < BYTES; i += 4096) *reinterpret_cast<u32x4*>(p + i) = u32x4{0, 0, 0, 0};
+}
+
+// Eight values of a row as an operand fragment, from memory; zero beyond the head or where the row is not to be read.
+template <typename T, int DP>
+__device__ __forceinline__ void row_frags(const T* row, bool ok, int dim, Frag<T> (&f)[DP / 16]) {
+    const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+        if (ok && 16 * c + 8 * h < dim) {
+            __builtin_memcpy(&f[c], row + 16 * c + 8 * h, sizeof(Frag<T>));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[c][e] = static_cast<T>(0.f);
+        }
+    }
+}
+template <typename T, int DP>
+__device__ __forceinline__ void negate(Frag<T> (&f)[DP / 16]) {
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) f[c] = -f[c];
+}
+
+// Sixteen result registers as the operands of two steps of the next product, rounded to the inputs' type: the products
+// of weights are the one place where attention rounds before its end.
+template <typename T>
+__device__ __forceinline__ void to_frags(const f32x16& s, Frag<T> (&f)[2]) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[k][e] = static_cast<T>(s[8 * k + e]);
+}
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// Scores in powers of two, as an affine function of what the tiles hold: score = mul * x + add. Plainly x is the dot
+// product and mul = scale log2 e, so that scaling costs nothing beyond the subtraction of the maximum. Capped, with
+// e = exp(2 z / cap), tanh = 1 - 2 / (e + 1), x is -1 / (e + 1): the cap's slope is 1 - tanh^2 = -4 x (1 + x). Its error
+// of 2^-24 or two of the cap is below what 16-bit weights keep; float32 takes the library's tanh, good to an ulp. With a
+// bias x is the score itself, mul = 1. mul is never negative: a negative scale has turned q (or k) over before.
+struct Shape {
+    float raw, mul, add;      // of the score before the bias
+    float twice, turn;        // 2 |scale| log2 e / cap;  |scale| / cap
+    bool cap;
+    template <typename T>
+    static __device__ __forceinline__ Shape of(const wst_attention_desc& d) {
+        Shape s;
+        const float scale = fabsf(d.scale);
+        s.cap = d.cap > 0.f;
+        s.twice = s.cap ? 2.f * scale * kLog2e / d.cap : 0.f;
+        s.turn = s.cap ? scale / d.cap : 0.f;
+        s.raw = !s.cap ? scale * kLog2e : sizeof(T) == 4 ? d.cap * kLog2e : 2.f * d.cap * kLog2e;
+        s.mul = d.slopes ? 1.f : s.raw;
+        s.add = s.cap && sizeof(T) != 4 ? d.cap * kLog2e : 0.f;
+        return s;
+    }
+    // dot products to x before the bias, and the cap's slope
+    template <typename T, bool GRAD>
+    __device__ __forceinline__ void bend(f32x16& x, f32x16& grad) const {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            if constexpr (sizeof(T) == 4) {
+                x[r] = tanhf(x[r] * turn);
+                if constexpr (GRAD) grad[r] = 1.f - x[r] * x[r];
+            } else {
+                x[r] = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(x[r] * twice));
+                if constexpr (GRAD) {
+                    const float y = -4.f * x[r];
+                    grad[r] = fmaf(y, x[r], y);
+                }
+            }
+        }
+    }
+};
+
+// What a lane's query (forward, dq) needs: the first key it may not see in order, its document and coordinates.
+struct Query {
+    int limit, doc, place;
+    uint32_t pos[WST_MAX_AXES];
+};
+constexpr uint32_t kPosBias = 0x40000000u;   // coordinates in +-2^29 as unsigned numbers
+
+__device__ __forceinline__ Query query_of(const Scope& sc, int i, bool ok) {
+    Query q;
+    q.limit = ok ? sc.limit(i) : 0;
+    q.doc = sc.q_doc && ok ? sc.q_doc[i] : -1;
+    if (sc.q_doc && q.doc < 0) q.limit = 0;
+    q.place = i + sc.shift;
+#pragma unroll
+    for (int a = 0; a < WST_MAX_AXES; ++a)
+        q.pos[a] = sc.q_pos && a < sc.axes && ok ? static_cast<uint32_t>(sc.q_pos[static_cast<int64_t>(i) * sc.axes + a]) + kPosBias : 0u;
+    return q;
+}
+
+__device__ __forceinline__ uint32_t away(uint32_t a, uint32_t b, uint32_t sum) { return (a > b ? a - b : b - a) + sum; }
+
+// Which tiles of 64 tokens a block has to visit. With documents: those where some token's document lies in the block's
+// own range; and whether a tile's tokens all belong to the one document that all of the block's own do, so that no pair
+// needs a look. Up to kWords * 64 tiles are marked, tiles beyond are visited.
+constexpr int kWords = 64;
+struct Marks {
+    uint64_t any[kWords], full[kWords];
+};
+
+// own: the documents of the block's tokens own0 .. own0 + own_count - 1 (those below own_rows exist); other: of the tiles
+// tile0 .. tile1 - 1, tokens below other_rows. A wave takes sixteen tiles at a time, all loads on their way at once.
+__device__ __forceinline__ void scan_documents(Marks& m, const int32_t* own, int own0, int own_count, int own_rows,
+                                               const int32_t* other, int tile0, int tile1, int other_rows) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    int lo = INT32_MAX, hi = -1;
+    bool all = true;
+    for (int x = lane; x < own_count && own0 + x < own_rows; x += 64) {
+        const int v = own[own0 + x];
+        all = all && v >= 0;
+        if (v >= 0) {
+            lo = v < lo ? v : lo;
+            hi = v > hi ? v : hi;
+        }
+    }
+#pragma unroll
+    for (int k = 32; k; k >>= 1) {
+        const int a = __shfl_xor(lo, k), b = __shfl_xor(hi, k);
+        lo = a < lo ? a : lo;
+        hi = b > hi ? b : hi;
+    }
+    const bool one = __all(all) && lo == hi;
+    const int count = tile1 - tile0 < kWords * 64 ? tile1 - tile0 : kWords * 64;
+    for (int k0 = w * 16; k0 < count; k0 += 64) {
+        int v[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            const int j = (tile0 + k0 + k) * 64 + lane;
+            v[k] = k0 + k < count && j < other_rows ? other[j] : -1;
+        }
+        uint32_t any = 0, full = 0;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            if (__ballot(v[k] >= lo && v[k] <= hi)) any |= 1u << k;
+            if (one && __ballot(v[k] == lo) == ~0ull) full |= 1u << k;
+        }
+        if (lane == 0) {
+            reinterpret_cast<uint16_t*>(m.any)[k0 >> 4] = static_cast<uint16_t>(any);
+            reinterpret_cast<uint16_t*>(m.full)[k0 >> 4] = static_cast<uint16_t>(full);
+        }
+    }
+}
+
+// The next tile to visit after `t` (of tile0 .. tile1 - 1), tile1 when there is none. Marks of tiles past the last are
+// never set within a group of sixteen; groups past it are not read.
+__device__ __forceinline__ int next_tile(const Marks& m, bool marked, int t, int tile0, int tile1) {
+    ++t;
+    if (!marked) return t < tile1 ? t : tile1;
+    while (t < tile1) {
+        const int k = t - tile0;
+        if (k >= kWords * 64) return t;
+        const uint32_t u = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(m.any)[k >> 4]) >> (k & 15));
+        if (u) return t + __builtin_ctz(u);
+        t += 16 - (k & 15);
+    }
+    return tile1;
+}
+__device__ __forceinline__ bool full_tile(const Marks& m, int k) {
+    return k < kWords * 64 && (__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(m.full)[k >> 4])) >> (k & 15) & 1);
+}
+
+// What goes along with a key tile in LDS: coordinates and documents, ready to compare.
+struct Along {
+    uint32_t pos[WST_MAX_AXES][64];
+    int doc[64];
+};
+
+// One thread's share of it on its way: t < 256 one coordinate, t < 64 one document.
+struct AlongStage {
+    uint32_t pos;
+    int doc;
+    __device__ __forceinline__ void load(const int32_t* p, const int32_t* d, int axes, int row0, int rows, int t) {
+        const int row = row0 + (t & 63);
+        const bool ok = row < rows;
+        if (p) pos = (t >> 6) < axes && ok ? static_cast<uint32_t>(p[static_cast<int64_t>(row) * axes + (t >> 6)]) + kPosBias : 0u;
+        if (d) {
+            doc = t < 64 && ok ? d[row] : -2;    // -2 matches nobody; a key without a document holds a negative number,
+            if (doc < 0) doc = -2;               // and queries without one see nothing anyway
+        }
+    }
+    __device__ __forceinline__ void store(Along& al, const int32_t* p, const int32_t* d, int t) const {
+        if (p) al.pos[t >> 6][t & 63] = pos;
+        if (d && t < 64) al.doc[t] = doc;
+    }
+};
+
+// Turns 32 x 32 dot products (rows: keys key0 + 32 sub .., column: the lane's query) into x of Shape, -inf where the
+// query does not see the key. GRAD: also the cap's slope and the distances.
+template <typename T, bool GRAD>
+__device__ __forceinline__ void scores(f32x16& x, const Shape& sh, float slope2, bool bias, const Scope& sc, const Query& q,
+                                       const Along& al, int key0, int sub, bool masked, f32x16& grad, f32x16& far) {
+    const int h = (threadIdx.x & 63) >> 5;
+    if (sh.cap) sh.bend<T, GRAD>(x, grad);
+    if (bias) {
+        if (sc.q_pos) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                uint32_t sum[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int a = 0; a < WST_MAX_AXES; ++a)
+                    if (a < sc.axes) {
+                        const u32x4 k = *reinterpret_cast<const u32x4*>(&al.pos[a][32 * sub + 8 * g + 4 * h]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sum[e] = away(q.pos[a], k[e], sum[e]);
+                    }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float f = static_cast<float>(sum[e]);
+                    if constexpr (GRAD) far[4 * g + e] = f;
+                    x[4 * g + e] = fmaf(-slope2, f, x[4 * g + e] * sh.raw);
+                }
+            }
+        } else {
+            const float base = static_cast<float>(q.place - (key0 + 32 * sub + 4 * h));
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float f = fabsf(base - static_cast<float>(8 * (r >> 2) + (r & 3)));
+                if constexpr (GRAD) far[r] = f;
+                x[r] = fmaf(-slope2, f, x[r] * sh.raw);
+            }
+        }
+    }
+    if (masked) {
+        const int rel = q.limit - (key0 + 32 * sub + 4 * h);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            if (sc.q_doc) {
+                const i32x4 k = *reinterpret_cast<const i32x4*>(&al.doc[32 * sub + 8 * g + 4 * h]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[4 * g + e] = 8 * g + e < rel && k[e] == q.doc ? x[4 * g + e] : -INFINITY;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[4 * g + e] = 8 * g + e < rel ? x[4 * g + e] : -INFINITY;
+            }
+        }
+    }
+}
+
+template <typename T, int DP>
+__device__ __forceinline__ bool not_finite(const f32x16 (&o)[DP / 32]) {
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < DP / 32; ++k)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) t = fmaf(o[k][r], 0.f, t);
+    return t != t;
+}
+
+constexpr int kBQ = 128, kBK = 64;
+
+// Forward pass: a block takes 128 queries of a head, 32 a wave, and walks the key tiles that any of them may see, keeping
+// the running maximum, sum and output of the softmax in registers; keys and values of a tile are shared through LDS.
+// The maximum moves only when a score exceeds it by 2^8 or more: weights up to 2^8 cost neither sums nor roundings
+// anything, and the output is rarely scaled.
+template <typename T, int DP>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(AttnArgs a) {
+    using L = Tile<T, DP>;
+    __shared__ __attribute__((aligned(256))) char kt[2][kBK * L::kRowBytes], vt[2][kBK * L::kRowBytes];
+    __shared__ Along al[3];
+    __shared__ Marks marks;
+    __shared__ float scratch[4][DP];
+    const wst_attention_desc& d = a.d;
+    const int t = threadIdx.x, lane = t & 63, w = t >> 6, hl = lane >> 5;
+    const uint32_t cells = static_cast<uint32_t>(d.batch) * d.q_heads, bh = blockIdx.x % cells;
+    const int nq = static_cast<int>((d.q_len + kBQ - 1) / kBQ), i0 = (nq - 1 - static_cast<int>(blockIdx.x / cells)) * kBQ;   // long rows first
+    const int64_t b = bh / d.q_heads;
+    const int h = static_cast<int>(bh % d.q_heads), kvh = h / (d.q_heads / d.k_heads);
+    const Scope sc(d, b);
+    const Shape sh = Shape::of<T>(d);
+    const int i = i0 + w * 32 + (lane & 31);
+    const bool ok = i < d.q_len;
+    const Query q = query_of(sc, i, ok);
+    const float slope2 = d.slopes ? d.slopes[h] * kLog2e : 0.f;
+    Frag<T> qf[DP / 16];
+    row_frags<T, DP>(at<T>(d.q, d.q_strides, b, ok ? i : 0, h), ok && q.limit > 0, d.dim, qf);
+    if (d.scale < 0.f) negate<T, DP>(qf);
+
+    // keys below `end` may be seen by some query of the block, keys below `open` by all of its queries in order
+    const int last = i0 + kBQ < d.q_len ? i0 + kBQ - 1 : static_cast<int>(d.q_len) - 1;
+    const int end = sc.limit(last), open = sc.limit(i0);
+    const int tiles = end > 0 ? (end + kBK - 1) / kBK : 0;
+    const bool marked = sc.q_doc != nullptr, along = sc.q_doc || sc.q_pos;
+    if (marked) scan_documents(marks, sc.q_doc, i0, kBQ, static_cast<int>(d.q_len), sc.k_doc, 0, tiles, sc.length);
+    if (marked || d.dim != DP || sc.length % kBK) {
+        clear<sizeof(kt)>(&kt[0][0], t);
+        clear<sizeof(vt)>(&vt[0][0], t);
+    }
+    f32x16 o[DP / 32];
+#pragma unroll
+    for (int k = 0; k < DP / 32; ++k) o[k] = zero16();
+    float m = -INFINITY, l = 0.f;
+
+    const T *kb = at<T>(d.k, d.k_strides, b, 0, kvh), *vb = at<T>(d.v, d.v_strides, b, 0, kvh);
+    const int64_t ks = d.k_strides[1], vs = d.v_strides[1];
+    Fetch<T, DP, kBK> kf, vf;
+    kf.init(ks, d.dim, t);
+    vf.init(vs, d.dim, t);
+    // a tile's keys and values are on their way while the tile before is worked on, its documents and coordinates (which
+    // decide what to fetch) one tile earlier still
+    auto fetch = [&](int n, int buf, const Along& with) {
+        const int* doc = marked ? with.doc : nullptr;
+        kf.issue(kb + static_cast<int64_t>(n) * kBK * ks, ks, sc.length - n * kBK, doc, d.dim, kt[buf], t);
+        vf.issue(vb + static_cast<int64_t>(n) * kBK * vs, vs, sc.length - n * kBK, doc, d.dim, vt[buf], t);
+    };
+    AlongStage as{};
+    if (marked) __syncthreads();       // the marks
+    int tile = next_tile(marks, marked, -1, 0, tiles), next = tile < tiles ? next_tile(marks, marked, tile, 0, tiles) : tiles;
+    if (along) {
+        if (tile < tiles) {
+            as.load(sc.k_pos, sc.k_doc, sc.axes, tile * kBK, sc.length, t);
+            as.store(al[0], sc.k_pos, sc.k_doc, t);
+        }
+        if (next < tiles) {
+            as.load(sc.k_pos, sc.k_doc, sc.axes, next * kBK, sc.length, t);
+            as.store(al[1], sc.k_pos, sc.k_doc, t);
+        }
+    }
+    __syncthreads();                   // documents and zeros
+    if (tile < tiles) fetch(tile, 0, al[0]);
+    int buf = 0, turn = 0;
+    while (tile < tiles) {
+        const int key0 = tile * kBK;
+        const int turn1 = turn == 2 ? 0 : turn + 1, turn2 = turn1 == 2 ? 0 : turn1 + 1;
+        arrived();
+        __syncthreads();               // the tile is there, and nobody reads the other buffer any more
+        if (next < tiles) fetch(next, buf ^ 1, al[turn1]);
+        const int after = next < tiles ? next_tile(marks, marked, next, 0, tiles) : tiles;
+        if (along && after < tiles) as.load(sc.k_pos, sc.k_doc, sc.axes, after * kBK, sc.length, t);
+        const bool masked = key0 + kBK > open || (marked && !full_tile(marks, tile));
+        const char *kc = kt[buf], *vc = vt[buf];
+        f32x16 x[2], unused;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            x[n] = zero16();
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) x[n] = Mma<T>::mul(L::row_frag(kc, 32 * n, c), qf[c], x[n]);
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            scores<T, false>(x[n], sh, slope2, d.slopes != nullptr, sc, q, al[turn], key0, n, masked, unused, unused);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, x[n][r]);
+        }
+        const float mn = halves_max(top) * sh.mul;
+        if (__ballot(mn > m + 8.f)) {
+            const float m1 = fmaxf(m, mn), f = __builtin_amdgcn_exp2f(m - fmaxf(m1, -3.0e38f));
+            m = m1;
+            l *= f;
+#pragma unroll
+            for (int k = 0; k < DP / 32; ++k)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[k][r] *= f;
+        }
+        const float base = fmaxf(m, -3.0e38f);         // nothing seen yet: exp2(-inf) = 0 either way
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                x[n][r] = __builtin_amdgcn_exp2f(fmaf(x[n][r], sh.mul, -base));
+                l += x[n][r];
+            }
+            Frag<T> p[2];
+            to_frags<T>(x[n], p);
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int db = 0; db < DP / 32; ++db) o[db] = Mma<T>::mul(L::col_frag(vc, 32 * n + 16 * k, db), p[k], o[db]);
+        }
+        if (along && after < tiles) as.store(al[turn2], sc.k_pos, sc.k_doc, t);
+        tile = next;
+        next = after;
+        buf ^= 1;
+        turn = turn1;
+    }
+    l = halves_sum(l);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (ok) {
+        T* out = const_cast<T*>(at<T>(a.o, d.o_strides, b, i, h));
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int c = 32 * db + 8 * g + 4 * hl;
+                const float v[4] = {o[db][4 * g] * inv, o[db][4 * g + 1] * inv, o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv};
+                if (c < d.dim) store<4>(out + c, v);
+            }
+        if (hl == 0 && a.lse) a.lse[(b * d.q_heads + h) * d.q_len + i] = l == 0.f ? -INFINITY : (m + sh.add) * kLn2 + logf(l);
+    }
+    // A value that is not finite, of a key that some query of the wave does not see, has reached that query as 0 * inf:
+    // the queries whose output is not finite are done over, key by key. In ordinary data there are none.
+    uint64_t bad = __ballot(ok && not_finite<T, DP>(o));
+    for (bad = (bad | bad >> 32) & 0xffffffffu; bad; bad &= bad - 1)
+        row_forward<T>(a, sc, b, h, i0 + w * 32 + __builtin_ctzll(bad), scratch[w]);
+}
+
+// Few queries over many keys: the queries of all heads that share a key head make up to 32 rows, and the keys are split
+// over blocks, and in a block over its waves, each of which walks its own tiles of 32 keys through its own part of LDS
+// with nothing to wait for. The parts are joined by their maxima and sums, in the block and then by k_attn_join.
+template <typename T, int DP>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_split(AttnArgs a) {
+    using L = Tile<T, DP>;
+    constexpr int kTile = 32 * L::kRowBytes, kLd = DP + 4;
+    constexpr int kBytes = 8 * kTile > 32 * kLd * 4 ? 8 * kTile : 32 * kLd * 4;
+    __shared__ __attribute__((aligned(256))) char pool[kBytes];
+    __shared__ Along al[2];          // a wave's 32 keys in half of one
+    __shared__ Marks marks;
+    __shared__ float wm[4][32], wl[4][32];
+    __shared__ float scratch[4][DP];
+    const wst_attention_desc& d = a.d;
+    const int t = threadIdx.x, lane = t & 63, w = t >> 6, hl = lane >> 5;
+    const int group = d.q_heads / d.k_heads;
+    const int64_t rows = group * d.q_len;
+    // blocks: splits, then tiles of rows, then key heads, then sequences
+    const uint32_t split = blockIdx.x % a.splits, cell = blockIdx.x / a.splits, row_tiles = static_cast<uint32_t>((rows + 31) / 32);
+    const int64_t b = cell / row_tiles / d.k_heads;
+    const int kvh = static_cast<int>(cell / row_tiles % d.k_heads);
+    const int64_t r0 = static_cast<int64_t>(cell % row_tiles) * 32, r = r0 + (lane & 31);
+    const bool ok = r < rows;
+    const int i = static_cast<int>(ok ? r % d.q_len : 0);
+    const int h = kvh * group + static_cast<int>(ok ? r / d.q_len : 0);
+    const Scope sc(d, b);
+    const Shape sh = Shape::of<T>(d);
+    const Query q = query_of(sc, i, ok);
+    const float slope2 = d.slopes ? d.slopes[h] * kLog2e : 0.f;
+    Frag<T> qf[DP / 16];
+    row_frags<T, DP>(at<T>(d.q, d.q_strides, b, i, h), ok && q.limit > 0, d.dim, qf);
+
+    if (d.scale < 0.f) negate<T, DP>(qf);
+    const int end = sc.limit(static_cast<int>(d.q_len) - 1);
+    // this split's keys, in whole groups of 128: a wave has 32 of each
+    const int groups = end > 0 ? (end + 127) / 128 : 0, per = (groups + a.splits - 1) / a.splits;
+    const int g0 = min(static_cast<int>(split) * per, groups), g1 = min(g0 + per, groups);
+    const bool marked = sc.q_doc != nullptr;
+    if (marked) {
+        scan_documents(marks, sc.q_doc, 0, static_cast<int>(d.q_len < 1024 ? d.q_len : 1024), static_cast<int>(d.q_len), sc.k_doc, 2 * g0, 2 * g1, sc.length);
+        __syncthreads();
+    }
+    const bool skip = marked && d.q_len <= 1024;   // else the marks do not speak for all queries
+    auto wanted = [&](int g) {                  // the next group of 128 in whose 64 keys this wave has work
+        for (; g < g1; ++g) {
+            const int k = 2 * (g - g0) + (w >> 1);
+            if (!skip || k >= kWords * 64) return g;
+            if (__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(marks.any)[k >> 4]) >> (k & 15) & 1u)) return g;
+        }
+        return g1;
+    };
+    f32x16 o[DP / 32];
+#pragma unroll
+    for (int k = 0; k < DP / 32; ++k) o[k] = zero16();
+    float m = -INFINITY, l = 0.f;
+    const T *kb = at<T>(d.k, d.k_strides, b, 0, kvh), *vb = at<T>(d.v, d.v_strides, b, 0, kvh);
+    char *kt = pool + 2 * w * kTile, *vt = kt + kTile;
+    Stage<T, DP, 32, 64> ks, vs;
+    uint32_t pos[WST_MAX_AXES];
+    int doc = -2;
+    auto fetch = [&](int key0) {
+        ks.load(kb, d.k_strides[1], key0, sc.length, sc.k_doc, d.dim, lane);
+        vs.load(vb, d.v_strides[1], key0, sc.length, sc.k_doc, d.dim, lane);
+        const int j = key0 + (lane & 31);
+        if (sc.k_pos)
+#pragma unroll
+            for (int x = 0; x < WST_MAX_AXES; ++x)
+                pos[x] = x < sc.axes && j < sc.length ? static_cast<uint32_t>(sc.k_pos[static_cast<int64_t>(j) * sc.axes + x]) + kPosBias : 0u;
+        if (sc.k_doc) {
+            doc = j < sc.length ? sc.k_doc[j] : -2;
+            if (doc < 0) doc = -2;
+        }
+    };
+    Along& mine = al[w >> 1];
+    const int sub = w & 1;
+    int g = wanted(g0);
+    if (g < g1) fetch(g * 128 + 32 * w);
+    while (g < g1) {
+        const int key0 = g * 128 + 32 * w;
+        __builtin_amdgcn_wave_barrier();
+        ks.store(kt, lane);
+        vs.store(vt, lane);
+        if (lane < 32) {
+            if (sc.k_pos)
+#pragma unroll
+                for (int x = 0; x < WST_MAX_AXES; ++x) mine.pos[x][32 * sub + lane] = pos[x];
+            mine.doc[32 * sub + lane] = doc;
+        }
+        __builtin_amdgcn_wave_barrier();
+        const int next = wanted(g + 1);
+        if (next < g1) fetch(next * 128 + 32 * w);
+        f32x16 s = zero16(), unused;
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) s = Mma<T>::mul(L::row_frag(kt, 0, c), qf[c], s);
+        scores<T, false>(s, sh, slope2, d.slopes != nullptr, sc, q, mine, key0 - 32 * sub, sub, true, unused, unused);
+        float top = -INFINITY;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) top = fmaxf(top, s[x]);
+        const float mn = halves_max(top) * sh.mul;
+        if (__ballot(mn > m + 8.f)) {
+            const float m1 = fmaxf(m, mn), f = __builtin_amdgcn_exp2f(m - fmaxf(m1, -3.0e38f));
+            m = m1;
+            l *= f;
+#pragma unroll
+            for (int k = 0; k < DP / 32; ++k)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) o[k][x] *= f;
+        }
+        const float base = fmaxf(m, -3.0e38f);
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+            s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], sh.mul, -base));
+            l += s[x];
+        }
+        Frag<T> p[2];
+        to_frags<T>(s, p);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int db = 0; db < DP / 32; ++db) o[db] = Mma<T>::mul(L::col_frag(vt, 16 * k, db), p[k], o[db]);
+        g = next;
+    }
+    // join the waves
+    l = halves_sum(l);
+    if (hl == 0) {
+        wm[w][lane] = m;
+        wl[w][lane] = l;
+    }
+    __syncthreads();               // and every wave is done with its tiles
+    const int x = lane & 31;
+    const float mm = fmaxf(fmaxf(wm[0][x], wm[1][x]), fmaxf(wm[2][x], wm[3][x])), base = fmaxf(mm, -3.0e38f);
+    float total = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) total += wl[k][x] * __builtin_amdgcn_exp2f(wm[k][x] - base);
+    const float f = __builtin_amdgcn_exp2f(m - base);
+    float* sum = reinterpret_cast<float*>(pool);
+    for (int turn = 0; turn < 4; ++turn) {
+        if (turn == w) {
+#pragma unroll
+            for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    f32x4* c = reinterpret_cast<f32x4*>(sum + x * kLd + 32 * db + 8 * e + 4 * hl);
+                    f32x4 v = turn ? *c : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) v[y] += o[db][4 * e + y] * f;
+                    *c = v;
+                }
+        }
+        __syncthreads();
+    }
+    // a wave writes eight rows
+    for (int y = w * 8; y < w * 8 + 8 && r0 + y < rows; ++y) {
+        const int ii = static_cast<int>((r0 + y) % d.q_len);
+        const int hh = kvh * group + static_cast<int>((r0 + y) / d.q_len);
+        const int64_t row = (b * d.q_heads + hh) * d.q_len + ii;
+        const float my = __shfl(mm, y), ly = __shfl(total, y);
+        if (a.splits > 1) {
+            const int64_t all = d.batch * d.q_heads * d.q_len, slot = split * all + row;
+            for (int e = lane; e < d.dim; e += 64) a.part[slot * d.dim + e] = sum[y * kLd + e];
+            if (lane == 0) {
+                a.part_ml[2 * slot] = my + sh.add;
+                a.part_ml[2 * slot + 1] = ly;
+            }
+        } else {
+            const float inv = ly == 0.f ? 0.f : 1.f / ly;
+            T* out = const_cast<T*>(at<T>(a.o, d.o_strides, b, ii, hh));
+            bool bad = false;
+            for (int e = lane; e < d.dim; e += 64) {
+                const float v = sum[y * kLd + e] * inv;
+                bad = bad || !(fabsf(v) < INFINITY);
+                out[e] = static_cast<T>(v);
+            }
+            if (lane == 0 && a.lse) a.lse[row] = ly == 0.f ? -INFINITY : (my + sh.add) * kLn2 + logf(ly);
+            if (__ballot(bad)) row_forward<T>(a, sc, b, hh, ii, scratch[w]);   // see k_attn_fwd
+        }
+    }
+}
+
+// Joins the splits of a row, a wave a row.
+template <typename T>
+__global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
+    __shared__ float scratch[4][kD];
+    const wst_attention_desc& d = a.d;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t all = d.batch * d.q_heads * d.q_len, row = static_cast<int64_t>(blockIdx.x) * 4 + w;
+    if (row >= all) return;
+    const int64_t bh = row / d.q_len, b = bh / d.q_heads;
+    const int i = static_cast<int>(row % d.q_len);
+    const int h = static_cast<int>(bh % d.q_heads);
+    float m = -INFINITY;
+    for (int s = lane; s < a.splits; s += 64) m = fmaxf(m, a.part_ml[2 * (s * all + row)]);
+    m = wave_max(m);
+    const float base = fmaxf(m, -3.0e38f);
+    float l = 0.f, v[2] = {0.f, 0.f};
+    for (int s = 0; s < a.splits; ++s) {
+        const int64_t slot = s * all + row;
+        const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * slot] - base);
+        l += f * a.part_ml[2 * slot + 1];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            if (lane + 64 * e < d.dim) v[e] += f * a.part[slot * d.dim + lane + 64 * e];
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T* out = const_cast<T*>(at<T>(a.o, d.o_strides, b, i, h));
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+        if (lane + 64 * e < d.dim) {
+            bad = bad || !(fabsf(v[e] * inv) < INFINITY);
+            out[lane + 64 * e] = static_cast<T>(v[e] * inv);
+        }
+    if (lane == 0 && a.lse) a.lse[row] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+    if (__ballot(bad)) row_forward<T>(a, Scope(d, b), b, h, i, scratch[w]);
+}
+
+// Float16 loses small numbers before large ones: weights and score gradients are held 2^6 times as large there, so that
+// they keep their precision down to 2^-20; a score gradient beyond 2^10 then overflows, and its row is done over in
+// float32 like any that is not finite.
+template <typename T>
+inline constexpr float kUp = 1.f;
+template <>
+inline constexpr float kUp<f16> = 64.f;
+
+// dq, the slopes' shares and delta: walks the keys as the forward pass does. Scores come back as (keys x queries), so
+// their gradient is the operand of dq^T = k^T dz^T as it stands; keys are read from LDS both ways. delta goes in as the
+// product's starting value.
+template <typename T, int DP>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(AttnArgs a) {
+    using L = Tile<T, DP>;
+    __shared__ __attribute__((aligned(256))) char kt[2][kBK * L::kRowBytes], vt[2][kBK * L::kRowBytes];
+    __shared__ Along al[3];
+    __shared__ Marks marks;
+    __shared__ float scratch[4][2][DP];
+    const wst_attention_desc& d = a.d;
+    const int t = threadIdx.x, lane = t & 63, w = t >> 6, hl = lane >> 5;
+    const uint32_t cells = static_cast<uint32_t>(d.batch) * d.q_heads, bh = blockIdx.x % cells;
+    const int nq = static_cast<int>((d.q_len + kBQ - 1) / kBQ), qt = nq - 1 - static_cast<int>(blockIdx.x / cells), i0 = qt * kBQ;
+    const int64_t b = bh / d.q_heads;
+    const int h = static_cast<int>(bh % d.q_heads), kvh = h / (d.q_heads / d.k_heads);
+    const Scope sc(d, b);
+    const Shape sh = Shape::of<T>(d);
+    const int i = i0 + w * 32 + (lane & 31);
+    const int64_t row = (b * d.q_heads + h) * d.q_len + i;
+    const bool ok = i < d.q_len;
+    const Query q = query_of(sc, i, ok);
+    const float slope2 = d.slopes ? d.slopes[h] * kLog2e : 0.f;
+    const float lse = ok ? a.g.lse[row] : -INFINITY;
+    const bool live = ok && q.limit > 0 && lse != -INFINITY;
+    const float base = live ? sh.add - lse * kLog2e : -INFINITY;         // of a query that sees nothing every weight is 0
+    Frag<T> qf[DP / 16], df[DP / 16];
+    float delta = 0.f;
+    {
+        Frag<T> of[DP / 16];
+        row_frags<T, DP>(at<T>(a.g.d_o, a.g.do_strides, b, ok ? i : 0, h), live, d.dim, df);
+        row_frags<T, DP>(at<T>(a.g.o, d.o_strides, b, ok ? i : 0, h), live, d.dim, of);
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) delta += static_cast<float>(df[c][e]) * static_cast<float>(of[c][e]);
+        delta = halves_sum(delta);
+        if (ok && hl == 0) a.delta[row] = delta;
+    }
+    row_frags<T, DP>(at<T>(d.q, d.q_strides, b, ok ? i : 0, h), live, d.dim, qf);
+    if (d.scale < 0.f) negate<T, DP>(qf);
+
+    // keys below `end` may be seen by some query of the block, keys below `open` by all of its queries in order
+    const int last = i0 + kBQ < d.q_len ? i0 + kBQ - 1 : static_cast<int>(d.q_len) - 1;
+    const int end = sc.limit(last), open = sc.limit(i0);
+    const int tiles = end > 0 ? (end + kBK - 1) / kBK : 0;
+    const bool marked = sc.q_doc != nullptr, along = sc.q_doc || sc.q_pos;
+    if (marked) scan_documents(marks, sc.q_doc, i0, kBQ, static_cast<int>(d.q_len), sc.k_doc, 0, tiles, sc.length);
+    if (marked || d.dim != DP || sc.length % kBK) {
+        clear<sizeof(kt)>(&kt[0][0], t);
+        clear<sizeof(vt)>(&vt[0][0], t);
+    }
+    f32x16 dq[DP / 32];
+#pragma unroll
+    for (int k = 0; k < DP / 32; ++k) dq[k] = zero16();
+    // The slopes' share, -sum ds far. delta comes from the rounded output, and its error would meet a mean distance: with
+    // e = sum ds (0, were delta exact) the share is -(sum ds far - e sum p far).
+    float pf = 0.f, e0 = 0.f, e1 = 0.f;
+
+    const T *kb = at<T>(d.k, d.k_strides, b, 0, kvh), *vb = at<T>(d.v, d.v_strides, b, 0, kvh);
+    const int64_t ks = d.k_strides[1], vs = d.v_strides[1];
+    Fetch<T, DP, kBK> kf, vf;
+    kf.init(ks, d.dim, t);
+    vf.init(vs, d.dim, t);
+    // a tile's keys and values are on their way while the tile before is worked on, its documents and coordinates (which
+    // decide what to fetch) one tile earlier still
+    auto fetch = [&](int n, int buf, const Along& with) {
+        const int* doc = marked ? with.doc : nullptr;
+        kf.issue(kb + static_cast<int64_t>(n) * kBK * ks, ks, sc.length - n * kBK, doc, d.dim, kt[buf], t);
+        vf.issue(vb + static_cast<int64_t>(n) * kBK * vs, vs, sc.length - n * kBK, doc, d.dim, vt[buf], t);
+    };
+    AlongStage as{};
+    if (marked) __syncthreads();       // the marks
+    int tile = next_tile(marks, marked, -1, 0, tiles), next = tile < tiles ? next_tile(marks, marked, tile, 0, tiles) : tiles;
+    if (along) {
+        if (tile < tiles) {
+            as.load(sc.k_pos, sc.k_doc, sc.axes, tile * kBK, sc.length, t);
+            as.store(al[0], sc.k_pos, sc.k_doc, t);
+        }
+        if (next < tiles) {
+            as.load(sc.k_pos, sc.k_doc, sc.axes, next * kBK, sc.length, t);
+            as.store(al[1], sc.k_pos, sc.k_doc, t);
+        }
+    }
+    __syncthreads();                   // documents and zeros
+    if (tile < tiles) fetch(tile, 0, al[0]);
+    int buf = 0, turn = 0;
+    while (tile < tiles) {
+        const int key0 = tile * kBK;
+        const int turn1 = turn == 2 ? 0 : turn + 1, turn2 = turn1 == 2 ? 0 : turn1 + 1;
+        arrived();
+        __syncthreads();               // the tile is there, and nobody reads the other buffer any more
+        if (next < tiles) fetch(next, buf ^ 1, al[turn1]);
+        const int after = next < tiles ? next_tile(marks, marked, next, 0, tiles) : tiles;
+        if (along && after < tiles) as.load(sc.k_pos, sc.k_doc, sc.axes, after * kBK, sc.length, t);
+        const bool masked = key0 + kBK > open || (marked && !full_tile(marks, tile));
+        const char *kc = kt[buf], *vc = vt[buf];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            f32x16 x = zero16(), dp, grad, far;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dp[r] = -delta;
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) x = Mma<T>::mul(L::row_frag(kc, 32 * n, c), qf[c], x);
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) dp = Mma<T>::mul(L::row_frag(vc, 32 * n, c), df[c], dp);
+            scores<T, true>(x, sh, slope2, d.slopes != nullptr, sc, q, al[turn], key0, n, masked, grad, far);
+            if (masked) {     // a weight of 0 may meet a value that is not finite
+#pragma unroll
+                for (int r = 0; r < 16; ++r) dp[r] = x[r] == -INFINITY ? 0.f : dp[r];
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], sh.mul, base));
+                dp[r] *= x[r];
+            }
+            if (a.slope_part) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    pf = fmaf(x[r], far[r], pf);
+                    e0 += dp[r];
+                    e1 = fmaf(dp[r], far[r], e1);
+                }
+            }
+            if (sh.cap) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) dp[r] *= grad[r];
+            }
+            if constexpr (kUp<T> != 1.f) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) dp[r] *= kUp<T>;
+            }
+            Frag<T> z[2];
+            to_frags<T>(dp, z);
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int db = 0; db < DP / 32; ++db) dq[db] = Mma<T>::mul(L::col_frag(kc, 32 * n + 16 * k, db), z[k], dq[db]);
+        }
+        if (along && after < tiles) as.store(al[turn2], sc.k_pos, sc.k_doc, t);
+        tile = next;
+        next = after;
+        buf ^= 1;
+        turn = turn1;
+    }
+    const float mul = d.scale / kUp<T>;
+    if (ok && a.g.dq) {
+        T* out = const_cast<T*>(at<T>(a.g.dq, a.g.dq_strides, b, i, h));
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int c = 32 * db + 8 * g + 4 * hl;
+                const float v[4] = {dq[db][4 * g] * mul, dq[db][4 * g + 1] * mul, dq[db][4 * g + 2] * mul, dq[db][4 * g + 3] * mul};
+                if (c < d.dim) store<4>(out + c, v);
+            }
+    }
+    if (a.slope_part) {
+        const float share = halves_sum(e0) * halves_sum(pf) - halves_sum(e1), sum = wave_sum(hl ? 0.f : share);
+        if (lane == 0) a.slope_part[(static_cast<int64_t>(h) * d.batch + b) * a.slots + qt * 4 + w] = sum;
+    }
+    uint64_t bad = __ballot(ok && not_finite<T, DP>(dq));      // see k_attn_fwd
+    for (bad = (bad | bad >> 32) & 0xffffffffu; bad; bad &= bad - 1) {
+        __builtin_amdgcn_wave_barrier();
+        row_dq<T>(a, sc, b, h, i0 + w * 32 + __builtin_ctzll(bad), scratch[w][0], scratch[w][1]);
+    }
+}
+
+// What goes along with a tile of 64 queries.
+struct Rows {
+    float base[64], delta[64];     // add - lse log2 e; -delta
+    int limit[64], doc[64], place[64];
+    uint32_t pos[WST_MAX_AXES][64];
+};
+
+// dk and dv: a block takes 128 keys of a key head, 32 a wave, held as operands in registers, and walks tiles of 64
+// queries of the heads that share it. Scores come as (queries x keys), one key a lane, so weights and score gradients
+// are the operands of dv^T = do^T p and dk^T = q^T dz as they stand. With few key tiles the walk is split in parts whose
+// sums k_attn_dkv_join adds in order.
+template <typename T, int DP>
+__global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64) ? 2 : 1) void k_attn_dkv(AttnArgs a) {
+    using L = Tile<T, DP>;
+    constexpr int kRows = 64;
+    __shared__ __attribute__((aligned(256))) char qt[2][kRows * L::kRowBytes], dt[2][kRows * L::kRowBytes];
+    __shared__ Rows rows[3];
+    __shared__ Marks marks;
+    __shared__ float scratch[4][2][DP];
+    const wst_attention_desc& d = a.d;
+    const int t = threadIdx.x, lane = t & 63, w = t >> 6, hl = lane >> 5, group = d.q_heads / d.k_heads;
+    const uint32_t cells = static_cast<uint32_t>(d.batch) * d.k_heads, bh = blockIdx.x % cells, part = blockIdx.y;
+    const int j0 = static_cast<int>(blockIdx.x / cells) * kBQ;         // early keys are seen by most: first
+    const int64_t b = bh / d.k_heads;
+    const int kvh = static_cast<int>(bh % d.k_heads);
+    const Scope sc(d, b);
+    const Shape sh = Shape::of<T>(d);
+    const int j = j0 + w * 32 + (lane & 31), q_len = static_cast<int>(d.q_len);
+    const bool exists = j < d.k_len, ok = j < sc.length && (!sc.k_doc || sc.k_doc[j] >= 0);
+    const int kdoc = ok && sc.k_doc ? sc.k_doc[j] : -2;
+    uint32_t kpos[WST_MAX_AXES];
+#pragma unroll
+    for (int x = 0; x < WST_MAX_AXES; ++x)
+        kpos[x] = ok && sc.k_pos && x < sc.axes ? static_cast<uint32_t>(sc.k_pos[static_cast<int64_t>(j) * sc.axes + x]) + kPosBias : 0u;
+    Frag<T> kf[DP / 16], vf[DP / 16];
+    row_frags<T, DP>(at<T>(d.k, d.k_strides, b, ok ? j : 0, kvh), ok, d.dim, kf);
+    row_frags<T, DP>(at<T>(d.v, d.v_strides, b, ok ? j : 0, kvh), ok, d.dim, vf);
+    if (d.scale < 0.f) negate<T, DP>(kf);
+    f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+    for (int k = 0; k < DP / 32; ++k) dk[k] = dv[k] = zero16();
+
+    // queries from `first` on may see one of the block's keys; keys past the length are seen by none
+    const int nqt = (q_len + kRows - 1) / kRows, keys = min(sc.length - j0, kBQ);
+    const int first = sc.causal && j0 >= sc.prefix ? max(j0 - sc.shift, 0) : 0;
+    const int tile0 = first / kRows, tiles = keys > 0 ? nqt : 0;
+    const bool marked = sc.q_doc != nullptr;
+    if (marked && tile0 < tiles) scan_documents(marks, sc.k_doc, j0, kBQ, sc.length, sc.q_doc, tile0, tiles, q_len);
+    if (marked || d.dim != DP || q_len % kRows) {
+        clear<sizeof(qt)>(&qt[0][0], t);
+        clear<sizeof(dt)>(&dt[0][0], t);
+    }
+    const int64_t qs = d.q_strides[1], ds = a.g.do_strides[1];
+    Fetch<T, DP, kRows> qfetch, dfetch;
+    qfetch.init(qs, d.dim, t);
+    dfetch.init(ds, d.dim, t);
+
+    // items of work: the visited tiles of the first head, then of the next, ...; this part takes every a.parts-th
+    struct Item {
+        int tile, g;
+    };
+    auto step = [&](Item x) {
+        x.tile = next_tile(marks, marked, x.tile, tile0, tiles);
+        while (x.tile >= tiles && x.g + 1 < group) {
+            ++x.g;
+            x.tile = next_tile(marks, marked, tile0 - 1, tile0, tiles);
+            if (x.tile >= tiles) x.g = group;    // nothing to visit in any head
+        }
+        return x;
+    };
+    auto skip = [&](Item x, int n) {
+        for (int k = 0; k < n && x.tile < tiles; ++k) x = step(x);
+        return x;
+    };
+    float r_base = -INFINITY, r_delta = 0.f;
+    int r_limit = 0, r_doc = -1, r_place = 0;
+    uint32_t r_pos = 0;
+    auto load = [&](Item x) {
+        const int h = kvh * group + x.g, i = x.tile * kRows + (t & 63);
+        const bool in = i < q_len;
+        if (t < 64) {
+            const int64_t row = (b * d.q_heads + h) * d.q_len + i;
+            const float lse = in ? a.g.lse[row] : -INFINITY;
+            r_limit = in ? sc.limit(i) : 0;
+            r_doc = sc.q_doc && in ? sc.q_doc[i] : -1;
+            if (sc.q_doc && r_doc < 0) r_limit = 0;
+            r_base = lse == -INFINITY || r_limit <= 0 ? -INFINITY : sh.add - lse * kLog2e;
+            r_delta = in ? -a.delta[row] : 0.f;
+            r_place = i + sc.shift;
+        }
+        if (sc.q_pos) r_pos = (t >> 6) < sc.axes && in ? static_cast<uint32_t>(sc.q_pos[static_cast<int64_t>(i) * sc.axes + (t >> 6)]) + kPosBias : 0u;
+    };
+    auto put = [&](Rows& rw) {
+        if (t < 64) {
+            rw.base[t] = r_base;
+            rw.delta[t] = r_delta;
+            rw.limit[t] = r_limit;
+            rw.doc[t] = r_doc;
+            rw.place[t] = r_place;
+        }
+        if (sc.q_pos) rw.pos[t >> 6][t & 63] = r_pos;
+    };
+    auto fetch = [&](Item x, int buf, const Rows& with) {
+        const int h = kvh * group + x.g, i = x.tile * kRows;
+        const int* doc = marked ? with.doc : nullptr;
+        qfetch.issue(at<T>(d.q, d.q_strides, b, i, h), qs, q_len - i, doc, d.dim, qt[buf], t);
+        dfetch.issue(at<T>(a.g.d_o, a.g.do_strides, b, i, h), ds, q_len - i, doc, d.dim, dt[buf], t);
+    };
+    if (marked) __syncthreads();       // the marks
+    Item cur{tile0 - 1, 0};
+    if (tile0 < tiles) cur = skip(step(cur), part);
+    else cur.tile = tiles;
+    Item nxt = skip(cur, a.parts);
+    if (cur.tile < tiles) {
+        load(cur);
+        put(rows[0]);
+    }
+    if (nxt.tile < tiles) {
+        load(nxt);
+        put(rows[1]);
+    }
+    __syncthreads();
+    if (cur.tile < tiles) fetch(cur, 0, rows[0]);
+    int buf = 0, turn = 0;
+    while (cur.tile < tiles) {
+        const int row0 = cur.tile * kRows, turn1 = turn == 2 ? 0 : turn + 1, turn2 = turn1 == 2 ? 0 : turn1 + 1;
+        const float slope2 = d.slopes ? d.slopes[kvh * group + cur.g] * kLog2e : 0.f;
+        const Rows& rw = rows[turn];
+        const char *qc = qt[buf], *dc = dt[buf];
+        arrived();
+        __syncthreads();
+        if (nxt.tile < tiles) fetch(nxt, buf ^ 1, rows[turn1]);
+        const Item after = skip(nxt, a.parts);
+        if (after.tile < tiles) load(after);
+        // no pair needs a look when all rows and keys exist and the tile's first query sees the block's last key
+        const bool masked = row0 + kRows > q_len || keys < kBQ || sc.limit(row0) < j0 + kBQ || (marked && !full_tile(marks, cur.tile - tile0));
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            f32x16 x = zero16(), dp, grad;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const f32x4 v = *reinterpret_cast<const f32x4*>(&rw.delta[32 * n + 8 * c + 4 * hl]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) dp[4 * c + e] = v[e];
+            }
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) x = Mma<T>::mul(L::row_frag(qc, 32 * n, c), kf[c], x);
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) dp = Mma<T>::mul(L::row_frag(dc, 32 * n, c), vf[c], dp);
+            if (sh.cap) sh.bend<T, true>(x, grad);
+            if (d.slopes) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int y = 32 * n + 8 * c + 4 * hl;
+                    float f[4];
+                    if (sc.q_pos) {
+                        uint32_t sum[4] = {0, 0, 0, 0};
+#pragma unroll
+                        for (int k = 0; k < WST_MAX_AXES; ++k)
+                            if (k < sc.axes) {
+                                const u32x4 v = *reinterpret_cast<const u32x4*>(&rw.pos[k][y]);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) sum[e] = away(kpos[k], v[e], sum[e]);
+                            }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) f[e] = static_cast<float>(sum[e]);
+                    } else {
+                        const i32x4 v = *reinterpret_cast<const i32x4*>(&rw.place[y]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) f[e] = fabsf(static_cast<float>(v[e] - j));
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[4 * c + e] = fmaf(-slope2, f[e], x[4 * c + e] * sh.raw);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const f32x4 v = *reinterpret_cast<const f32x4*>(&rw.base[32 * n + 8 * c + 4 * hl]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[4 * c + e] = __builtin_amdgcn_exp2f(fmaf(x[4 * c + e], sh.mul, v[e]));
+            }
+            if (masked) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int y = 32 * n + 8 * c + 4 * hl;
+                    const i32x4 lim = *reinterpret_cast<const i32x4*>(&rw.limit[y]), doc = *reinterpret_cast<const i32x4*>(&rw.doc[y]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const bool see = j < lim[e] && (!marked || kdoc == doc[e]);
+                        x[4 * c + e] = see ? x[4 * c + e] : 0.f;
+                        dp[4 * c + e] = see ? dp[4 * c + e] : 0.f;
+                    }
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                x[r] *= kUp<T>;
+                dp[r] *= x[r];
+            }
+            if (sh.cap) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) dp[r] *= grad[r];
+            }
+            Frag<T> p[2], z[2];
+            to_frags<T>(x, p);
+            to_frags<T>(dp, z);
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int db = 0; db < DP / 32; ++db) {
+                    dv[db] = Mma<T>::mul(L::col_frag(dc, 32 * n + 16 * k, db), p[k], dv[db]);
+                    dk[db] = Mma<T>::mul(L::col_frag(qc, 32 * n + 16 * k, db), z[k], dk[db]);
+                }
+        }
+        if (after.tile < tiles) put(rows[turn2]);
+        cur = nxt;
+        nxt = after;
+        buf ^= 1;
+        turn = turn1;
+    }
+    const float up = 1.f / kUp<T>, mul = d.scale * up;
+    if (a.parts > 1) {
+        if (exists) {
+            const int64_t row = ((static_cast<int64_t>(part) * d.batch + b) * d.k_heads + kvh) * d.k_len + j;
+#pragma unroll
+            for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+                for (int g4 = 0; g4 < 4; ++g4) {
+                    const int x = 32 * db + 8 * g4 + 4 * hl;
+                    if (x < d.dim) {
+                        float u[4], v[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            u[e] = dk[db][4 * g4 + e] * mul;
+                            v[e] = dv[db][4 * g4 + e] * up;
+                        }
+                        store<4>(a.part + (2 * row) * d.dim + x, u);
+                        store<4>(a.part + (2 * row + 1) * d.dim + x, v);
+                    }
+                }
+        }
+        return;
+    }
+    if (exists) {
+        T* out_k = a.g.dk ? const_cast<T*>(at<T>(a.g.dk, a.g.dk_strides, b, j, kvh)) : nullptr;
+        T* out_v = a.g.dv ? const_cast<T*>(at<T>(a.g.dv, a.g.dv_strides, b, j, kvh)) : nullptr;
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+            for (int g4 = 0; g4 < 4; ++g4) {
+                const int x = 32 * db + 8 * g4 + 4 * hl;
+                if (x < d.dim) {
+                    float u[4], v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        u[e] = dk[db][4 * g4 + e] * mul;
+                        v[e] = dv[db][4 * g4 + e] * up;
+                    }
+                    if (out_k) store<4>(out_k + x, u);
+                    if (out_v) store<4>(out_v + x, v);
+                }
+            }
+    }
+    uint64_t bad = __ballot(exists && (not_finite<T, DP>(dk) || not_finite<T, DP>(dv)));      // see k_attn_fwd
+    for (bad = (bad | bad >> 32) & 0xffffffffu; bad; bad &= bad - 1) {
+        __builtin_amdgcn_wave_barrier();
+        row_dkv<T>(a, sc, b, kvh, j0 + w * 32 + __builtin_ctzll(bad), scratch[w][0], scratch[w][1]);
+    }
+}
+
+// Adds the parts of a key's gradients, a wave a key.
+template <typename T>
+__global__ __launch_bounds__(256) void k_attn_dkv_join(AttnArgs a) {
+    __shared__ float scratch[4][2][kD];
+    const wst_attention_desc& d = a.d;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int j = static_cast<int>(blockIdx.x) * 4 + w;
+    const int64_t b = blockIdx.z;
+    const int kvh = blockIdx.y;
+    if (j >= d.k_len) return;
+    float v[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+    for (int p = 0; p < a.parts; ++p) {
+        const float* s = a.part + 2 * (((p * d.batch + b) * d.k_heads + kvh) * d.k_len + j) * d.dim;
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            if (lane + 64 * e < d.dim) {
+                v[0][e] += s[lane + 64 * e];
+                v[1][e] += s[d.dim + lane + 64 * e];
+            }
+    }
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+        if (lane + 64 * e < d.dim) {
+            bad = bad || !(fabsf(v[0][e]) < INFINITY) || !(fabsf(v[1][e]) < INFINITY);
+            if (a.g.dk) const_cast<T*>(at<T>(a.g.dk, a.g.dk_strides, b, j, kvh))[lane + 64 * e] = static_cast<T>(v[0][e]);
+            if (a.g.dv) const_cast<T*>(at<T>(a.g.dv, a.g.dv_strides, b, j, kvh))[lane + 64 * e] = static_cast<T>(v[1][e]);
+        }
+    if (__ballot(bad)) row_dkv<T>(a, Scope(d, b), b, kvh, j, scratch[w][0], scratch[w][1]);
+}
+
+template <typename F>
+void with_width(int dim, F f) {
+    if (dim <= 32) f(std::integral_constant<int, 32>{});
+    else if (dim <= 64) f(std::integral_constant<int, 64>{});
+    else if (dim <= 96) f(std::integral_constant<int, 96>{});
+    else f(std::integral_constant<int, 128>{});
+}
+
+// Launches for one element type (wst_attention_t.hip).
+template <typename T>
+__attribute__((visibility("hidden"))) void attend(const AttnArgs& a, const AttnPlan& p, hipStream_t st);
+template <typename T>
+__attribute__((visibility("hidden"))) void attend_backward(const AttnArgs& a, const AttnPlan& p, hipStream_t st);
+
+}  // namespace wst_tok
+
+#endif  // WST_ATTENTION_H
