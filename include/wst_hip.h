@@ -283,7 +283,8 @@ const char* wst_aux_last_error(void);
 
 enum wst_dtype { WST_F32 = 0, WST_BF16 = 1, WST_F16 = 2 };
 
-#define WST_MAX_AXES 4
+#define WST_MAX_AXES 4            /* of rotary positions */
+#define WST_MAX_DISTANCE_AXES 3   /* of attention's distances */
 #define WST_MAX_HEAD_DIM 256
 
 /* Thread-local message of the last failed wst_layer_norm_* / wst_rotary / wst_attention_* call. */
@@ -349,7 +350,7 @@ typedef struct wst_attention_desc {
     int64_t q_pos_stride, k_pos_stride, q_doc_stride, k_doc_stride;   /* of a batch entry; 0 when shared */
     const void *q, *k, *v;
     const float* slopes;                       /* (q_heads) or NULL: no distance bias */
-    const int32_t *q_pos, *k_pos;              /* (q_len, axes), (k_len, axes) or both NULL */
+    const int32_t *q_pos, *k_pos;              /* (q_len, axes), (k_len, axes), or both NULL; axes <= WST_MAX_DISTANCE_AXES */
     const int32_t *q_doc, *k_doc;              /* (q_len), (k_len) or both NULL; negative: belongs to none */
     const int32_t* k_lengths;                  /* (batch) or NULL */
     const int32_t* prefix;                     /* (batch) or NULL; needs causal */

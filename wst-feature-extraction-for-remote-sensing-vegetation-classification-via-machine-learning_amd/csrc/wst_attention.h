@@ -84,6 +84,7 @@ struct Scope {
     }
 };
 
+constexpr int kAxes = WST_MAX_DISTANCE_AXES;
 constexpr int kD = WST_MAX_HEAD_DIM, kPer = kD / 64;   // values of a row a lane holds: d = lane + 64 c
 
 template <typename T>
@@ -378,15 +379,47 @@ struct Tile {
     }
     static __device__ __forceinline__ int at(int row, int unit) { return row * kRowBytes + ((unit ^ swizzle(row)) << 4); }
 
+    // Where a lane reads in a tile. Unit indexes enter the swizzle by exclusive or, so every fragment's address is the
+    // lane's own, exclusive-or a constant, plus a constant that the instruction adds: one operation a read, and one
+    // register kept. (Taken as a sum, the compiler keeps the address of every fragment in a register, and spills.)
+    struct Lane {
+        uint32_t row, col;
+        // anew for each tile, and in a way the compiler does not see through, or it would keep them all again
+        __device__ __forceinline__ Lane at_tile(const char* tile) const {
+            const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((WST_LDS const char*)tile));
+            Lane l{row + base, col + base};
+            asm volatile("" : "+v"(l.row), "+v"(l.col));
+            return l;
+        }
+    };
+    static __device__ __forceinline__ Lane lane() {
+        const int x = threadIdx.x & 63, h = x >> 5;
+        Lane l;
+        if constexpr (sizeof(T) == 2) {
+            l.row = at(x & 31, h);
+            // the transposing read: sixteen lanes hand in four rows of sixteen values and get a column of four each
+            const int g = x >> 4, y = x & 15;
+            l.col = at(4 * (g >> 1) + (y >> 2), 2 * (g & 1) + ((y & 3) >> 1)) + 8 * (y & 1);
+        } else {
+            l.row = at(x & 31, 2 * h);
+            l.col = 4 * h * kRowBytes + 4 * (x & 31);      // unswizzled
+        }
+        return l;
+    }
+    // of a constant unit offset: the bits the swizzle reaches, and the rest
+    static constexpr int kBits = kUnits % 16 == 0 ? 15 : kUnits % 8 == 0 ? 7 : 3;
+    static __device__ __forceinline__ uint32_t to(uint32_t lane, int row, int unit) {
+        return (lane ^ ((unit & kBits) << 4)) + row * kRowBytes + ((unit & ~kBits) << 4);
+    }
+
     // row row0 + lane % 32, values 16 c + 8 (lane / 32) .. + 7; row0 a multiple of 16
-    static __device__ __forceinline__ Frag<T> row_frag(const char* t, int row0, int c) {
-        const int lane = threadIdx.x & 63, row = lane & 31, h = lane >> 5;
+    static __device__ __forceinline__ Frag<T> row_frag(const Lane& l, int row0, int c) {
         Frag<T> f;
         if constexpr (sizeof(T) == 2) {
-            f = *reinterpret_cast<const Frag<T>*>(t + row0 * kRowBytes + at(row, 2 * c + h));
+            f = *(WST_LDS const Frag<T>*)(to(l.row, row0, 2 * c));
         } else {
-            const f32x4 a = *reinterpret_cast<const f32x4*>(t + row0 * kRowBytes + at(row, 4 * c + 2 * h));
-            const f32x4 b = *reinterpret_cast<const f32x4*>(t + row0 * kRowBytes + at(row, 4 * c + 2 * h + 1));
+            const f32x4 a = *(WST_LDS const f32x4*)(to(l.row, row0, 4 * c));
+            const f32x4 b = *(WST_LDS const f32x4*)(to(l.row, row0, 4 * c + 1));
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 f[e] = a[e];
@@ -396,27 +429,26 @@ struct Tile {
         return f;
     }
     // value 32 db + lane % 32 of the eight rows row0 + 8 (e / 4) + 4 (lane / 32) + e % 4; row0 a multiple of 16
-    static __device__ __forceinline__ Frag<T> col_frag(const char* t, int row0, int db) {
-        const int lane = threadIdx.x & 63;
+    static __device__ __forceinline__ Frag<T> col_frag(const Lane& l, int row0, int db) {
         Frag<T> f;
         if constexpr (sizeof(T) == 2) {
-            // the transposing read: sixteen lanes hand in four rows of sixteen values and get a column of four each
-            const int g = lane >> 4, x = lane & 15, row = 4 * (g >> 1) + (x >> 2), unit = 4 * db + 2 * (g & 1) + ((x & 3) >> 1);
             typedef short s16x4 __attribute__((ext_vector_type(4)));
             union {
                 s16x4 q[2];
                 Frag<T> f;
             } u;
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
-                u.q[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (WST_LDS s16x4*)(t + row0 * kRowBytes + at(8 * k + row, unit) + 8 * (x & 1)));
+            for (int k = 0; k < 2; ++k)      // eight rows on, swizzle bit 1 turns
+                u.q[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((WST_LDS s16x4*)(to(l.col, row0 + 8 * k, 4 * db + 2 * k)));
             f = u.f;
         } else {
-            const int d = 32 * db + (lane & 31), h = lane >> 5;
+            const int h = (threadIdx.x & 63) >> 5;
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                f[e] = *reinterpret_cast<const float*>(t + row0 * kRowBytes + at(8 * (e >> 2) + 4 * h + (e & 3), d >> 2) + 4 * (d & 3));
+            for (int e = 0; e < 8; ++e) {
+                const int row = 8 * (e >> 2) + (e & 3);
+                const uint32_t swz = (swizzle(row) << 4) ^ (swizzle(4 * h) << 4);
+                f[e] = *(WST_LDS const float*)(((l.col + db * 128) ^ swz) + (row0 + row) * kRowBytes);
+            }
         }
         return f;
     }
@@ -449,6 +481,14 @@ struct Stage {
     }
 };
 
+// A pointer that is the same for all lanes, as a scalar.
+template <typename T>
+__device__ __forceinline__ T* uniform(T* p) {
+    const uint64_t x = reinterpret_cast<uint64_t>(p);
+    return reinterpret_cast<T*>(static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x >> 32))) << 32 |
+                                static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x))));
+}
+
 // N rows of a tensor straight into LDS, past the registers, by 256 threads: each lane names the 16 bytes it wants, and a
 // wave's land one after the other, so the swizzle is in the choice of the source. A lane's offsets from the tile's first
 // row are the same for every tile; what moves is the scalar base. Lanes whose row does not exist or belongs to no
@@ -464,8 +504,12 @@ struct Fetch {
     static constexpr bool kSame = 256 % L::kUnits == 0 && kStep % 16 == 0;            // the same unit and swizzle in each
     static constexpr int kOff = kSame ? 1 : kCount;
     uint32_t off[kOff], live;
+    int64_t stride;
+    uint32_t wave;          // this wave's part of a tile
 
-    __device__ __forceinline__ void init(int64_t stride, int dim, int t) {
+    __device__ __forceinline__ void init(int64_t stride_, int dim, int t) {
+        stride = stride_;
+        wave = __builtin_amdgcn_readfirstlane(t >> 6) * 1024;
         live = 0;
 #pragma unroll
         for (int i = 0; i < kCount; ++i) {
@@ -474,24 +518,18 @@ struct Fetch {
             live |= static_cast<uint32_t>(unit * L::kElems < dim) << i;
         }
     }
-    // base: the tile's first row; left: rows that exist from there on; doc: the rows' documents in LDS, or nullptr
-    __device__ __forceinline__ void issue(const T* base, int64_t stride, int left, const int* doc, int dim, const char* tile, int t) const {
-        const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((WST_LDS const char*)tile)) + (t & ~63) * 16;
-        if (left >= N && !doc && dim == DP) {
+    // base: the tile's first row; whole: all its rows exist, and belong to some document; left: rows that exist from
+    // there on; doc: the rows' documents in LDS, or nullptr
+    __device__ __forceinline__ void issue(const T* base, bool whole, int left, const int* doc, const char* tile, int t) const {
+        const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((WST_LDS const char*)tile)) + wave;
 #pragma unroll
-            for (int i = 0; i < kCount; ++i) load(base, stride, i, lds);
-        } else {
-#pragma unroll
-            for (int i = 0; i < kCount; ++i) {
-                const int row = (t + i * 256) / L::kUnits;
-                if ((live >> i & 1) && row < left && (!doc || doc[row] >= 0)) load(base, stride, i, lds);
-            }
+        for (int i = 0; i < kCount; ++i) {
+            const int row = (t + i * 256) / L::kUnits;
+            const T* b = kSame ? base + i * kStep * stride : base;
+            if (whole || ((live >> i & 1) && row < left && (!doc || doc[row] >= 0)))
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                             : : "s"(__builtin_amdgcn_readfirstlane(lds + i * 4096)), "v"(off[kSame ? 0 : i]), "s"(uniform(b)) : "memory", "m0");
         }
-    }
-    __device__ __forceinline__ void load(const T* base, int64_t stride, int i, uint32_t lds) const {
-        const T* b = kSame ? base + i * kStep * stride : base;
-        const uint32_t dst = __builtin_amdgcn_readfirstlane(lds + i * 4096);
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(dst), "v"(off[kSame ? 0 : i]), "s"(b) : "memory", "m0");
     }
 };
 __device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
@@ -576,7 +614,7 @@ struct Shape {
 // What a lane's query (forward, dq) needs: the first key it may not see in order, its document and coordinates.
 struct Query {
     int limit, doc, place;
-    uint32_t pos[WST_MAX_AXES];
+    uint32_t pos[kAxes];
 };
 constexpr uint32_t kPosBias = 0x40000000u;   // coordinates in +-2^29 as unsigned numbers
 
@@ -587,7 +625,7 @@ __device__ __forceinline__ Query query_of(const Scope& sc, int i, bool ok) {
     if (sc.q_doc && q.doc < 0) q.limit = 0;
     q.place = i + sc.shift;
 #pragma unroll
-    for (int a = 0; a < WST_MAX_AXES; ++a)
+    for (int a = 0; a < kAxes; ++a)
         q.pos[a] = sc.q_pos && a < sc.axes && ok ? static_cast<uint32_t>(sc.q_pos[static_cast<int64_t>(i) * sc.axes + a]) + kPosBias : 0u;
     return q;
 }
@@ -645,31 +683,63 @@ __device__ __forceinline__ void scan_documents(Marks& m, const int32_t* own, int
     }
 }
 
-// The next tile to visit after `t` (of tile0 .. tile1 - 1), tile1 when there is none. Marks of tiles past the last are
-// never set within a group of sixteen; groups past it are not read.
-__device__ __forceinline__ int next_tile(const Marks& m, bool marked, int t, int tile0, int tile1) {
-    ++t;
-    if (!marked) return t < tile1 ? t : tile1;
-    while (t < tile1) {
-        const int k = t - tile0;
-        if (k >= kWords * 64) return t;
-        const uint32_t u = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(m.any)[k >> 4]) >> (k & 15));
-        if (u) return t + __builtin_ctz(u);
-        t += 16 - (k & 15);
+// The order of a block's tiles: first those in which no pair needs a look (full), then the others, so that each kind has
+// a loop of its own. (One loop that chooses its body costs registers: where the bodies meet the compiler keeps two copies
+// of the sums.) Tiles full0 .. full1 - 1 are full as far as lengths and order go; with documents, those of them that the
+// marks say so.
+struct Walk {
+    int tile0, tile1, full0, full1;
+    bool marked;
+};
+struct Step {
+    int tile, rest;       // rest: 0 among the full tiles, 1 among the others
+
+    __device__ __forceinline__ bool done(const Walk& w) const { return tile >= w.tile1; }
+    __device__ __forceinline__ void find(const Walk& w, const Marks& m) {
+        int t = tile + 1;
+        if (!w.marked) {
+            if (rest) t = t >= w.full0 && t < w.full1 ? w.full1 : t;
+            else t = max(t, w.full0) < w.full1 ? max(t, w.full0) : w.tile1;
+            tile = t < w.tile1 ? t : w.tile1;
+            return;
+        }
+        tile = w.tile1;
+        while (t < w.tile1) {
+            const int k = t - w.tile0, first = t - (k & 15);
+            if (k >= kWords * 64) {
+                if (rest) tile = t;
+                return;
+            }
+            // sixteen tiles' marks; those past the last are never set
+            uint32_t any = __builtin_amdgcn_readfirstlane(reinterpret_cast<const uint16_t*>(m.any)[k >> 4]);
+            uint32_t full = __builtin_amdgcn_readfirstlane(reinterpret_cast<const uint16_t*>(m.full)[k >> 4]);
+            const int a = w.full0 - first, b = w.full1 - first;
+            full &= (a <= 0 ? ~0u : a >= 16 ? 0u : ~0u << a) & (b >= 16 ? ~0u : b <= 0 ? 0u : ~(~0u << b));
+            any = (rest ? any & ~full : full) >> (k & 15);
+            if (any) {
+                tile = t + __builtin_ctz(any);
+                return;
+            }
+            t = first + 16;
+        }
     }
-    return tile1;
-}
-__device__ __forceinline__ bool full_tile(const Marks& m, int k) {
-    return k < kWords * 64 && (__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(m.full)[k >> 4])) >> (k & 15) & 1);
-}
+    __device__ __forceinline__ void go(const Walk& w, const Marks& m) {
+        find(w, m);
+        if (tile >= w.tile1 && !rest) {
+            rest = 1;
+            tile = w.tile0 - 1;
+            find(w, m);
+        }
+    }
+};
 
 // What goes along with a key tile in LDS: coordinates and documents, ready to compare.
 struct Along {
-    uint32_t pos[WST_MAX_AXES][64];
+    uint32_t pos[kAxes][64];
     int doc[64];
 };
 
-// One thread's share of it on its way: t < 256 one coordinate, t < 64 one document.
+// One thread's share of it on its way: t < 192 one coordinate, t < 64 one document.
 struct AlongStage {
     uint32_t pos;
     int doc;
@@ -683,30 +753,45 @@ struct AlongStage {
         }
     }
     __device__ __forceinline__ void store(Along& al, const int32_t* p, const int32_t* d, int t) const {
-        if (p) al.pos[t >> 6][t & 63] = pos;
+        if (p && t < 64 * kAxes) al.pos[t >> 6][t & 63] = pos;
         if (d && t < 64) al.doc[t] = doc;
     }
 };
 
+// The kinds of scores a kernel is compiled for: CAP 0 or 1; BIAS 0 none, 1 by place, 2 by coordinates; 2 and 3 stand for
+// "as the call says". Branches on these inside the loop over tiles cost more than the branch: the compiler moves whole
+// tiles of registers where the ways meet (measured at 8192 x 8 heads x 128, no cap, no bias: 318 us with such branches).
+// float32, whose products take sixteen times as long, has the one general kernel.
+struct Kind {
+    bool cap, bias, coordinates;
+};
+template <int CAP, int BIAS>
+__device__ __forceinline__ Kind kind_of(const wst_attention_desc& d) {
+    Kind k;
+    k.cap = CAP == 2 ? d.cap > 0.f : CAP == 1;
+    k.bias = BIAS == 3 ? d.slopes != nullptr : BIAS != 0;
+    k.coordinates = BIAS == 3 ? d.q_pos != nullptr : BIAS == 2;
+    return k;
+}
+
 // Turns 32 x 32 dot products (rows: keys key0 + 32 sub .., column: the lane's query) into x of Shape, -inf where the
 // query does not see the key. GRAD: also the cap's slope and the distances.
-template <typename T, bool GRAD>
-__device__ __forceinline__ void scores(f32x16& x, const Shape& sh, float slope2, bool bias, const Scope& sc, const Query& q,
-                                       const Along& al, int key0, int sub, bool masked, f32x16& grad, f32x16& far) {
+template <typename T, bool GRAD, int MASK>
+__device__ __forceinline__ void scores(f32x16& x, const Kind& kind, const Shape& sh, float slope2, const Query& q, const Along& al,
+                                       int key0, int sub, f32x16& grad, f32x16& far) {
     const int h = (threadIdx.x & 63) >> 5;
-    if (sh.cap) sh.bend<T, GRAD>(x, grad);
-    if (bias) {
-        if (sc.q_pos) {
+    if (kind.cap) sh.bend<T, GRAD>(x, grad);
+    if (kind.bias) {
+        if (kind.coordinates) {
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 uint32_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
-                for (int a = 0; a < WST_MAX_AXES; ++a)
-                    if (a < sc.axes) {
-                        const u32x4 k = *reinterpret_cast<const u32x4*>(&al.pos[a][32 * sub + 8 * g + 4 * h]);
+                for (int a = 0; a < kAxes; ++a) {
+                    const u32x4 k = *reinterpret_cast<const u32x4*>(&al.pos[a][32 * sub + 8 * g + 4 * h]);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) sum[e] = away(q.pos[a], k[e], sum[e]);
-                    }
+                    for (int e = 0; e < 4; ++e) sum[e] = away(q.pos[a], k[e], sum[e]);
+                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float f = static_cast<float>(sum[e]);
@@ -724,14 +809,14 @@ __device__ __forceinline__ void scores(f32x16& x, const Shape& sh, float slope2,
             }
         }
     }
-    if (masked) {
+    if constexpr (MASK != 0) {
         const int rel = q.limit - (key0 + 32 * sub + 4 * h);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            if (sc.q_doc) {
+            if constexpr (MASK == 2) {
                 const i32x4 k = *reinterpret_cast<const i32x4*>(&al.doc[32 * sub + 8 * g + 4 * h]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[4 * g + e] = 8 * g + e < rel && k[e] == q.doc ? x[4 * g + e] : -INFINITY;
+                for (int e = 0; e < 4; ++e) x[4 * g + e] = ((8 * g + e < rel) & (k[e] == q.doc)) ? x[4 * g + e] : -INFINITY;
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[4 * g + e] = 8 * g + e < rel ? x[4 * g + e] : -INFINITY;
@@ -750,13 +835,28 @@ __device__ __forceinline__ bool not_finite(const f32x16 (&o)[DP / 32]) {
     return t != t;
 }
 
+// The order of LDS reads and matrix instructions in a product of STEPS instructions that take READS reads each: AHEAD
+// instructions' operands are read before the first, then each instruction is followed by the reads of a later one.
+// Left to itself the compiler reads either one operand at a time, and waits for each, or all of them, and spills.
+template <int STEPS, int READS, int AHEAD>
+__device__ __forceinline__ void paced() {
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * READS, 0);
+#pragma unroll
+    for (int i = 0; i < STEPS - AHEAD; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 constexpr int kBQ = 128, kBK = 64;
 
 // Forward pass: a block takes 128 queries of a head, 32 a wave, and walks the key tiles that any of them may see, keeping
 // the running maximum, sum and output of the softmax in registers; keys and values of a tile are shared through LDS.
 // The maximum moves only when a score exceeds it by 2^8 or more: weights up to 2^8 cost neither sums nor roundings
 // anything, and the output is rarely scaled.
-template <typename T, int DP>
+template <typename T, int DP, int CAP, int BIAS>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(AttnArgs a) {
     using L = Tile<T, DP>;
     __shared__ __attribute__((aligned(256))) char kt[2][kBK * L::kRowBytes], vt[2][kBK * L::kRowBytes];
@@ -771,6 +871,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(AttnAr
     const int h = static_cast<int>(bh % d.q_heads), kvh = h / (d.q_heads / d.k_heads);
     const Scope sc(d, b);
     const Shape sh = Shape::of<T>(d);
+    const Kind kind = kind_of<CAP, BIAS>(d);
     const int i = i0 + w * 32 + (lane & 31);
     const bool ok = i < d.q_len;
     const Query q = query_of(sc, i, ok);
@@ -803,46 +904,55 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(AttnAr
     // decide what to fetch) one tile earlier still
     auto fetch = [&](int n, int buf, const Along& with) {
         const int* doc = marked ? with.doc : nullptr;
-        kf.issue(kb + static_cast<int64_t>(n) * kBK * ks, ks, sc.length - n * kBK, doc, d.dim, kt[buf], t);
-        vf.issue(vb + static_cast<int64_t>(n) * kBK * vs, vs, sc.length - n * kBK, doc, d.dim, vt[buf], t);
+        const int left = sc.length - n * kBK;
+        const bool whole = !marked && d.dim == DP && left >= kBK;
+        kf.issue(kb + static_cast<int64_t>(n) * kBK * ks, whole, left, doc, kt[buf], t);
+        vf.issue(vb + static_cast<int64_t>(n) * kBK * vs, whole, left, doc, vt[buf], t);
     };
     AlongStage as{};
     if (marked) __syncthreads();       // the marks
-    int tile = next_tile(marks, marked, -1, 0, tiles), next = tile < tiles ? next_tile(marks, marked, tile, 0, tiles) : tiles;
+    const Walk walk{0, tiles, 0, open / kBK, marked};
+    Step cur{-1, 0};
+    cur.go(walk, marks);
+    Step next = cur;
+    if (!cur.done(walk)) next.go(walk, marks);
     if (along) {
-        if (tile < tiles) {
-            as.load(sc.k_pos, sc.k_doc, sc.axes, tile * kBK, sc.length, t);
+        if (!cur.done(walk)) {
+            as.load(sc.k_pos, sc.k_doc, sc.axes, cur.tile * kBK, sc.length, t);
             as.store(al[0], sc.k_pos, sc.k_doc, t);
         }
-        if (next < tiles) {
-            as.load(sc.k_pos, sc.k_doc, sc.axes, next * kBK, sc.length, t);
+        if (!next.done(walk)) {
+            as.load(sc.k_pos, sc.k_doc, sc.axes, next.tile * kBK, sc.length, t);
             as.store(al[1], sc.k_pos, sc.k_doc, t);
         }
     }
     __syncthreads();                   // documents and zeros
-    if (tile < tiles) fetch(tile, 0, al[0]);
+    if (!cur.done(walk)) fetch(cur.tile, 0, al[0]);
+    const typename L::Lane lanes = L::lane();
     int buf = 0, turn = 0;
-    while (tile < tiles) {
-        const int key0 = tile * kBK;
+    auto work = [&](auto mask) {       // a tile; compiled without, with the ordinary and with the documents' mask
+        constexpr int MASK = decltype(mask)::value;
+        const int key0 = cur.tile * kBK;
         const int turn1 = turn == 2 ? 0 : turn + 1, turn2 = turn1 == 2 ? 0 : turn1 + 1;
         arrived();
         __syncthreads();               // the tile is there, and nobody reads the other buffer any more
-        if (next < tiles) fetch(next, buf ^ 1, al[turn1]);
-        const int after = next < tiles ? next_tile(marks, marked, next, 0, tiles) : tiles;
-        if (along && after < tiles) as.load(sc.k_pos, sc.k_doc, sc.axes, after * kBK, sc.length, t);
-        const bool masked = key0 + kBK > open || (marked && !full_tile(marks, tile));
-        const char *kc = kt[buf], *vc = vt[buf];
-        f32x16 x[2], unused;
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            x[n] = zero16();
-#pragma unroll
-            for (int c = 0; c < DP / 16; ++c) x[n] = Mma<T>::mul(L::row_frag(kc, 32 * n, c), qf[c], x[n]);
+        Step after = next;
+        if (!next.done(walk)) {
+            fetch(next.tile, buf ^ 1, al[turn1]);
+            after.go(walk, marks);
+            if (along && !after.done(walk)) as.load(sc.k_pos, sc.k_doc, sc.axes, after.tile * kBK, sc.length, t);
         }
+        const typename L::Lane kc = lanes.at_tile(kt[buf]), vc = lanes.at_tile(vt[buf]);
+        f32x16 x[2] = {zero16(), zero16()}, unused;
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) x[n] = Mma<T>::mul(L::row_frag(kc, 32 * n, c), qf[c], x[n]);
+        if constexpr (sizeof(T) == 2) paced<DP / 8, 1, 4>();
         float top = -INFINITY;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            scores<T, false>(x[n], sh, slope2, d.slopes != nullptr, sc, q, al[turn], key0, n, masked, unused, unused);
+            scores<T, false, MASK>(x[n], kind, sh, slope2, q, al[turn], key0, n, unused, unused);
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = fmaxf(top, x[n][r]);
         }
@@ -857,6 +967,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(AttnAr
                 for (int r = 0; r < 16; ++r) o[k][r] *= f;
         }
         const float base = fmaxf(m, -3.0e38f);         // nothing seen yet: exp2(-inf) = 0 either way
+        Frag<T> p[2][2];
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
 #pragma unroll
@@ -864,19 +975,25 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(AttnAr
                 x[n][r] = __builtin_amdgcn_exp2f(fmaf(x[n][r], sh.mul, -base));
                 l += x[n][r];
             }
-            Frag<T> p[2];
-            to_frags<T>(x[n], p);
+            to_frags<T>(x[n], p[n]);
+        }
+        if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int k = 0; k < 2; ++k)
 #pragma unroll
-                for (int db = 0; db < DP / 32; ++db) o[db] = Mma<T>::mul(L::col_frag(vc, 32 * n + 16 * k, db), p[k], o[db]);
-        }
-        if (along && after < tiles) as.store(al[turn2], sc.k_pos, sc.k_doc, t);
-        tile = next;
+                for (int db = 0; db < DP / 32; ++db) o[db] = Mma<T>::mul(L::col_frag(vc, 32 * n + 16 * k, db), p[n][k], o[db]);
+        if constexpr (sizeof(T) == 2) paced<DP / 8, 2, 3>();
+        if (along && !after.done(walk)) as.store(al[turn2], sc.k_pos, sc.k_doc, t);
+        cur = next;
         next = after;
         buf ^= 1;
         turn = turn1;
-    }
+    };
+    while (!cur.done(walk) && !cur.rest) work(std::integral_constant<int, 0>{});
+    while (!cur.done(walk) && !marked) work(std::integral_constant<int, 1>{});
+    while (!cur.done(walk)) work(std::integral_constant<int, 2>{});
     l = halves_sum(l);
     const float inv = l == 0.f ? 0.f : 1.f / l;
     if (ok) {
@@ -901,7 +1018,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(AttnAr
 // Few queries over many keys: the queries of all heads that share a key head make up to 32 rows, and the keys are split
 // over blocks, and in a block over its waves, each of which walks its own tiles of 32 keys through its own part of LDS
 // with nothing to wait for. The parts are joined by their maxima and sums, in the block and then by k_attn_join.
-template <typename T, int DP>
+template <typename T, int DP, int CAP, int BIAS>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_split(AttnArgs a) {
     using L = Tile<T, DP>;
     constexpr int kTile = 32 * L::kRowBytes, kLd = DP + 4;
@@ -925,6 +1042,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_split(Attn
     const int h = kvh * group + static_cast<int>(ok ? r / d.q_len : 0);
     const Scope sc(d, b);
     const Shape sh = Shape::of<T>(d);
+    const Kind kind = kind_of<CAP, BIAS>(d);
     const Query q = query_of(sc, i, ok);
     const float slope2 = d.slopes ? d.slopes[h] * kLog2e : 0.f;
     Frag<T> qf[DP / 16];
@@ -956,7 +1074,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_split(Attn
     const T *kb = at<T>(d.k, d.k_strides, b, 0, kvh), *vb = at<T>(d.v, d.v_strides, b, 0, kvh);
     char *kt = pool + 2 * w * kTile, *vt = kt + kTile;
     Stage<T, DP, 32, 64> ks, vs;
-    uint32_t pos[WST_MAX_AXES];
+    uint32_t pos[kAxes];
     int doc = -2;
     auto fetch = [&](int key0) {
         ks.load(kb, d.k_strides[1], key0, sc.length, sc.k_doc, d.dim, lane);
@@ -964,7 +1082,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_split(Attn
         const int j = key0 + (lane & 31);
         if (sc.k_pos)
 #pragma unroll
-            for (int x = 0; x < WST_MAX_AXES; ++x)
+            for (int x = 0; x < kAxes; ++x)
                 pos[x] = x < sc.axes && j < sc.length ? static_cast<uint32_t>(sc.k_pos[static_cast<int64_t>(j) * sc.axes + x]) + kPosBias : 0u;
         if (sc.k_doc) {
             doc = j < sc.length ? sc.k_doc[j] : -2;
@@ -973,6 +1091,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_split(Attn
     };
     Along& mine = al[w >> 1];
     const int sub = w & 1;
+    const typename L::Lane lanes = L::lane();
     int g = wanted(g0);
     if (g < g1) fetch(g * 128 + 32 * w);
     while (g < g1) {
@@ -983,16 +1102,18 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_split(Attn
         if (lane < 32) {
             if (sc.k_pos)
 #pragma unroll
-                for (int x = 0; x < WST_MAX_AXES; ++x) mine.pos[x][32 * sub + lane] = pos[x];
+                for (int x = 0; x < kAxes; ++x) mine.pos[x][32 * sub + lane] = pos[x];
             mine.doc[32 * sub + lane] = doc;
         }
         __builtin_amdgcn_wave_barrier();
         const int next = wanted(g + 1);
         if (next < g1) fetch(next * 128 + 32 * w);
+        const typename L::Lane kc = lanes.at_tile(kt), vc = lanes.at_tile(vt);
         f32x16 s = zero16(), unused;
 #pragma unroll
-        for (int c = 0; c < DP / 16; ++c) s = Mma<T>::mul(L::row_frag(kt, 0, c), qf[c], s);
-        scores<T, false>(s, sh, slope2, d.slopes != nullptr, sc, q, mine, key0 - 32 * sub, sub, true, unused, unused);
+        for (int c = 0; c < DP / 16; ++c) s = Mma<T>::mul(L::row_frag(kc, 0, c), qf[c], s);
+        if (marked) scores<T, false, 2>(s, kind, sh, slope2, q, mine, key0 - 32 * sub, sub, unused, unused);
+        else scores<T, false, 1>(s, kind, sh, slope2, q, mine, key0 - 32 * sub, sub, unused, unused);
         float top = -INFINITY;
 #pragma unroll
         for (int x = 0; x < 16; ++x) top = fmaxf(top, s[x]);
@@ -1017,7 +1138,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_split(Attn
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
-            for (int db = 0; db < DP / 32; ++db) o[db] = Mma<T>::mul(L::col_frag(vt, 16 * k, db), p[k], o[db]);
+            for (int db = 0; db < DP / 32; ++db) o[db] = Mma<T>::mul(L::col_frag(vc, 16 * k, db), p[k], o[db]);
         g = next;
     }
     // join the waves
@@ -1125,7 +1246,7 @@ inline constexpr float kUp<f16> = 64.f;
 // dq, the slopes' shares and delta: walks the keys as the forward pass does. Scores come back as (keys x queries), so
 // their gradient is the operand of dq^T = k^T dz^T as it stands; keys are read from LDS both ways. delta goes in as the
 // product's starting value.
-template <typename T, int DP>
+template <typename T, int DP, int CAP, int BIAS>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(AttnArgs a) {
     using L = Tile<T, DP>;
     __shared__ __attribute__((aligned(256))) char kt[2][kBK * L::kRowBytes], vt[2][kBK * L::kRowBytes];
@@ -1140,6 +1261,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(AttnArg
     const int h = static_cast<int>(bh % d.q_heads), kvh = h / (d.q_heads / d.k_heads);
     const Scope sc(d, b);
     const Shape sh = Shape::of<T>(d);
+    const Kind kind = kind_of<CAP, BIAS>(d);
     const int i = i0 + w * 32 + (lane & 31);
     const int64_t row = (b * d.q_heads + h) * d.q_len + i;
     const bool ok = i < d.q_len;
@@ -1190,46 +1312,58 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(AttnArg
     // decide what to fetch) one tile earlier still
     auto fetch = [&](int n, int buf, const Along& with) {
         const int* doc = marked ? with.doc : nullptr;
-        kf.issue(kb + static_cast<int64_t>(n) * kBK * ks, ks, sc.length - n * kBK, doc, d.dim, kt[buf], t);
-        vf.issue(vb + static_cast<int64_t>(n) * kBK * vs, vs, sc.length - n * kBK, doc, d.dim, vt[buf], t);
+        const int left = sc.length - n * kBK;
+        const bool whole = !marked && d.dim == DP && left >= kBK;
+        kf.issue(kb + static_cast<int64_t>(n) * kBK * ks, whole, left, doc, kt[buf], t);
+        vf.issue(vb + static_cast<int64_t>(n) * kBK * vs, whole, left, doc, vt[buf], t);
     };
     AlongStage as{};
     if (marked) __syncthreads();       // the marks
-    int tile = next_tile(marks, marked, -1, 0, tiles), next = tile < tiles ? next_tile(marks, marked, tile, 0, tiles) : tiles;
+    const Walk walk{0, tiles, 0, open / kBK, marked};
+    Step cur{-1, 0};
+    cur.go(walk, marks);
+    Step next = cur;
+    if (!cur.done(walk)) next.go(walk, marks);
     if (along) {
-        if (tile < tiles) {
-            as.load(sc.k_pos, sc.k_doc, sc.axes, tile * kBK, sc.length, t);
+        if (!cur.done(walk)) {
+            as.load(sc.k_pos, sc.k_doc, sc.axes, cur.tile * kBK, sc.length, t);
             as.store(al[0], sc.k_pos, sc.k_doc, t);
         }
-        if (next < tiles) {
-            as.load(sc.k_pos, sc.k_doc, sc.axes, next * kBK, sc.length, t);
+        if (!next.done(walk)) {
+            as.load(sc.k_pos, sc.k_doc, sc.axes, next.tile * kBK, sc.length, t);
             as.store(al[1], sc.k_pos, sc.k_doc, t);
         }
     }
     __syncthreads();                   // documents and zeros
-    if (tile < tiles) fetch(tile, 0, al[0]);
+    if (!cur.done(walk)) fetch(cur.tile, 0, al[0]);
+    const typename L::Lane lanes = L::lane();
     int buf = 0, turn = 0;
-    while (tile < tiles) {
-        const int key0 = tile * kBK;
+    auto work = [&](auto mask) {       // a tile; compiled without, with the ordinary and with the documents' mask
+        constexpr int MASK = decltype(mask)::value;
+        const int key0 = cur.tile * kBK;
         const int turn1 = turn == 2 ? 0 : turn + 1, turn2 = turn1 == 2 ? 0 : turn1 + 1;
         arrived();
         __syncthreads();               // the tile is there, and nobody reads the other buffer any more
-        if (next < tiles) fetch(next, buf ^ 1, al[turn1]);
-        const int after = next < tiles ? next_tile(marks, marked, next, 0, tiles) : tiles;
-        if (along && after < tiles) as.load(sc.k_pos, sc.k_doc, sc.axes, after * kBK, sc.length, t);
-        const bool masked = key0 + kBK > open || (marked && !full_tile(marks, tile));
-        const char *kc = kt[buf], *vc = vt[buf];
+        Step after = next;
+        if (!next.done(walk)) {
+            fetch(next.tile, buf ^ 1, al[turn1]);
+            after.go(walk, marks);
+            if (along && !after.done(walk)) as.load(sc.k_pos, sc.k_doc, sc.axes, after.tile * kBK, sc.length, t);
+        }
+        const typename L::Lane kc = lanes.at_tile(kt[buf]), vc = lanes.at_tile(vt[buf]);
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             f32x16 x = zero16(), dp, grad, far;
 #pragma unroll
             for (int r = 0; r < 16; ++r) dp[r] = -delta;
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) x = Mma<T>::mul(L::row_frag(kc, 32 * n, c), qf[c], x);
-#pragma unroll
-            for (int c = 0; c < DP / 16; ++c) dp = Mma<T>::mul(L::row_frag(vc, 32 * n, c), df[c], dp);
-            scores<T, true>(x, sh, slope2, d.slopes != nullptr, sc, q, al[turn], key0, n, masked, grad, far);
-            if (masked) {     // a weight of 0 may meet a value that is not finite
+            for (int c = 0; c < DP / 16; ++c) {
+                x = Mma<T>::mul(L::row_frag(kc, 32 * n, c), qf[c], x);
+                dp = Mma<T>::mul(L::row_frag(vc, 32 * n, c), df[c], dp);
+            }
+            if constexpr (sizeof(T) == 2) paced<DP / 8, 1, 4>();
+            scores<T, true, MASK>(x, kind, sh, slope2, q, al[turn], key0, n, grad, far);
+            if constexpr (MASK != 0) {     // a weight of 0 may meet a value that is not finite
 #pragma unroll
                 for (int r = 0; r < 16; ++r) dp[r] = x[r] == -INFINITY ? 0.f : dp[r];
             }
@@ -1238,7 +1372,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(AttnArg
                 x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], sh.mul, base));
                 dp[r] *= x[r];
             }
-            if (a.slope_part) {
+            if (kind.bias && a.slope_part) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     pf = fmaf(x[r], far[r], pf);
@@ -1246,7 +1380,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(AttnArg
                     e1 = fmaf(dp[r], far[r], e1);
                 }
             }
-            if (sh.cap) {
+            if (kind.cap) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) dp[r] *= grad[r];
             }
@@ -1256,17 +1390,22 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(AttnArg
             }
             Frag<T> z[2];
             to_frags<T>(dp, z);
+            if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int k = 0; k < 2; ++k)
 #pragma unroll
                 for (int db = 0; db < DP / 32; ++db) dq[db] = Mma<T>::mul(L::col_frag(kc, 32 * n + 16 * k, db), z[k], dq[db]);
+            if constexpr (sizeof(T) == 2) paced<DP / 16, 2, 2>();
         }
-        if (along && after < tiles) as.store(al[turn2], sc.k_pos, sc.k_doc, t);
-        tile = next;
+        if (along && !after.done(walk)) as.store(al[turn2], sc.k_pos, sc.k_doc, t);
+        cur = next;
         next = after;
         buf ^= 1;
         turn = turn1;
-    }
+    };
+    while (!cur.done(walk) && !cur.rest) work(std::integral_constant<int, 0>{});
+    while (!cur.done(walk) && !marked) work(std::integral_constant<int, 1>{});
+    while (!cur.done(walk)) work(std::integral_constant<int, 2>{});
     const float mul = d.scale / kUp<T>;
     if (ok && a.g.dq) {
         T* out = const_cast<T*>(at<T>(a.g.dq, a.g.dq_strides, b, i, h));
@@ -1294,14 +1433,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(AttnArg
 struct Rows {
     float base[64], delta[64];     // add - lse log2 e; -delta
     int limit[64], doc[64], place[64];
-    uint32_t pos[WST_MAX_AXES][64];
+    uint32_t pos[kAxes][64];
 };
 
 // dk and dv: a block takes 128 keys of a key head, 32 a wave, held as operands in registers, and walks tiles of 64
 // queries of the heads that share it. Scores come as (queries x keys), one key a lane, so weights and score gradients
 // are the operands of dv^T = do^T p and dk^T = q^T dz as they stand. With few key tiles the walk is split in parts whose
 // sums k_attn_dkv_join adds in order.
-template <typename T, int DP>
+template <typename T, int DP, int CAP, int BIAS>
 __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64) ? 2 : 1) void k_attn_dkv(AttnArgs a) {
     using L = Tile<T, DP>;
     constexpr int kRows = 64;
@@ -1317,12 +1456,13 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64) ? 2 : 1) void k_a
     const int kvh = static_cast<int>(bh % d.k_heads);
     const Scope sc(d, b);
     const Shape sh = Shape::of<T>(d);
+    const Kind kind = kind_of<CAP, BIAS>(d);
     const int j = j0 + w * 32 + (lane & 31), q_len = static_cast<int>(d.q_len);
     const bool exists = j < d.k_len, ok = j < sc.length && (!sc.k_doc || sc.k_doc[j] >= 0);
     const int kdoc = ok && sc.k_doc ? sc.k_doc[j] : -2;
-    uint32_t kpos[WST_MAX_AXES];
+    uint32_t kpos[kAxes];
 #pragma unroll
-    for (int x = 0; x < WST_MAX_AXES; ++x)
+    for (int x = 0; x < kAxes; ++x)
         kpos[x] = ok && sc.k_pos && x < sc.axes ? static_cast<uint32_t>(sc.k_pos[static_cast<int64_t>(j) * sc.axes + x]) + kPosBias : 0u;
     Frag<T> kf[DP / 16], vf[DP / 16];
     row_frags<T, DP>(at<T>(d.k, d.k_strides, b, ok ? j : 0, kvh), ok, d.dim, kf);
@@ -1347,28 +1487,42 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64) ? 2 : 1) void k_a
     qfetch.init(qs, d.dim, t);
     dfetch.init(ds, d.dim, t);
 
-    // items of work: the visited tiles of the first head, then of the next, ...; this part takes every a.parts-th
+    // no pair needs a look when all rows and keys exist and the tile's first query sees the block's last key: from the
+    // first such tile to the last whole one
+    int full0 = tile0, full1 = keys == kBQ ? q_len / kRows : 0;
+    if (sc.causal && j0 + kBQ > sc.prefix) full0 = max(tile0, (max(j0 + kBQ - 1 - sc.shift, 0) + kRows - 1) / kRows);
+    const Walk walk{tile0, tiles, full0, max(full0, full1), marked};
+    // items of work: the full tiles of the first head, then of the next, ..., then the others; this part takes every
+    // a.parts-th
     struct Item {
-        int tile, g;
+        Step s;
+        int g;
     };
     auto step = [&](Item x) {
-        x.tile = next_tile(marks, marked, x.tile, tile0, tiles);
-        while (x.tile >= tiles && x.g + 1 < group) {
-            ++x.g;
-            x.tile = next_tile(marks, marked, tile0 - 1, tile0, tiles);
-            if (x.tile >= tiles) x.g = group;    // nothing to visit in any head
+        x.s.find(walk, marks);
+        for (int k = 0; x.s.done(walk) && k < 2 * group; ++k) {       // bounded: there may be no tile at all
+            if (x.g + 1 < group) {
+                ++x.g;
+            } else if (!x.s.rest) {
+                x.g = 0;
+                x.s.rest = 1;
+            } else {
+                break;
+            }
+            x.s.tile = tile0 - 1;
+            x.s.find(walk, marks);
         }
         return x;
     };
     auto skip = [&](Item x, int n) {
-        for (int k = 0; k < n && x.tile < tiles; ++k) x = step(x);
+        for (int k = 0; k < n && !x.s.done(walk); ++k) x = step(x);
         return x;
     };
     float r_base = -INFINITY, r_delta = 0.f;
     int r_limit = 0, r_doc = -1, r_place = 0;
     uint32_t r_pos = 0;
     auto load = [&](Item x) {
-        const int h = kvh * group + x.g, i = x.tile * kRows + (t & 63);
+        const int h = kvh * group + x.g, i = x.s.tile * kRows + (t & 63);
         const bool in = i < q_len;
         if (t < 64) {
             const int64_t row = (b * d.q_heads + h) * d.q_len + i;
@@ -1390,42 +1544,43 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64) ? 2 : 1) void k_a
             rw.doc[t] = r_doc;
             rw.place[t] = r_place;
         }
-        if (sc.q_pos) rw.pos[t >> 6][t & 63] = r_pos;
+        if (sc.q_pos && t < 64 * kAxes) rw.pos[t >> 6][t & 63] = r_pos;
     };
     auto fetch = [&](Item x, int buf, const Rows& with) {
-        const int h = kvh * group + x.g, i = x.tile * kRows;
+        const int h = kvh * group + x.g, i = x.s.tile * kRows;
         const int* doc = marked ? with.doc : nullptr;
-        qfetch.issue(at<T>(d.q, d.q_strides, b, i, h), qs, q_len - i, doc, d.dim, qt[buf], t);
-        dfetch.issue(at<T>(a.g.d_o, a.g.do_strides, b, i, h), ds, q_len - i, doc, d.dim, dt[buf], t);
+        const bool whole = !marked && d.dim == DP && q_len - i >= kRows;
+        qfetch.issue(at<T>(d.q, d.q_strides, b, i, h), whole, q_len - i, doc, qt[buf], t);
+        dfetch.issue(at<T>(a.g.d_o, a.g.do_strides, b, i, h), whole, q_len - i, doc, dt[buf], t);
     };
     if (marked) __syncthreads();       // the marks
-    Item cur{tile0 - 1, 0};
+    Item cur{{tile0 - 1, 0}, 0};
     if (tile0 < tiles) cur = skip(step(cur), part);
-    else cur.tile = tiles;
+    else cur.s.tile = tiles;
     Item nxt = skip(cur, a.parts);
-    if (cur.tile < tiles) {
+    if (!cur.s.done(walk)) {
         load(cur);
         put(rows[0]);
     }
-    if (nxt.tile < tiles) {
+    if (!nxt.s.done(walk)) {
         load(nxt);
         put(rows[1]);
     }
     __syncthreads();
-    if (cur.tile < tiles) fetch(cur, 0, rows[0]);
+    if (!cur.s.done(walk)) fetch(cur, 0, rows[0]);
+    const typename L::Lane lanes = L::lane();
     int buf = 0, turn = 0;
-    while (cur.tile < tiles) {
-        const int row0 = cur.tile * kRows, turn1 = turn == 2 ? 0 : turn + 1, turn2 = turn1 == 2 ? 0 : turn1 + 1;
-        const float slope2 = d.slopes ? d.slopes[kvh * group + cur.g] * kLog2e : 0.f;
+    auto work = [&](auto mask) {
+        constexpr int MASK = decltype(mask)::value;
+        const int turn1 = turn == 2 ? 0 : turn + 1, turn2 = turn1 == 2 ? 0 : turn1 + 1;
+        const float slope2 = kind.bias ? d.slopes[kvh * group + cur.g] * kLog2e : 0.f;
         const Rows& rw = rows[turn];
-        const char *qc = qt[buf], *dc = dt[buf];
+        const typename L::Lane qc = lanes.at_tile(qt[buf]), dc = lanes.at_tile(dt[buf]);
         arrived();
         __syncthreads();
-        if (nxt.tile < tiles) fetch(nxt, buf ^ 1, rows[turn1]);
+        if (!nxt.s.done(walk)) fetch(nxt, buf ^ 1, rows[turn1]);
         const Item after = skip(nxt, a.parts);
-        if (after.tile < tiles) load(after);
-        // no pair needs a look when all rows and keys exist and the tile's first query sees the block's last key
-        const bool masked = row0 + kRows > q_len || keys < kBQ || sc.limit(row0) < j0 + kBQ || (marked && !full_tile(marks, cur.tile - tile0));
+        if (!after.s.done(walk)) load(after);
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             f32x16 x = zero16(), dp, grad;
@@ -1439,21 +1594,20 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64) ? 2 : 1) void k_a
             for (int c = 0; c < DP / 16; ++c) x = Mma<T>::mul(L::row_frag(qc, 32 * n, c), kf[c], x);
 #pragma unroll
             for (int c = 0; c < DP / 16; ++c) dp = Mma<T>::mul(L::row_frag(dc, 32 * n, c), vf[c], dp);
-            if (sh.cap) sh.bend<T, true>(x, grad);
-            if (d.slopes) {
+            if (kind.cap) sh.bend<T, true>(x, grad);
+            if (kind.bias) {
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     const int y = 32 * n + 8 * c + 4 * hl;
                     float f[4];
-                    if (sc.q_pos) {
+                    if (kind.coordinates) {
                         uint32_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
-                        for (int k = 0; k < WST_MAX_AXES; ++k)
-                            if (k < sc.axes) {
-                                const u32x4 v = *reinterpret_cast<const u32x4*>(&rw.pos[k][y]);
+                        for (int k = 0; k < kAxes; ++k) {
+                            const u32x4 v = *reinterpret_cast<const u32x4*>(&rw.pos[k][y]);
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) sum[e] = away(kpos[k], v[e], sum[e]);
-                            }
+                            for (int e = 0; e < 4; ++e) sum[e] = away(kpos[k], v[e], sum[e]);
+                        }
 #pragma unroll
                         for (int e = 0; e < 4; ++e) f[e] = static_cast<float>(sum[e]);
                     } else {
@@ -1471,14 +1625,17 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64) ? 2 : 1) void k_a
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[4 * c + e] = __builtin_amdgcn_exp2f(fmaf(x[4 * c + e], sh.mul, v[e]));
             }
-            if (masked) {
+            if constexpr (MASK != 0) {
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     const int y = 32 * n + 8 * c + 4 * hl;
-                    const i32x4 lim = *reinterpret_cast<const i32x4*>(&rw.limit[y]), doc = *reinterpret_cast<const i32x4*>(&rw.doc[y]);
+                    const i32x4 lim = *reinterpret_cast<const i32x4*>(&rw.limit[y]);
+                    i32x4 doc;
+                    if constexpr (MASK == 2) doc = *reinterpret_cast<const i32x4*>(&rw.doc[y]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const bool see = j < lim[e] && (!marked || kdoc == doc[e]);
+                        bool see = j < lim[e];
+                        if constexpr (MASK == 2) see &= kdoc == doc[e];
                         x[4 * c + e] = see ? x[4 * c + e] : 0.f;
                         dp[4 * c + e] = see ? dp[4 * c + e] : 0.f;
                     }
@@ -1489,7 +1646,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64) ? 2 : 1) void k_a
                 x[r] *= kUp<T>;
                 dp[r] *= x[r];
             }
-            if (sh.cap) {
+            if (kind.cap) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) dp[r] *= grad[r];
             }
@@ -1504,12 +1661,15 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64) ? 2 : 1) void k_a
                     dk[db] = Mma<T>::mul(L::col_frag(qc, 32 * n + 16 * k, db), z[k], dk[db]);
                 }
         }
-        if (after.tile < tiles) put(rows[turn2]);
+        if (!after.s.done(walk)) put(rows[turn2]);
         cur = nxt;
         nxt = after;
         buf ^= 1;
         turn = turn1;
-    }
+    };
+    while (!cur.s.done(walk) && !cur.s.rest) work(std::integral_constant<int, 0>{});
+    while (!cur.s.done(walk) && !marked) work(std::integral_constant<int, 1>{});
+    while (!cur.s.done(walk)) work(std::integral_constant<int, 2>{});
     const float up = 1.f / kUp<T>, mul = d.scale * up;
     if (a.parts > 1) {
         if (exists) {
@@ -1591,18 +1751,16 @@ __global__ __launch_bounds__(256) void k_attn_dkv_join(AttnArgs a) {
     if (__ballot(bad)) row_dkv<T>(a, Scope(d, b), b, kvh, j, scratch[w][0], scratch[w][1]);
 }
 
-template <typename F>
-void with_width(int dim, F f) {
-    if (dim <= 32) f(std::integral_constant<int, 32>{});
-    else if (dim <= 64) f(std::integral_constant<int, 64>{});
-    else if (dim <= 96) f(std::integral_constant<int, 96>{});
-    else f(std::integral_constant<int, 128>{});
+template <typename T>
+void launch_delta(const AttnArgs& a, hipStream_t st) {
+    const dim3 rows(static_cast<unsigned>((a.d.q_len + 3) / 4), a.d.q_heads, static_cast<unsigned>(a.d.batch));
+    k_attn_delta<T><<<rows, dim3(256), 0, st>>>(a);
 }
 
-// Launches for one element type (wst_attention_t.hip).
-template <typename T>
+// Launches through matrix instructions, for one element type and padded width (wst_attention_t.hip).
+template <typename T, int DP>
 __attribute__((visibility("hidden"))) void attend(const AttnArgs& a, const AttnPlan& p, hipStream_t st);
-template <typename T>
+template <typename T, int DP>
 __attribute__((visibility("hidden"))) void attend_backward(const AttnArgs& a, const AttnPlan& p, hipStream_t st);
 
 }  // namespace wst_tok

@@ -22,6 +22,24 @@ __global__ __launch_bounds__(1024) void k_attn_slopes(const float* part, int64_t
     }
 }
 
+template <typename T>
+struct Tag {
+    using type = T;
+};
+template <typename F>
+void with_type(int dtype, F f) {
+    if (dtype == WST_F32) f(Tag<float>{});
+    else if (dtype == WST_BF16) f(Tag<bf16>{});
+    else f(Tag<f16>{});
+}
+template <typename F>
+void with_width(int dim, F f) {
+    if (dim <= 32) f(std::integral_constant<int, 32>{});
+    else if (dim <= 64) f(std::integral_constant<int, 64>{});
+    else if (dim <= 96) f(std::integral_constant<int, 96>{});
+    else f(std::integral_constant<int, 128>{});
+}
+
 int check(const wst_attention_desc* d) {
     if (!d) return fail(WST_ERR_INVALID, "attention: descriptor is NULL");
     if (d->batch < 0 || d->q_len < 0 || d->k_len < 0) return fail(WST_ERR_INVALID, "attention: negative size");
@@ -34,7 +52,8 @@ int check(const wst_attention_desc* d) {
     if (!(d->cap >= 0.f) || !std::isfinite(d->cap)) return fail(WST_ERR_INVALID, "attention: cap must be finite and not negative");
     if (!d->q_pos != !d->k_pos || !d->q_doc != !d->k_doc)
         return fail(WST_ERR_INVALID, "attention: positions and documents are given for queries and keys alike");
-    if (d->q_pos && (d->axes < 1 || d->axes > WST_MAX_AXES)) return fail(WST_ERR_INVALID, "attention: 1 to %d axes", WST_MAX_AXES);
+    if (d->q_pos && (d->axes < 1 || d->axes > WST_MAX_DISTANCE_AXES))
+        return fail(WST_ERR_INVALID, "attention: 1 to %d axes", WST_MAX_DISTANCE_AXES);
     if (d->prefix && !d->causal) return fail(WST_ERR_INVALID, "attention: a prefix needs causal order");
     if (d->batch > 65535 || d->q_heads > 65535) return fail(WST_ERR_UNSUPPORTED, "attention: more than 65535 sequences or heads");
     // blocks of every kernel are counted in 31 bits: a tile or row of each has at most eight splits or so in flight
@@ -118,9 +137,14 @@ int wst_attention_forward(const wst_attention_desc* d, void* o, float* lse, void
     a.part = static_cast<float*>(workspace);
     if (p.splits > 1) a.part_ml = a.part + static_cast<size_t>(p.splits) * rows_of(*d) * d->dim;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    if (d->dtype == WST_F32) attend<float>(a, p, st);
-    else if (d->dtype == WST_BF16) attend<bf16>(a, p, st);
-    else attend<f16>(a, p, st);
+    with_type(d->dtype, [&](auto t) {
+        using T = typename decltype(t)::type;
+        if (p.tiles) {
+            with_width(d->dim, [&](auto w) { attend<T, decltype(w)::value>(a, p, st); });
+        } else {
+            k_attn_rows<T><<<dim3(static_cast<unsigned>((d->q_len + 3) / 4), d->q_heads, static_cast<unsigned>(d->batch)), dim3(256), 0, st>>>(a);
+        }
+    });
     return launched("attention");
 }
 
@@ -146,9 +170,18 @@ int wst_attention_backward(const wst_attention_desc* d, const wst_attention_grad
     }
     a.part = rest;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    if (d->dtype == WST_F32) attend_backward<float>(a, p, st);
-    else if (d->dtype == WST_BF16) attend_backward<bf16>(a, p, st);
-    else attend_backward<f16>(a, p, st);
+    with_type(d->dtype, [&](auto t) {
+        using T = typename decltype(t)::type;
+        if (p.tiles) {
+            with_width(d->dim, [&](auto w) { attend_backward<T, decltype(w)::value>(a, p, st); });
+            return;
+        }
+        launch_delta<T>(a, st);
+        if (g->dq || g->dslopes)
+            k_attn_dq_rows<T><<<dim3(static_cast<unsigned>((d->q_len + 3) / 4), d->q_heads, static_cast<unsigned>(d->batch)), dim3(256), 0, st>>>(a);
+        if (g->dk || g->dv)
+            k_attn_dkv_rows<T><<<dim3(static_cast<unsigned>((d->k_len + 3) / 4), d->k_heads, static_cast<unsigned>(d->batch)), dim3(256), 0, st>>>(a);
+    });
     if (g->dslopes) k_attn_slopes<<<dim3(d->q_heads), dim3(1024), 0, st>>>(a.slope_part, d->batch * static_cast<int64_t>(a.slots), g->dslopes);
     return launched("attention backward");
 }

@@ -362,7 +362,7 @@ def attention(q, k, v, *, scale=None, cap=0.0, slopes=None, q_positions=None, k_
     With ``L = k_lengths[b]`` (default Tk) and ``place(i) = i + L - Tq``, query i scores key j as
     ``z = scale * q_i.k_j`` (scale defaults to ``D ** -0.5``), ``z = cap * tanh(z / cap)`` where ``cap > 0``, and
     ``z - slopes[h] * distance``: slopes float32 (H,); the distance is the sum over axes of
-    ``|q_positions[i] - k_positions[j]|`` (int32 (T, A) or (B, T, A), A <= 4, within +-2**29), or ``|place(i) - j|``
+    ``|q_positions[i] - k_positions[j]|`` (int32 (T, A) or (B, T, A), A <= 3, within +-2**29), or ``|place(i) - j|``
     without positions.  Key j is seen iff
 
     * ``j < L`` (k_lengths int32 (B,): keys behind are not read into any result), and
@@ -402,8 +402,8 @@ def attention(q, k, v, *, scale=None, cap=0.0, slopes=None, q_positions=None, k_
     A = 0
     if q_positions is not None and torch.is_tensor(q_positions):
         A = q_positions.shape[-1] if q_positions.dim() else 0
-        if not 1 <= A <= _lib.MAX_AXES:
-            raise RuntimeError(f"positions must have 1 to {_lib.MAX_AXES} axes")
+        if not 1 <= A <= _lib.MAX_DISTANCE_AXES:
+            raise RuntimeError(f"positions must have 1 to {_lib.MAX_DISTANCE_AXES} axes")
     s.q_pos = _check_side(q_positions, "q_positions", q, ((Tq, A), (B, Tq, A)))
     s.k_pos = _check_side(k_positions, "k_positions", q, ((Tk, A), (B, Tk, A)))
     s.q_doc = _check_side(q_documents, "q_documents", q, ((Tq,), (B, Tq)))
