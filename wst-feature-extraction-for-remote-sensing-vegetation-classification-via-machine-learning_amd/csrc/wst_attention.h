@@ -356,6 +356,13 @@ __device__ __forceinline__ f32x16 zero16() {
     return z;
 }
 
+__device__ __forceinline__ float sum16(const f32x16& x) {      // as a tree: a chain would wait for each addition
+    float s[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) s[r] = x[r] + x[r + 8];
+    return ((s[0] + s[4]) + (s[2] + s[6])) + ((s[1] + s[5]) + (s[3] + s[7]));
+}
+
 // max / sum with the lane 32 away
 __device__ __forceinline__ float halves_max(float x) {
     auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -487,6 +494,14 @@ __device__ __forceinline__ T* uniform(T* p) {
     const uint64_t x = reinterpret_cast<uint64_t>(p);
     return reinterpret_cast<T*>(static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x >> 32))) << 32 |
                                 static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x))));
+}
+
+// The kernel's arguments, read again: what only the end of a kernel needs then takes no scalar registers before (the
+// compiler loads all arguments at the start, and at about a hundred scalars spills them to vector lanes in the loop).
+__device__ __forceinline__ const AttnArgs& again() {
+    auto p = (const __attribute__((address_space(4))) AttnArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const AttnArgs*)p;
 }
 
 // N rows of a tensor straight into LDS, past the registers, by 256 threads: each lane names the 16 bytes it wants, and a
@@ -835,6 +850,11 @@ __device__ __forceinline__ bool not_finite(const f32x16 (&o)[DP / 32]) {
     return t != t;
 }
 
+template <typename T>
+inline constexpr float kSlack = 40.f;
+template <>
+inline constexpr float kSlack<f16> = 12.f;     // weights below 2^13 times the sum's rounding to float16
+
 // The order of LDS reads and matrix instructions in a product of STEPS instructions that take READS reads each: AHEAD
 // instructions' operands are read before the first, then each instruction is followed by the reads of a later one.
 // Left to itself the compiler reads either one operand at a time, and waits for each, or all of them, and spills.
@@ -854,8 +874,10 @@ constexpr int kBQ = 128, kBK = 64;
 
 // Forward pass: a block takes 128 queries of a head, 32 a wave, and walks the key tiles that any of them may see, keeping
 // the running maximum, sum and output of the softmax in registers; keys and values of a tile are shared through LDS.
-// The maximum moves only when a score exceeds it by 2^8 or more: weights up to 2^8 cost neither sums nor roundings
-// anything, and the output is rarely scaled.
+// The maximum is that of the first tile that shows the query anything, and stays as long as no score exceeds it by
+// kSlack powers of two: larger weights cost neither sums nor roundings anything, and the output is not scaled. A wave
+// that meets such a score goes on in loops that move the maximum with every tile. (As a branch inside the loop the
+// scaling costs as much when it is not taken: where the ways meet, the compiler copies all sums between registers.)
 template <typename T, int DP, int CAP, int BIAS>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(AttnArgs a) {
     using L = Tile<T, DP>;
@@ -930,51 +952,55 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(AttnAr
     if (!cur.done(walk)) fetch(cur.tile, 0, al[0]);
     const typename L::Lane lanes = L::lane();
     int buf = 0, turn = 0;
-    auto work = [&](auto mask) {       // a tile; compiled without, with the ordinary and with the documents' mask
-        constexpr int MASK = decltype(mask)::value;
-        const int key0 = cur.tile * kBK;
-        const int turn1 = turn == 2 ? 0 : turn + 1, turn2 = turn1 == 2 ? 0 : turn1 + 1;
+    int turn1 = 0, turn2 = 0;
+    Step after = next;
+    auto enter = [&]() {               // the tile is there, and nobody reads the other buffer any more
+        turn1 = turn == 2 ? 0 : turn + 1;
+        turn2 = turn1 == 2 ? 0 : turn1 + 1;
         arrived();
-        __syncthreads();               // the tile is there, and nobody reads the other buffer any more
-        Step after = next;
+        __syncthreads();
+        after = next;
         if (!next.done(walk)) {
             fetch(next.tile, buf ^ 1, al[turn1]);
             after.go(walk, marks);
             if (along && !after.done(walk)) as.load(sc.k_pos, sc.k_doc, sc.axes, after.tile * kBK, sc.length, t);
         }
-        const typename L::Lane kc = lanes.at_tile(kt[buf]), vc = lanes.at_tile(vt[buf]);
-        f32x16 x[2] = {zero16(), zero16()}, unused;
+    };
+    auto leave = [&]() {
+        if (along && !after.done(walk)) as.store(al[turn2], sc.k_pos, sc.k_doc, t);
+        cur = next;
+        next = after;
+        buf ^= 1;
+        turn = turn1;
+    };
+    // x of a tile, and the query's largest
+    auto look = [&](auto mask, f32x16 (&x)[2]) {
+        const typename L::Lane kc = lanes.at_tile(kt[buf]);
+        x[0] = x[1] = zero16();
 #pragma unroll
         for (int c = 0; c < DP / 16; ++c)
 #pragma unroll
             for (int n = 0; n < 2; ++n) x[n] = Mma<T>::mul(L::row_frag(kc, 32 * n, c), qf[c], x[n]);
         if constexpr (sizeof(T) == 2) paced<DP / 8, 1, 4>();
+        f32x16 unused;
         float top = -INFINITY;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            scores<T, false, MASK>(x[n], kind, sh, slope2, q, al[turn], key0, n, unused, unused);
+            scores<T, false, decltype(mask)::value>(x[n], kind, sh, slope2, q, al[turn], cur.tile * kBK, n, unused, unused);
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = fmaxf(top, x[n][r]);
         }
-        const float mn = halves_max(top) * sh.mul;
-        if (__ballot(mn > m + 8.f)) {
-            const float m1 = fmaxf(m, mn), f = __builtin_amdgcn_exp2f(m - fmaxf(m1, -3.0e38f));
-            m = m1;
-            l *= f;
-#pragma unroll
-            for (int k = 0; k < DP / 32; ++k)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[k][r] *= f;
-        }
+        return halves_max(top) * sh.mul;
+    };
+    auto add = [&](f32x16 (&x)[2]) {
+        const typename L::Lane vc = lanes.at_tile(vt[buf]);
         const float base = fmaxf(m, -3.0e38f);         // nothing seen yet: exp2(-inf) = 0 either way
         Frag<T> p[2][2];
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                x[n][r] = __builtin_amdgcn_exp2f(fmaf(x[n][r], sh.mul, -base));
-                l += x[n][r];
-            }
+            for (int r = 0; r < 16; ++r) x[n][r] = __builtin_amdgcn_exp2f(fmaf(x[n][r], sh.mul, -base));
+            l += sum16(x[n]);
             to_frags<T>(x[n], p[n]);
         }
         if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
@@ -985,34 +1011,59 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(AttnAr
 #pragma unroll
                 for (int db = 0; db < DP / 32; ++db) o[db] = Mma<T>::mul(L::col_frag(vc, 32 * n + 16 * k, db), p[n][k], o[db]);
         if constexpr (sizeof(T) == 2) paced<DP / 8, 2, 3>();
-        if (along && !after.done(walk)) as.store(al[turn2], sc.k_pos, sc.k_doc, t);
-        cur = next;
-        next = after;
-        buf ^= 1;
-        turn = turn1;
     };
-    while (!cur.done(walk) && !cur.rest) work(std::integral_constant<int, 0>{});
-    while (!cur.done(walk) && !marked) work(std::integral_constant<int, 1>{});
-    while (!cur.done(walk)) work(std::integral_constant<int, 2>{});
+    bool slow = false;                 // of the wave: a score has come that the maximum must move for
+    auto fast = [&](auto mask) {
+        enter();
+        f32x16 x[2];
+        const float mn = look(mask, x);
+        m = m == -INFINITY ? mn : m;
+        slow = __ballot(mn > m + kSlack<T>) != 0;
+        if (slow) return;
+        add(x);
+        leave();
+    };
+    bool entered = false;
+    auto careful = [&](auto mask) {
+        if (!entered) enter();
+        entered = false;
+        f32x16 x[2];
+        const float m1 = fmaxf(m, look(mask, x)), f = __builtin_amdgcn_exp2f(m - fmaxf(m1, -3.0e38f));
+        m = m1;
+        l *= f;
+#pragma unroll
+        for (int k = 0; k < DP / 32; ++k)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[k][r] *= f;
+        add(x);
+        leave();
+    };
+    while (!cur.done(walk) && !cur.rest && !slow) fast(std::integral_constant<int, 0>{});
+    while (!cur.done(walk) && !marked && !slow) fast(std::integral_constant<int, 1>{});
+    while (!cur.done(walk) && !slow) fast(std::integral_constant<int, 2>{});
+    entered = slow;
+    while (!cur.done(walk) && !marked) careful(std::integral_constant<int, 1>{});
+    while (!cur.done(walk)) careful(std::integral_constant<int, 2>{});
+    const AttnArgs& z = again();
     l = halves_sum(l);
     const float inv = l == 0.f ? 0.f : 1.f / l;
     if (ok) {
-        T* out = const_cast<T*>(at<T>(a.o, d.o_strides, b, i, h));
+        T* out = const_cast<T*>(at<T>(z.o, z.d.o_strides, b, i, h));
 #pragma unroll
         for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int c = 32 * db + 8 * g + 4 * hl;
                 const float v[4] = {o[db][4 * g] * inv, o[db][4 * g + 1] * inv, o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv};
-                if (c < d.dim) store<4>(out + c, v);
+                if (c < z.d.dim) store<4>(out + c, v);
             }
-        if (hl == 0 && a.lse) a.lse[(b * d.q_heads + h) * d.q_len + i] = l == 0.f ? -INFINITY : (m + sh.add) * kLn2 + logf(l);
+        if (hl == 0 && z.lse) z.lse[(b * z.d.q_heads + h) * z.d.q_len + i] = l == 0.f ? -INFINITY : (m + sh.add) * kLn2 + logf(l);
     }
     // A value that is not finite, of a key that some query of the wave does not see, has reached that query as 0 * inf:
     // the queries whose output is not finite are done over, key by key. In ordinary data there are none.
     uint64_t bad = __ballot(ok && not_finite<T, DP>(o));
     for (bad = (bad | bad >> 32) & 0xffffffffu; bad; bad &= bad - 1)
-        row_forward<T>(a, sc, b, h, i0 + w * 32 + __builtin_ctzll(bad), scratch[w]);
+        row_forward<T>(z, Scope(z.d, b), b, h, i0 + w * 32 + __builtin_ctzll(bad), scratch[w]);
 }
 
 // Few queries over many keys: the queries of all heads that share a key head make up to 32 rows, and the keys are split
@@ -1118,21 +1169,17 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_split(Attn
 #pragma unroll
         for (int x = 0; x < 16; ++x) top = fmaxf(top, s[x]);
         const float mn = halves_max(top) * sh.mul;
-        if (__ballot(mn > m + 8.f)) {
-            const float m1 = fmaxf(m, mn), f = __builtin_amdgcn_exp2f(m - fmaxf(m1, -3.0e38f));
-            m = m1;
-            l *= f;
+        const float m1 = fmaxf(m, mn), f = __builtin_amdgcn_exp2f(m - fmaxf(m1, -3.0e38f));
+        m = m1;
+        l *= f;
 #pragma unroll
-            for (int k = 0; k < DP / 32; ++k)
+        for (int k = 0; k < DP / 32; ++k)
 #pragma unroll
-                for (int x = 0; x < 16; ++x) o[k][x] *= f;
-        }
+            for (int x = 0; x < 16; ++x) o[k][x] *= f;
         const float base = fmaxf(m, -3.0e38f);
 #pragma unroll
-        for (int x = 0; x < 16; ++x) {
-            s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], sh.mul, -base));
-            l += s[x];
-        }
+        for (int x = 0; x < 16; ++x) s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], sh.mul, -base));
+        l += sum16(s);
         Frag<T> p[2];
         to_frags<T>(s, p);
 #pragma unroll
@@ -1302,6 +1349,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(AttnArg
     // The slopes' share, -sum ds far. delta comes from the rounded output, and its error would meet a mean distance: with
     // e = sum ds (0, were delta exact) the share is -(sum ds far - e sum p far).
     float pf = 0.f, e0 = 0.f, e1 = 0.f;
+    const bool slopes_too = a.slope_part != nullptr;
 
     const T *kb = at<T>(d.k, d.k_strides, b, 0, kvh), *vb = at<T>(d.v, d.v_strides, b, 0, kvh);
     const int64_t ks = d.k_strides[1], vs = d.v_strides[1];
@@ -1372,7 +1420,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(AttnArg
                 x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], sh.mul, base));
                 dp[r] *= x[r];
             }
-            if (kind.bias && a.slope_part) {
+            if (kind.bias && slopes_too) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     pf = fmaf(x[r], far[r], pf);
@@ -1406,26 +1454,27 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(AttnArg
     while (!cur.done(walk) && !cur.rest) work(std::integral_constant<int, 0>{});
     while (!cur.done(walk) && !marked) work(std::integral_constant<int, 1>{});
     while (!cur.done(walk)) work(std::integral_constant<int, 2>{});
-    const float mul = d.scale / kUp<T>;
-    if (ok && a.g.dq) {
-        T* out = const_cast<T*>(at<T>(a.g.dq, a.g.dq_strides, b, i, h));
+    const AttnArgs& z = again();
+    const float mul = z.d.scale / kUp<T>;
+    if (ok && z.g.dq) {
+        T* out = const_cast<T*>(at<T>(z.g.dq, z.g.dq_strides, b, i, h));
 #pragma unroll
         for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int c = 32 * db + 8 * g + 4 * hl;
                 const float v[4] = {dq[db][4 * g] * mul, dq[db][4 * g + 1] * mul, dq[db][4 * g + 2] * mul, dq[db][4 * g + 3] * mul};
-                if (c < d.dim) store<4>(out + c, v);
+                if (c < z.d.dim) store<4>(out + c, v);
             }
     }
-    if (a.slope_part) {
+    if (z.slope_part) {
         const float share = halves_sum(e0) * halves_sum(pf) - halves_sum(e1), sum = wave_sum(hl ? 0.f : share);
-        if (lane == 0) a.slope_part[(static_cast<int64_t>(h) * d.batch + b) * a.slots + qt * 4 + w] = sum;
+        if (lane == 0) z.slope_part[(static_cast<int64_t>(h) * z.d.batch + b) * z.slots + qt * 4 + w] = sum;
     }
     uint64_t bad = __ballot(ok && not_finite<T, DP>(dq));      // see k_attn_fwd
     for (bad = (bad | bad >> 32) & 0xffffffffu; bad; bad &= bad - 1) {
         __builtin_amdgcn_wave_barrier();
-        row_dq<T>(a, sc, b, h, i0 + w * 32 + __builtin_ctzll(bad), scratch[w][0], scratch[w][1]);
+        row_dq<T>(z, Scope(z.d, b), b, h, i0 + w * 32 + __builtin_ctzll(bad), scratch[w][0], scratch[w][1]);
     }
 }
 
@@ -1670,38 +1719,39 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64) ? 2 : 1) void k_a
     while (!cur.s.done(walk) && !cur.s.rest) work(std::integral_constant<int, 0>{});
     while (!cur.s.done(walk) && !marked) work(std::integral_constant<int, 1>{});
     while (!cur.s.done(walk)) work(std::integral_constant<int, 2>{});
-    const float up = 1.f / kUp<T>, mul = d.scale * up;
-    if (a.parts > 1) {
+    const AttnArgs& z = again();
+    const float up = 1.f / kUp<T>, mul = z.d.scale * up;
+    if (z.parts > 1) {
         if (exists) {
-            const int64_t row = ((static_cast<int64_t>(part) * d.batch + b) * d.k_heads + kvh) * d.k_len + j;
+            const int64_t row = ((static_cast<int64_t>(part) * z.d.batch + b) * z.d.k_heads + kvh) * z.d.k_len + j;
 #pragma unroll
             for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
                 for (int g4 = 0; g4 < 4; ++g4) {
                     const int x = 32 * db + 8 * g4 + 4 * hl;
-                    if (x < d.dim) {
+                    if (x < z.d.dim) {
                         float u[4], v[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             u[e] = dk[db][4 * g4 + e] * mul;
                             v[e] = dv[db][4 * g4 + e] * up;
                         }
-                        store<4>(a.part + (2 * row) * d.dim + x, u);
-                        store<4>(a.part + (2 * row + 1) * d.dim + x, v);
+                        store<4>(z.part + (2 * row) * z.d.dim + x, u);
+                        store<4>(z.part + (2 * row + 1) * z.d.dim + x, v);
                     }
                 }
         }
         return;
     }
     if (exists) {
-        T* out_k = a.g.dk ? const_cast<T*>(at<T>(a.g.dk, a.g.dk_strides, b, j, kvh)) : nullptr;
-        T* out_v = a.g.dv ? const_cast<T*>(at<T>(a.g.dv, a.g.dv_strides, b, j, kvh)) : nullptr;
+        T* out_k = z.g.dk ? const_cast<T*>(at<T>(z.g.dk, z.g.dk_strides, b, j, kvh)) : nullptr;
+        T* out_v = z.g.dv ? const_cast<T*>(at<T>(z.g.dv, z.g.dv_strides, b, j, kvh)) : nullptr;
 #pragma unroll
         for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
             for (int g4 = 0; g4 < 4; ++g4) {
                 const int x = 32 * db + 8 * g4 + 4 * hl;
-                if (x < d.dim) {
+                if (x < z.d.dim) {
                     float u[4], v[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -1716,7 +1766,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64) ? 2 : 1) void k_a
     uint64_t bad = __ballot(exists && (not_finite<T, DP>(dk) || not_finite<T, DP>(dv)));      // see k_attn_fwd
     for (bad = (bad | bad >> 32) & 0xffffffffu; bad; bad &= bad - 1) {
         __builtin_amdgcn_wave_barrier();
-        row_dkv<T>(a, sc, b, kvh, j0 + w * 32 + __builtin_ctzll(bad), scratch[w][0], scratch[w][1]);
+        row_dkv<T>(z, Scope(z.d, b), b, kvh, j0 + w * 32 + __builtin_ctzll(bad), scratch[w][0], scratch[w][1]);
     }
 }
 
