@@ -549,9 +549,9 @@ struct Fetch {
 };
 __device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
 
-template <int BYTES>
+template <int BYTES, int TH = 256>
 __device__ __forceinline__ void clear(char* p, int t) {
-    for (int i = t * 16; i < BYTES; i += 4096) *reinterpret_cast<u32x4*>(p + i) = u32x4{0, 0, 0, 0};
+    for (int i = t * 16; i < BYTES; i += TH * 16) *reinterpret_cast<u32x4*>(p + i) = u32x4{0, 0, 0, 0};
 }
 
 // Eight values of a row as an operand fragment, from memory; zero beyond the head or where the row is not to be read.
@@ -590,15 +590,16 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // product and mul = scale log2 e, so that scaling costs nothing beyond the subtraction of the maximum. Capped, with
 // e = exp(2 z / cap), tanh = 1 - 2 / (e + 1), x is -1 / (e + 1): the cap's slope is 1 - tanh^2 = -4 x (1 + x). Its error
 // of 2^-24 or two of the cap is below what 16-bit weights keep; float32 takes the library's tanh, good to an ulp. With a
-// bias x is the score itself, mul = 1. mul is never negative: a negative scale has turned q (or k) over before.
+// bias x is the score itself, mul = 1. For a maximum over x mul must not be negative: there a negative
+// scale turns q over instead (sign = false).
 struct Shape {
     float raw, mul, add;      // of the score before the bias
     float twice, turn;        // 2 |scale| log2 e / cap;  |scale| / cap
     bool cap;
     template <typename T>
-    static __device__ __forceinline__ Shape of(const wst_attention_desc& d) {
+    static __device__ __forceinline__ Shape of(const wst_attention_desc& d, bool sign = false) {
         Shape s;
-        const float scale = fabsf(d.scale);
+        const float scale = sign ? d.scale : fabsf(d.scale);
         s.cap = d.cap > 0.f;
         s.twice = s.cap ? 2.f * scale * kLog2e / d.cap : 0.f;
         s.turn = s.cap ? scale / d.cap : 0.f;
@@ -658,7 +659,7 @@ struct Marks {
 // own: the documents of the block's tokens own0 .. own0 + own_count - 1 (those below own_rows exist); other: of the tiles
 // tile0 .. tile1 - 1, tokens below other_rows. A wave takes sixteen tiles at a time, all loads on their way at once.
 __device__ __forceinline__ void scan_documents(Marks& m, const int32_t* own, int own0, int own_count, int own_rows,
-                                               const int32_t* other, int tile0, int tile1, int other_rows) {
+                                               const int32_t* other, int tile0, int tile1, int other_rows, int waves = 4) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     int lo = INT32_MAX, hi = -1;
     bool all = true;
@@ -678,7 +679,7 @@ __device__ __forceinline__ void scan_documents(Marks& m, const int32_t* own, int
     }
     const bool one = __all(all) && lo == hi;
     const int count = tile1 - tile0 < kWords * 64 ? tile1 - tile0 : kWords * 64;
-    for (int k0 = w * 16; k0 < count; k0 += 64) {
+    for (int k0 = w * 16; k0 < count; k0 += 16 * waves) {
         int v[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
@@ -1404,6 +1405,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(AttnArg
             f32x16 x = zero16(), dp, grad, far;
 #pragma unroll
             for (int r = 0; r < 16; ++r) dp[r] = -delta;
+            if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int c = 0; c < DP / 16; ++c) {
                 x = Mma<T>::mul(L::row_frag(kc, 32 * n, c), qf[c], x);
@@ -1485,26 +1487,38 @@ struct Rows {
     uint32_t pos[kAxes][64];
 };
 
-// dk and dv: a block takes 128 keys of a key head, 32 a wave, held as operands in registers, and walks tiles of 64
-// queries of the heads that share it. Scores come as (queries x keys), one key a lane, so weights and score gradients
-// are the operands of dv^T = do^T p and dk^T = q^T dz as they stand. With few key tiles the walk is split in parts whose
-// sums k_attn_dkv_join adds in order.
+// Threads of k_attn_dkv.
+template <typename T, int DP>
+constexpr int dkv_threads() { return sizeof(T) == 2 && DP > 64 ? 512 : 256; }
+
+// dk and dv: a block takes 128 keys of a key head, 32 a wave, and walks tiles of 64 queries of the heads that share it.
+// Scores come as (queries x keys), one key a lane, so weights and score gradients are the operands of dv^T = do^T p and
+// dk^T = q^T dz as they stand. With few key tiles the walk is split in parts whose sums k_attn_dkv_join adds in order.
+//
+// Heads up to 64 wide (and float32): four waves, keys and values held as operands in registers. Wider ones would then
+// leave room for one wave a SIMD, which waits for LDS most of its time (8192 x 8 heads x 128, cap and prefix: 870 us).
+// They take eight waves: keys and values stay in LDS, two waves share 32 keys and take half of each tile's queries, and
+// add their sums at the end.
 template <typename T, int DP, int CAP, int BIAS>
-__global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64) ? 2 : 1) void k_attn_dkv(AttnArgs a) {
+__global__ __launch_bounds__((dkv_threads<T, DP>()), sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnArgs a) {
     using L = Tile<T, DP>;
-    constexpr int kRows = 64;
-    __shared__ __attribute__((aligned(256))) char qt[2][kRows * L::kRowBytes], dt[2][kRows * L::kRowBytes];
+    constexpr int kRows = 64, TH = dkv_threads<T, DP>(), kTile = kRows * L::kRowBytes;
+    constexpr bool kWide = TH == 512;
+    constexpr int kOwn = kBQ * L::kRowBytes;                          // the block's keys (or values)
+    __shared__ __attribute__((aligned(256))) char pool[4 * kTile + (kWide ? 2 * kOwn : 0)];
+    char *qt = pool, *dt = pool + 2 * kTile, *kt = pool + 4 * kTile, *vt = kt + kOwn;
     __shared__ Rows rows[3];
     __shared__ Marks marks;
-    __shared__ float scratch[4][2][DP];
+    __shared__ float scratch[TH / 64][2][DP];
     const wst_attention_desc& d = a.d;
-    const int t = threadIdx.x, lane = t & 63, w = t >> 6, hl = lane >> 5, group = d.q_heads / d.k_heads;
+    const int t = threadIdx.x, lane = t & 63, w = (t >> 6) & 3, half = t >> 8, hl = lane >> 5;
+    const int group = d.q_heads / d.k_heads;
     const uint32_t cells = static_cast<uint32_t>(d.batch) * d.k_heads, bh = blockIdx.x % cells, part = blockIdx.y;
     const int j0 = static_cast<int>(blockIdx.x / cells) * kBQ;         // early keys are seen by most: first
     const int64_t b = bh / d.k_heads;
     const int kvh = static_cast<int>(bh % d.k_heads);
     const Scope sc(d, b);
-    const Shape sh = Shape::of<T>(d);
+    const Shape sh = Shape::of<T>(d, true);
     const Kind kind = kind_of<CAP, BIAS>(d);
     const int j = j0 + w * 32 + (lane & 31), q_len = static_cast<int>(d.q_len);
     const bool exists = j < d.k_len, ok = j < sc.length && (!sc.k_doc || sc.k_doc[j] >= 0);
@@ -1514,9 +1528,10 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64) ? 2 : 1) void k_a
     for (int x = 0; x < kAxes; ++x)
         kpos[x] = ok && sc.k_pos && x < sc.axes ? static_cast<uint32_t>(sc.k_pos[static_cast<int64_t>(j) * sc.axes + x]) + kPosBias : 0u;
     Frag<T> kf[DP / 16], vf[DP / 16];
-    row_frags<T, DP>(at<T>(d.k, d.k_strides, b, ok ? j : 0, kvh), ok, d.dim, kf);
-    row_frags<T, DP>(at<T>(d.v, d.v_strides, b, ok ? j : 0, kvh), ok, d.dim, vf);
-    if (d.scale < 0.f) negate<T, DP>(kf);
+    if constexpr (!kWide) {
+        row_frags<T, DP>(at<T>(d.k, d.k_strides, b, ok ? j : 0, kvh), ok, d.dim, kf);
+        row_frags<T, DP>(at<T>(d.v, d.v_strides, b, ok ? j : 0, kvh), ok, d.dim, vf);
+    }
     f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
     for (int k = 0; k < DP / 32; ++k) dk[k] = dv[k] = zero16();
@@ -1526,11 +1541,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64) ? 2 : 1) void k_a
     const int first = sc.causal && j0 >= sc.prefix ? max(j0 - sc.shift, 0) : 0;
     const int tile0 = first / kRows, tiles = keys > 0 ? nqt : 0;
     const bool marked = sc.q_doc != nullptr;
-    if (marked && tile0 < tiles) scan_documents(marks, sc.k_doc, j0, kBQ, sc.length, sc.q_doc, tile0, tiles, q_len);
-    if (marked || d.dim != DP || q_len % kRows) {
-        clear<sizeof(qt)>(&qt[0][0], t);
-        clear<sizeof(dt)>(&dt[0][0], t);
-    }
+    if (marked && tile0 < tiles) scan_documents(marks, sc.k_doc, j0, kBQ, sc.length, sc.q_doc, tile0, tiles, q_len, TH / 64);
+    if (marked || d.dim != DP || q_len % kRows || keys < kBQ) clear<sizeof(pool), TH>(pool, t);
     const int64_t qs = d.q_strides[1], ds = a.g.do_strides[1];
     Fetch<T, DP, kRows> qfetch, dfetch;
     qfetch.init(qs, d.dim, t);
@@ -1599,8 +1611,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64) ? 2 : 1) void k_a
         const int h = kvh * group + x.g, i = x.s.tile * kRows;
         const int* doc = marked ? with.doc : nullptr;
         const bool whole = !marked && d.dim == DP && q_len - i >= kRows;
-        qfetch.issue(at<T>(d.q, d.q_strides, b, i, h), whole, q_len - i, doc, qt[buf], t);
-        dfetch.issue(at<T>(a.g.d_o, a.g.do_strides, b, i, h), whole, q_len - i, doc, dt[buf], t);
+        if (kWide && half) return;
+        qfetch.issue(at<T>(d.q, d.q_strides, b, i, h), whole, q_len - i, doc, qt + buf * kTile, t);
+        dfetch.issue(at<T>(a.g.d_o, a.g.do_strides, b, i, h), whole, q_len - i, doc, dt + buf * kTile, t);
     };
     if (marked) __syncthreads();       // the marks
     Item cur{{tile0 - 1, 0}, 0};
@@ -1617,37 +1630,62 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64) ? 2 : 1) void k_a
     }
     __syncthreads();
     if (!cur.s.done(walk)) fetch(cur, 0, rows[0]);
+    if constexpr (kWide) {
+        if (!half && tiles) {
+            Fetch<T, DP, kBQ> own;
+            const bool whole = !marked && d.dim == DP && keys >= kBQ;
+            own.init(d.k_strides[1], d.dim, t);
+            own.issue(at<T>(d.k, d.k_strides, b, j0, kvh), whole, keys, marked ? sc.k_doc + j0 : nullptr, kt, t);
+            own.init(d.v_strides[1], d.dim, t);
+            own.issue(at<T>(d.v, d.v_strides, b, j0, kvh), whole, keys, marked ? sc.k_doc + j0 : nullptr, vt, t);
+        }
+    }
     const typename L::Lane lanes = L::lane();
+    const int row_half = kWide ? 32 * __builtin_amdgcn_readfirstlane(half) : 0;      // this wave's first row of a tile
     int buf = 0, turn = 0;
     auto work = [&](auto mask) {
         constexpr int MASK = decltype(mask)::value;
         const int turn1 = turn == 2 ? 0 : turn + 1, turn2 = turn1 == 2 ? 0 : turn1 + 1;
         const float slope2 = kind.bias ? d.slopes[kvh * group + cur.g] * kLog2e : 0.f;
         const Rows& rw = rows[turn];
-        const typename L::Lane qc = lanes.at_tile(qt[buf]), dc = lanes.at_tile(dt[buf]);
+        const typename L::Lane qc = lanes.at_tile(qt + buf * kTile + row_half * L::kRowBytes);
+        const typename L::Lane dc = lanes.at_tile(dt + buf * kTile + row_half * L::kRowBytes);
         arrived();
         __syncthreads();
         if (!nxt.s.done(walk)) fetch(nxt, buf ^ 1, rows[turn1]);
         const Item after = skip(nxt, a.parts);
         if (!after.s.done(walk)) load(after);
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
+        for (int n = 0; n < (kWide ? 1 : 2); ++n) {
             f32x16 x = zero16(), dp, grad;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                const f32x4 v = *reinterpret_cast<const f32x4*>(&rw.delta[32 * n + 8 * c + 4 * hl]);
+                const f32x4 v = *reinterpret_cast<const f32x4*>(&rw.delta[row_half + 32 * n + 8 * c + 4 * hl]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) dp[4 * c + e] = v[e];
             }
+            if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
+            if constexpr (kWide) {
+                const typename L::Lane kc = lanes.at_tile(kt + 32 * w * L::kRowBytes), vc = lanes.at_tile(vt + 32 * w * L::kRowBytes);
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) x = Mma<T>::mul(L::row_frag(qc, 32 * n, c), kf[c], x);
+                for (int c = 0; c < DP / 16; ++c) {
+                    x = Mma<T>::mul(L::row_frag(qc, 32 * n, c), L::row_frag(kc, 0, c), x);
+                    dp = Mma<T>::mul(L::row_frag(dc, 32 * n, c), L::row_frag(vc, 0, c), dp);
+                }
+                paced<DP / 8, 2, 3>();
+            } else {
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) dp = Mma<T>::mul(L::row_frag(dc, 32 * n, c), vf[c], dp);
+                for (int c = 0; c < DP / 16; ++c) {
+                    x = Mma<T>::mul(L::row_frag(qc, 32 * n, c), kf[c], x);
+                    dp = Mma<T>::mul(L::row_frag(dc, 32 * n, c), vf[c], dp);
+                }
+                if constexpr (sizeof(T) == 2) paced<DP / 8, 1, 6>();
+            }
             if (kind.cap) sh.bend<T, true>(x, grad);
             if (kind.bias) {
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    const int y = 32 * n + 8 * c + 4 * hl;
+                    const int y = row_half + 32 * n + 8 * c + 4 * hl;
                     float f[4];
                     if (kind.coordinates) {
                         uint32_t sum[4] = {0, 0, 0, 0};
@@ -1670,14 +1708,14 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64) ? 2 : 1) void k_a
             }
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                const f32x4 v = *reinterpret_cast<const f32x4*>(&rw.base[32 * n + 8 * c + 4 * hl]);
+                const f32x4 v = *reinterpret_cast<const f32x4*>(&rw.base[row_half + 32 * n + 8 * c + 4 * hl]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[4 * c + e] = __builtin_amdgcn_exp2f(fmaf(x[4 * c + e], sh.mul, v[e]));
             }
             if constexpr (MASK != 0) {
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    const int y = 32 * n + 8 * c + 4 * hl;
+                    const int y = row_half + 32 * n + 8 * c + 4 * hl;
                     const i32x4 lim = *reinterpret_cast<const i32x4*>(&rw.limit[y]);
                     i32x4 doc;
                     if constexpr (MASK == 2) doc = *reinterpret_cast<const i32x4*>(&rw.doc[y]);
@@ -1702,6 +1740,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64) ? 2 : 1) void k_a
             Frag<T> p[2], z[2];
             to_frags<T>(x, p);
             to_frags<T>(dp, z);
+            if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -1709,6 +1748,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64) ? 2 : 1) void k_a
                     dv[db] = Mma<T>::mul(L::col_frag(dc, 32 * n + 16 * k, db), p[k], dv[db]);
                     dk[db] = Mma<T>::mul(L::col_frag(qc, 32 * n + 16 * k, db), z[k], dk[db]);
                 }
+            if constexpr (sizeof(T) == 2) paced<DP / 8, 2, kWide ? 2 : 4>();
         }
         if (!after.s.done(walk)) put(rows[turn2]);
         cur = nxt;
@@ -1719,6 +1759,29 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64) ? 2 : 1) void k_a
     while (!cur.s.done(walk) && !cur.s.rest) work(std::integral_constant<int, 0>{});
     while (!cur.s.done(walk) && !marked) work(std::integral_constant<int, 1>{});
     while (!cur.s.done(walk)) work(std::integral_constant<int, 2>{});
+    if constexpr (kWide) {             // the second four waves hand their sums over, a lane its own registers
+        float* sums = reinterpret_cast<float*>(pool) + w * (DP * 64) + lane;
+        static_assert(sizeof(pool) >= 4 * DP * 64 * sizeof(float), "room for the sums");
+        __syncthreads();
+        if (half) {
+#pragma unroll
+            for (int k = 0; k < DP / 32; ++k)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    sums[(32 * k + 2 * r) * 64] = dk[k][r];
+                    sums[(32 * k + 2 * r + 1) * 64] = dv[k][r];
+                }
+        }
+        __syncthreads();
+        if (half) return;
+#pragma unroll
+        for (int k = 0; k < DP / 32; ++k)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                dk[k][r] += sums[(32 * k + 2 * r) * 64];
+                dv[k][r] += sums[(32 * k + 2 * r + 1) * 64];
+            }
+    }
     const AttnArgs& z = again();
     const float up = 1.f / kUp<T>, mul = z.d.scale * up;
     if (z.parts > 1) {
