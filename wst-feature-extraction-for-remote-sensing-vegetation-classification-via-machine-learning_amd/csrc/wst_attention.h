@@ -1667,12 +1667,24 @@ __global__ __launch_bounds__((dkv_threads<T, DP>()), sizeof(T) == 2 ? 2 : 1) voi
             if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
             if constexpr (kWide) {
                 const typename L::Lane kc = lanes.at_tile(kt + 32 * w * L::kRowBytes), vc = lanes.at_tile(vt + 32 * w * L::kRowBytes);
+                // one step's operands are read while the step before multiplies; said step by step, since with most
+                // registers taken the compiler does not follow paced()
+                Frag<T> f[2][4];
+                auto read = [&](int c) {
+                    f[c & 1][0] = L::row_frag(qc, 0, c);
+                    f[c & 1][1] = L::row_frag(kc, 0, c);
+                    f[c & 1][2] = L::row_frag(dc, 0, c);
+                    f[c & 1][3] = L::row_frag(vc, 0, c);
+                };
+                read(0);
 #pragma unroll
                 for (int c = 0; c < DP / 16; ++c) {
-                    x = Mma<T>::mul(L::row_frag(qc, 32 * n, c), L::row_frag(kc, 0, c), x);
-                    dp = Mma<T>::mul(L::row_frag(dc, 32 * n, c), L::row_frag(vc, 0, c), dp);
+                    if (c + 1 < DP / 16) read(c + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                    x = Mma<T>::mul(f[c & 1][0], f[c & 1][1], x);
+                    dp = Mma<T>::mul(f[c & 1][2], f[c & 1][3], dp);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                paced<DP / 8, 2, 3>();
             } else {
 #pragma unroll
                 for (int c = 0; c < DP / 16; ++c) {
@@ -1741,14 +1753,32 @@ __global__ __launch_bounds__((dkv_threads<T, DP>()), sizeof(T) == 2 ? 2 : 1) voi
             to_frags<T>(x, p);
             to_frags<T>(dp, z);
             if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
+            if constexpr (kWide) {
+                Frag<T> f[2][2];
+                auto read = [&](int c) {
+                    f[c & 1][0] = L::col_frag(dc, 16 * (c / (DP / 32)), c % (DP / 32));
+                    f[c & 1][1] = L::col_frag(qc, 16 * (c / (DP / 32)), c % (DP / 32));
+                };
+                read(0);
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-                for (int db = 0; db < DP / 32; ++db) {
-                    dv[db] = Mma<T>::mul(L::col_frag(dc, 32 * n + 16 * k, db), p[k], dv[db]);
-                    dk[db] = Mma<T>::mul(L::col_frag(qc, 32 * n + 16 * k, db), z[k], dk[db]);
+                for (int c = 0; c < DP / 16; ++c) {
+                    if (c + 1 < DP / 16) read(c + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                    const int k = c / (DP / 32), db = c % (DP / 32);
+                    dv[db] = Mma<T>::mul(f[c & 1][0], p[k], dv[db]);
+                    dk[db] = Mma<T>::mul(f[c & 1][1], z[k], dk[db]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-            if constexpr (sizeof(T) == 2) paced<DP / 8, 2, kWide ? 2 : 4>();
+            } else {
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int db = 0; db < DP / 32; ++db) {
+                        dv[db] = Mma<T>::mul(L::col_frag(dc, 32 * n + 16 * k, db), p[k], dv[db]);
+                        dk[db] = Mma<T>::mul(L::col_frag(qc, 32 * n + 16 * k, db), z[k], dk[db]);
+                    }
+                if constexpr (sizeof(T) == 2) paced<DP / 8, 2, 4>();
+            }
         }
         if (!after.s.done(walk)) put(rows[turn2]);
         cur = nxt;
