@@ -197,3 +197,14 @@ def test_attention_workspace_of_empty_sizes(sizes, dim):
     lib, need = _lib.load(), ctypes.c_size_t(1)
     for backward in (0, 1):
         assert lib.wst_attention_workspace(_attn(dim=dim, slopes=256, **sizes), backward, ctypes.byref(need)) == 0
+
+
+def test_packed_descriptors_match_the_structures():
+    for pack, kind in ((_lib.NORM_PACK, _lib.NormDesc), (_lib.ROTARY_PACK, _lib.RotaryDesc),
+                       (_lib.ATTENTION_PACK, _lib.AttentionDesc), (_lib.GRADS_PACK, _lib.AttentionGrads)):
+        assert pack.size == ctypes.sizeof(kind), kind
+    d = _lib.AttentionDesc.from_buffer_copy(_lib.ATTENTION_PACK.pack(*range(1, 30), 0.5, 2.0, *range(31, 37)))
+    assert (d.batch, d.k_len, d.v_strides[2], d.k_doc_stride, d.q, d.prefix, d.scale, d.q_heads, d.causal) == (
+        1, 3, 12, 19, 20, 29, 0.5, 31, 36)
+    r = _lib.RotaryDesc.from_buffer_copy(_lib.ROTARY_PACK.pack(*range(1, 15), 0.25, *range(16, 28)))
+    assert (r.tokens, r.k_out_strides[2], r.base, r.q_heads, r.sections[0], r.positions_shared) == (2, 14, 0.25, 16, 21, 27)

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 import numpy as np
@@ -110,6 +111,37 @@ class AttentionGrads(ctypes.Structure):
     """``wst_attention_grads``."""
     _fields_ = [(n, _PTR) for n in ("o", "d_o", "lse", "dq", "dk", "dv", "dslopes")] + \
                [(n, _STRIDES) for n in ("do_strides", "dq_strides", "dk_strides", "dv_strides")]
+
+
+# The descriptors as packed bytes: a call of a few microseconds should not spend as long on filling a Structure.
+NORM_PACK = struct.Struct("@9q3if")
+ROTARY_PACK = struct.Struct("@14qd12i")
+ATTENTION_PACK = struct.Struct("@19q10P2f6i")
+GRADS_PACK = struct.Struct("@7P12q")
+
+
+class TokenCalls:
+    """The token operators' entry points, taking packed descriptors."""
+
+    def __init__(self, lib):
+        b, p, sz, i = ctypes.c_char_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int
+        for name, types in (("wst_layer_norm_forward", [b] + [p] * 7), ("wst_layer_norm_workspace", [b, p]),
+                            ("wst_layer_norm_backward", [b] + [p] * 9 + [sz, p]), ("wst_rotary", [b] + [p] * 6),
+                            ("wst_attention_workspace", [b, i, p]), ("wst_attention_forward", [b] + [p] * 3 + [sz, p]),
+                            ("wst_attention_backward", [b, b, p, sz, p])):
+            fn = lib[name]                     # a function object of its own, beside the typed one
+            fn.restype, fn.argtypes = ctypes.c_int, types
+            setattr(self, name[4:], fn)
+
+
+_token_calls = None
+
+
+def token_calls() -> TokenCalls:
+    global _token_calls
+    if _token_calls is None:
+        _token_calls = TokenCalls(load())
+    return _token_calls
 
 
 class WSTError(RuntimeError):

@@ -17,7 +17,6 @@ from __future__ import annotations
 import ctypes
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .frontend import require_gpu
@@ -33,12 +32,12 @@ def _dtype_id(t, name):
 
 
 def _check_tensor(t, name, like=None):
-    if not torch.is_tensor(t):
+    if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a PyTorch Tensor.")
     if not t.is_cuda:
         require_gpu()
         raise RuntimeError(f"{name} must be on a ROCm GPU, not on {t.device}")
-    if like is not None and t.device != like.device:
+    if like is not None and t.get_device() != like.get_device():
         raise RuntimeError(f"{name} is on {t.device}, expected {like.device}")
 
 
@@ -48,14 +47,22 @@ def _check_ints(t, name, like):
         raise TypeError(f"{name} must be int32, not {t.dtype}")
 
 
-def _call(device, fn, *args):
+def _call(index, fn, *args):
     """Run a library call on the tensors' device and its current stream, and check the status."""
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if device.index == torch.cuda.current_device():
-        _lib.check_tokens(fn(*args, stream))
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if index == torch._C._cuda_getDevice():
+        code = fn(*args, stream)
     else:
-        with torch.cuda.device(device):
-            _lib.check_tokens(fn(*args, stream))
+        with torch.cuda.device(index):
+            code = fn(*args, stream)
+    if code:
+        _lib.check_tokens(code)
+
+
+def _first_order():
+    """Called by the backward passes: they have no backward pass of their own."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("the token operators have first-order gradients only")
 
 
 def _wants_grad(*tensors):
@@ -66,6 +73,8 @@ def _wants_grad(*tensors):
 def _token_view(x):
     """x (..., n) as (batch, points, n) strides the library reads, copied only when it has none."""
     n = x.shape[-1]
+    if x.is_contiguous():
+        return x, (1, x.numel() // n, n, 0, n, 1)
     lead = []                                   # (size, stride) of the leading dimensions, merged where adjacent
     for size, stride in zip(x.shape[:-1], x.stride()[:-1]):
         if size == 1:
@@ -85,7 +94,7 @@ def _token_view(x):
 
 def _norm_desc(view, dview, x, out_dtype, weight, bias, eps):
     w = weight if weight is not None else bias
-    return _lib.NormDesc(*view, *dview, DTYPES[x.dtype], DTYPES[out_dtype], 0 if w is None else DTYPES[w.dtype], eps)
+    return _lib.NORM_PACK.pack(*view, *dview, DTYPES[x.dtype], DTYPES[out_dtype], 0 if w is None else DTYPES[w.dtype], eps)
 
 
 def _ptr(t):
@@ -100,7 +109,7 @@ def _norm_forward(x, weight, bias, eps, out_dtype, stats):
         mean, rstd = torch.empty((2, view[0] * view[1]), dtype=torch.float32, device=x.device).unbind(0)
     if x.numel():
         d = _norm_desc(view, (0, 0, 0), x, out_dtype, weight, bias, eps)
-        _call(x.device, _lib.load().wst_layer_norm_forward, d, xs.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(),
+        _call(x.get_device(), _lib.token_calls().layer_norm_forward, d, xs.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(),
               _ptr(mean), _ptr(rstd))
     return y, xs, mean, rstd
 
@@ -115,8 +124,8 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        _first_order()
         xs, weight, mean, rstd = ctx.saved_tensors
         want_x, want_w, want_b = ctx.needs_input_grad[:3]
         dx = dw = db = None
@@ -139,12 +148,12 @@ class _LayerNorm(torch.autograd.Function):
             else:
                 dx = torch.empty(ctx.x_shape, dtype=xs.dtype, device=dev)
         dy = dy.contiguous()
-        d = _lib.NormDesc(*view, *dview, DTYPES[xs.dtype], DTYPES[dy.dtype],
-                          DTYPES[weight.dtype] if weight is not None else DTYPES[db.dtype] if want_b else 0, ctx.eps)
-        lib, need = _lib.load(), ctypes.c_size_t()
-        _lib.check_tokens(lib.wst_layer_norm_workspace(d, ctypes.byref(need)))
+        d = _lib.NORM_PACK.pack(*view, *dview, DTYPES[xs.dtype], DTYPES[dy.dtype],
+                                DTYPES[weight.dtype] if weight is not None else DTYPES[db.dtype] if want_b else 0, ctx.eps)
+        lib, need = _lib.token_calls(), ctypes.c_size_t()
+        _lib.check_tokens(lib.layer_norm_workspace(d, ctypes.byref(need)))
         ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
-        _call(dev, lib.wst_layer_norm_backward, d, xs.data_ptr(), _ptr(weight), dy.data_ptr(), mean.data_ptr(),
+        _call(xs.get_device(), lib.layer_norm_backward, d, xs.data_ptr(), _ptr(weight), dy.data_ptr(), mean.data_ptr(),
               rstd.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), ws.data_ptr(), need.value)
         return dx, dw, db, None, None
 
@@ -197,6 +206,8 @@ def _strides(t):
 
 def _lined_up(t):
     """t with rows the library can fetch 16 bytes at a time (heads of other widths go value by value anyway)."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
     t = _rows_of(t)
     if t.shape[-1] % 8 == 0:
         size = t.element_size()
@@ -207,6 +218,8 @@ def _lined_up(t):
 
 def _call_strides(t):
     """The strides of t for a call; of an axis of one entry, which is never stepped along, 0."""
+    if t.is_contiguous():
+        return t.stride()[:3]
     return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape))
 
 
@@ -219,9 +232,9 @@ def _rotate(q, k, positions, sections, base, interleaved, inverse):
         k = _rows_of(k)
         ko, Hk = torch.empty(k.shape, dtype=k.dtype, device=k.device), k.shape[2]
         ks, kos = _strides(k), _strides(ko)
-    d = _lib.RotaryDesc(B, T, _strides(q), ks, _strides(qo), kos, base, H, Hk, D, DTYPES[q.dtype], len(sections),
-                        sections, interleaved, inverse, positions.dim() == 2)
-    _call(q.device, _lib.load().wst_rotary, d, q.data_ptr(), qo.data_ptr(), _ptr(k), _ptr(ko), positions.data_ptr())
+    d = _lib.ROTARY_PACK.pack(B, T, *_strides(q), *ks, *_strides(qo), *kos, base, H, Hk, D, DTYPES[q.dtype], len(sections),
+                              *sections, *(0,) * (_lib.MAX_AXES - len(sections)), interleaved, inverse, positions.dim() == 2)
+    _call(q.get_device(), _lib.token_calls().rotary, d, q.data_ptr(), qo.data_ptr(), _ptr(k), _ptr(ko), positions.data_ptr())
     return qo, ko
 
 
@@ -234,8 +247,8 @@ class _Rotary(torch.autograd.Function):
         return qo if k is None else (qo, ko)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dq, dk=None):
+        _first_order()
         positions, = ctx.saved_tensors
         gq, gk = _rotate(dq, dk, positions, *ctx.how, 1)
         return gq, gk, None, None, None, None
@@ -293,17 +306,18 @@ def _attention_desc(q, k, v, slopes, side, o):
     def per_batch(t, dims):
         return 0 if t is None or t.dim() < dims else t.stride(0)
 
-    return _lib.AttentionDesc(
-        B, Tq, k.shape[1], _call_strides(q), _call_strides(k), _call_strides(v), _call_strides(o), per_batch(side.q_pos, 3),
+    return _lib.ATTENTION_PACK.pack(
+        B, Tq, k.shape[1], *_call_strides(q), *_call_strides(k), *_call_strides(v), *_strides(o), per_batch(side.q_pos, 3),
         per_batch(side.k_pos, 3), per_batch(side.q_doc, 2), per_batch(side.k_doc, 2), q.data_ptr(), k.data_ptr(),
-        v.data_ptr(), _ptr(slopes), _ptr(side.q_pos), _ptr(side.k_pos), _ptr(side.q_doc), _ptr(side.k_doc),
-        _ptr(side.k_lengths), _ptr(side.prefix), side.scale, side.cap, H, k.shape[2], D, DTYPES[q.dtype],
-        0 if side.q_pos is None else side.q_pos.shape[-1], side.causal)
+        v.data_ptr(), *(0 if t is None else t.data_ptr() for t in (slopes, side.q_pos, side.k_pos, side.q_doc, side.k_doc,
+                                                                    side.k_lengths, side.prefix)),
+        side.scale, side.cap, H, k.shape[2], D, DTYPES[q.dtype], 0 if side.q_pos is None else side.q_pos.shape[-1],
+        side.causal)
 
 
 def _workspace(d, backward, device):
-    lib, need = _lib.load(), ctypes.c_size_t()
-    _lib.check_tokens(lib.wst_attention_workspace(d, backward, ctypes.byref(need)))
+    need = ctypes.c_size_t()
+    _lib.check_tokens(_lib.token_calls().attention_workspace(d, backward, ctypes.byref(need)))
     return torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None, need.value
 
 
@@ -313,7 +327,7 @@ def _attend(q, k, v, slopes, side, want_lse):
     lse = torch.empty((B, H, Tq), dtype=torch.float32, device=q.device) if want_lse else None
     d = _attention_desc(q, k, v, slopes, side, o)
     ws, size = _workspace(d, 0, q.device)
-    _call(q.device, _lib.load().wst_attention_forward, d, o.data_ptr(), _ptr(lse), _ptr(ws), size)
+    _call(q.get_device(), _lib.token_calls().attention_forward, d, o.data_ptr(), _ptr(lse), _ptr(ws), size)
     return o, lse
 
 
@@ -327,8 +341,8 @@ class _Attention(torch.autograd.Function):
         return o, lse
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, do, _):
+        _first_order()
         q, k, v, slopes, o, lse = ctx.saved_tensors[:6]
         want = ctx.needs_input_grad
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if w else None
@@ -339,10 +353,11 @@ class _Attention(torch.autograd.Function):
         do = _lined_up(do)
         d = _attention_desc(q, k, v, slopes, ctx.side, o)
         none = (0, 0, 0)
-        g = _lib.AttentionGrads(o.data_ptr(), do.data_ptr(), lse.data_ptr(), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dslopes),
-                                _call_strides(do), *(none if t is None else _strides(t) for t in (dq, dk, dv)))
+        g = _lib.GRADS_PACK.pack(o.data_ptr(), do.data_ptr(), lse.data_ptr(),
+                                 *(0 if t is None else t.data_ptr() for t in (dq, dk, dv, dslopes)), *_call_strides(do),
+                                 *(s for t in (dq, dk, dv) for s in (none if t is None else t.stride()[:3])))
         ws, size = _workspace(d, 1, q.device)
-        _call(q.device, _lib.load().wst_attention_backward, d, g, _ptr(ws), size)
+        _call(q.get_device(), _lib.token_calls().attention_backward, d, g, _ptr(ws), size)
         return dq, dk, dv, dslopes, None
 
 
