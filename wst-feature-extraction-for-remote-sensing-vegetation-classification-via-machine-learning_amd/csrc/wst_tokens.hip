@@ -359,11 +359,11 @@ __global__ __launch_bounds__(1024) void k_norm_fold(NormArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------ layer norm, maps
-constexpr int kMapThreads = 512;
+constexpr int kMapThreads = 512, kMapBig = 1024;
 
 // Copies columns [k0, k0 + nk) of the points [p0, p0 + np) of one batch entry into LDS, turned: tile[p][k], row
-// stride ld. Global memory is read along the points (four at a time), LDS written so that the lanes of a wave, some
-// points by consecutive columns, fall on different banks (ld = 4 modulo 16).
+// stride ld. Global memory is read along the points (four at a time), LDS written so that the lanes of a wave, tp / 4
+// fours of points by 256 / tp consecutive columns, fall on different banks: ld = 64 / tp modulo 16 (map_ld).
 template <typename Tx>
 __device__ __forceinline__ void load_tile(const Tx* x, int64_t sn, int tp, int np, int64_t k0, int nk, float* tile, int ld) {
     const int quads = tp >> 2;                      // 4, 8 or 16
@@ -383,10 +383,15 @@ __device__ __forceinline__ void load_tile(const Tx* x, int64_t sn, int tp, int n
     }
 }
 
+// Values that a lane of a row in LDS stores at once: two of 16 bits or one of 32, so that reading LDS without bank
+// conflicts and writing memory in whole lines go together whatever ld is.
+template <typename Ty>
+constexpr int kPack = sizeof(Ty) == 2 ? 2 : 1;
+
 // A block takes tp points of one batch entry with all n values into LDS, then a wave takes a point at a time and
 // works as k_norm_rows does: one read of x, rows of y written whole. For n * 16 values that fit the LDS.
 template <typename Tx, typename Ty>
-__global__ __launch_bounds__(kMapThreads) void k_norm_maps(NormArgs a, int tp, int ld) {
+__global__ __launch_bounds__(kMapBig) void k_norm_maps(NormArgs a, int tp, int ld) {
     extern __shared__ float tile[];
     const int64_t tiles = (a.points + tp - 1) / tp;
     const int64_t b = blockIdx.x / tiles, p0 = (blockIdx.x - b * tiles) * tp;
@@ -395,23 +400,27 @@ __global__ __launch_bounds__(kMapThreads) void k_norm_maps(NormArgs a, int tp, i
     __syncthreads();
     const int lane = threadIdx.x & 63;
     const float count = static_cast<float>(n);
-    for (int p = threadIdx.x >> 6; p < np; p += kMapThreads / 64) {
+    for (int p = threadIdx.x >> 6; p < np; p += blockDim.x / 64) {
         const float* v = tile + p * ld;
         float s = 0.f;
+#pragma unroll 8
         for (int k = lane; k < n; k += 64) s += v[k];
         const float mu = wave_sum(s) / count;
         s = 0.f;
+#pragma unroll 8
         for (int k = lane; k < n; k += 64) s += (v[k] - mu) * (v[k] - mu);
         const float r = 1.f / sqrtf(wave_sum(s) / count + a.eps);
         const int64_t row = b * a.points + p0 + p;
         Ty* y = static_cast<Ty*>(a.y) + row * a.n;
-        for (int k = lane * 4; k < n; k += 256) {
-            float w[4], c[4], o[4];
-            load_w<4>(a.w, a.wdt, 1.f, k, n, w);
-            load_w<4>(a.b, a.wdt, 0.f, k, n, c);
+        constexpr int N = kPack<Ty>;
+#pragma unroll 4
+        for (int k = lane * N; k < n; k += 64 * N) {
+            float w[N], c[N], o[N];
+            load_w<N>(a.w, a.wdt, 1.f, k, n, w);
+            load_w<N>(a.b, a.wdt, 0.f, k, n, c);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = (v[k + e] - mu) * r * w[e] + c[e];   // ld is n rounded up to four or more
-            store_part<4>(y, k, n, o);
+            for (int e = 0; e < N; ++e) o[e] = (v[k + e] - mu) * r * w[e] + c[e];   // ld is n + 1 or more
+            store_part<N>(y, k, n, o);
         }
         if (lane == 0 && a.mean) {
             a.mean[row] = mu;
@@ -661,18 +670,20 @@ constexpr int kLdsMax = 160 * 1024;
 template <typename Tx, typename Ty>
 int norm_maps(const NormArgs& a, hipStream_t st) {
     const int64_t batch = a.rows / a.points;
-    // row stride in LDS: n rounded up to 4 modulo 16
-    const int64_t ld = (a.n + 11) / 16 * 16 + 4;
-    int tp = 64;                                               // as many points as let two blocks share a CU
-    while (tp > 16 && (tp / 2 >= a.points || tp * ld * 4 > kLdsMax / 2)) tp >>= 1;
-    const int64_t bytes = tp * ld * 4, tiles = (a.points + tp - 1) / tp;
+    // Points a block takes: 32 make whole lines of 128 bytes; fewer when there are no more, or when the block's share of
+    // the LDS would leave less than two to a CU.
+    auto map_ld = [&](int64_t tp) { return (a.n + 1 + 15 - 64 / tp) / 16 * 16 + 64 / tp; };   // n + 1 or more, 64 / tp modulo 16
+    int tp = 32;
+    while (tp > 16 && (tp / 2 >= a.points || tp * map_ld(tp) * 4 > kLdsMax / 2)) tp >>= 1;
+    const int64_t ld = map_ld(tp), bytes = tp * ld * 4, tiles = (a.points + tp - 1) / tp;
+    const int threads = bytes > kLdsMax / 4 ? kMapBig : kMapThreads;      // two blocks of sixteen waves, or four of eight
     if (bytes <= kLdsMax) {
         if (batch * tiles > 2147483647LL) return fail(WST_ERR_UNSUPPORTED, "layer norm: too many tiles");
         if (bytes > 64 * 1024 &&
             hipFuncSetAttribute(reinterpret_cast<const void*>(&k_norm_maps<Tx, Ty>), hipFuncAttributeMaxDynamicSharedMemorySize,
                                 kLdsMax) != hipSuccess)
             return launched("layer norm");
-        k_norm_maps<Tx, Ty><<<dim3(static_cast<unsigned>(batch * tiles)), dim3(kMapThreads), bytes, st>>>(a, tp, static_cast<int>(ld));
+        k_norm_maps<Tx, Ty><<<dim3(static_cast<unsigned>(batch * tiles)), dim3(threads), bytes, st>>>(a, tp, static_cast<int>(ld));
     } else {
         const int64_t all = batch * ((a.points + kPts - 1) / kPts);
         k_norm_maps_long<Tx, Ty><<<dim3(static_cast<unsigned>(all)), dim3(kMapThreads), 0, st>>>(a);
