@@ -92,6 +92,20 @@ __device__ __forceinline__ void load_part(const T* p, I col, I n, float (&v)[VEC
         for (int e = 0; e < VEC; ++e) v[e] = col + e < n ? static_cast<float>(p[col + e]) : 0.f;
     }
 }
+// the same, unconverted; WHOLE: n is a multiple of VEC
+template <int VEC, bool WHOLE, typename T>
+__device__ __forceinline__ Vec<T, VEC> load_raw(const T* p, int col, int n) {
+    Vec<T, VEC> v{};
+    if constexpr (WHOLE) {
+        if (col < n) __builtin_memcpy(&v, p + col, sizeof(v));
+    } else if (col + VEC <= n) {
+        __builtin_memcpy(&v, p + col, sizeof(v));
+    } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v.v[e] = col + e < n ? p[col + e] : static_cast<T>(0.f);
+    }
+    return v;
+}
 template <int VEC, typename T, typename I>
 __device__ __forceinline__ void store_part(T* p, I col, I n, const float (&v)[VEC]) {
     if (col + VEC <= n) {
@@ -206,7 +220,7 @@ __global__ __launch_bounds__(1024) void k_norm_long(NormArgs a) {
 // Backward pass of rows: a block walks rows block, block + groups, ...; dx leaves at once, the thread's columns of dw
 // and db stay in its registers until the block has added its waves' up and writes one partial row of each. The
 // partials are added in a fixed order (k_norm_fold), so results repeat bit for bit.
-template <typename Tx, typename Ty, int VEC, int CH, int TPR>
+template <typename Tx, typename Ty, int VEC, int CH, int TPR, bool WHOLE>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_bwd_rows(NormArgs a) {
     constexpr int kThreads = TPR > 256 ? TPR : 256, kRows = kThreads / TPR;
     __shared__ float slot[kThreads / 64 * 2];
@@ -220,18 +234,35 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_bwd_rows(NormArg
         for (int e = 0; e < VEC; ++e) dw[c][e] = db[c][e] = 0.f;
     }
     const float count = static_cast<float>(n);
-    for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + sub; row < a.rows;
-         row += static_cast<int64_t>(gridDim.x) * kRows) {
+    // the next row is on its way, as it is in memory, while one is worked on
+    Vec<Tx, VEC> xr[CH];
+    Vec<Ty, VEC> gr[CH];
+    float mu1 = 0.f, r1 = 0.f;
+    auto fetch = [&](int64_t row) {
         const Tx* x = static_cast<const Tx*>(a.x) + row_at(a, row, a.sb, a.sp);
         const Ty* dy = static_cast<const Ty*>(a.dy) + row * a.n;
-        const float mu = a.mean[row], r = a.rstd[row];
-        float h[CH][VEC], g[CH][VEC];
+        mu1 = a.mean[row];
+        r1 = a.rstd[row];
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            const int col = (c * TPR + t) * VEC;
-            load_part<VEC>(x, col, n, h[c]);
-            load_part<VEC>(dy, col, n, g[c]);
+            xr[c] = load_raw<VEC, WHOLE>(x, (c * TPR + t) * VEC, n);
+            gr[c] = load_raw<VEC, WHOLE>(dy, (c * TPR + t) * VEC, n);
         }
+    };
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+    int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + sub;
+    if (row < a.rows) fetch(row);
+    for (; row < a.rows; row += step) {
+        const float mu = mu1, r = r1;
+        float h[CH][VEC], g[CH][VEC];
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                h[c][e] = static_cast<float>(xr[c].v[e]);
+                g[c][e] = static_cast<float>(gr[c].v[e]);
+            }
+        if (row + step < a.rows) fetch(row + step);
         float s[2] = {0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < CH; ++c)
@@ -388,43 +419,86 @@ __device__ __forceinline__ void load_tile(const Tx* x, int64_t sn, int tp, int n
 template <typename Ty>
 constexpr int kPack = sizeof(Ty) == 2 ? 2 : 1;
 
-// A block takes tp points of one batch entry with all n values into LDS, then a wave takes a point at a time and
-// works as k_norm_rows does: one read of x, rows of y written whole. For n * 16 values that fit the LDS.
-template <typename Tx, typename Ty>
+// A block takes tp points of one batch entry with all n values into LDS, then a wave takes its points' mean and variance
+// out of LDS, and at last writes their rows whole, some columns at a time, with the weights of those columns in
+// registers: one read of x. For n * 16 values that fit the LDS. PLAIN: weight and bias are there, in float32 (a branch on
+// their type at every value took as many instructions as all else).
+template <typename Tx, typename Ty, bool PLAIN>
 __global__ __launch_bounds__(kMapBig) void k_norm_maps(NormArgs a, int tp, int ld) {
     extern __shared__ float tile[];
+    __shared__ float stat[2][32];
     const int64_t tiles = (a.points + tp - 1) / tp;
     const int64_t b = blockIdx.x / tiles, p0 = (blockIdx.x - b * tiles) * tp;
     const int np = static_cast<int>(a.points - p0 < tp ? a.points - p0 : tp), n = static_cast<int>(a.n);
     load_tile(static_cast<const Tx*>(a.x) + b * a.sb + p0, a.sn, tp, np, 0, n, tile, ld);
     __syncthreads();
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, w0 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const float count = static_cast<float>(n);
-    for (int p = threadIdx.x >> 6; p < np; p += blockDim.x / 64) {
-        const float* v = tile + p * ld;
+    const int64_t row0 = b * a.points + p0;
+    for (int p = w0; p < np; p += waves) {
+        const float* v = tile + p * ld + lane;
         float s = 0.f;
-#pragma unroll 8
-        for (int k = lane; k < n; k += 64) s += v[k];
+        int k = 0;
+        for (; k + 512 <= n; k += 512)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s += v[k + 64 * e];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (k + 64 * e + lane < n) s += v[k + 64 * e];
         const float mu = wave_sum(s) / count;
         s = 0.f;
-#pragma unroll 8
-        for (int k = lane; k < n; k += 64) s += (v[k] - mu) * (v[k] - mu);
-        const float r = 1.f / sqrtf(wave_sum(s) / count + a.eps);
-        const int64_t row = b * a.points + p0 + p;
-        Ty* y = static_cast<Ty*>(a.y) + row * a.n;
-        constexpr int N = kPack<Ty>;
-#pragma unroll 4
-        for (int k = lane * N; k < n; k += 64 * N) {
-            float w[N], c[N], o[N];
-            load_w<N>(a.w, a.wdt, 1.f, k, n, w);
-            load_w<N>(a.b, a.wdt, 0.f, k, n, c);
+        k = 0;
+        for (; k + 512 <= n; k += 512)
 #pragma unroll
-            for (int e = 0; e < N; ++e) o[e] = (v[k + e] - mu) * r * w[e] + c[e];   // ld is n + 1 or more
-            store_part<N>(y, k, n, o);
+            for (int e = 0; e < 8; ++e) {
+                const float d = v[k + 64 * e] - mu;
+                s = fmaf(d, d, s);
+            }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (k + 64 * e + lane < n) {
+                const float d = v[k + 64 * e] - mu;
+                s = fmaf(d, d, s);
+            }
+        const float r = 1.f / sqrtf(wave_sum(s) / count + a.eps);
+        if (lane == 0) {
+            stat[0][p] = mu;
+            stat[1][p] = r;
+            if (a.mean) {
+                a.mean[row0 + p] = mu;
+                a.rstd[row0 + p] = r;
+            }
         }
-        if (lane == 0 && a.mean) {
-            a.mean[row] = mu;
-            a.rstd[row] = r;
+    }
+    // a wave writes the rows whose statistics it took, so no barrier of the block
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    constexpr int N = kPack<Ty>, C = 4;      // C chunks of 64 N columns at a time
+    for (int k0 = lane * N; k0 < n; k0 += 64 * N * C) {
+        float w[C][N], c[C][N];
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            const int k = k0 + 64 * N * i;
+            if constexpr (PLAIN) {
+                load_part<N>(static_cast<const float*>(a.w), k, n, w[i]);
+                load_part<N>(static_cast<const float*>(a.b), k, n, c[i]);
+            } else {
+                load_w<N>(a.w, a.wdt, 1.f, k, n, w[i]);
+                load_w<N>(a.b, a.wdt, 0.f, k, n, c[i]);
+            }
+        }
+        for (int p = w0; p < np; p += waves) {
+            const float* v = tile + p * ld + k0;
+            const float mu = stat[0][p], r = stat[1][p];
+            Ty* y = static_cast<Ty*>(a.y) + (row0 + p) * a.n + k0;
+#pragma unroll
+            for (int i = 0; i < C; ++i) {
+                if (k0 + 64 * N * i >= n) break;
+                float o[N];
+#pragma unroll
+                for (int e = 0; e < N; ++e) o[e] = (v[64 * N * i + e] - mu) * r * w[i][e] + c[i][e];
+                store_part<N>(y + 64 * N * i, 0, n - k0 - 64 * N * i, o);
+            }
         }
     }
 }
@@ -524,37 +598,75 @@ __global__ __launch_bounds__(kMapThreads) void k_norm_bwd_maps_sums(NormArgs a) 
     }
 }
 
-// dx and the partial dw, db of maps: a block keeps 256 columns and walks tiles of 16 points, a thread half of the
-// points of one column. No sums over n are needed here, so any n goes through the same tile.
+constexpr int kBCols = 512, kBLd = 516;      // 516 = 4 modulo 16
+
+// dx and the partial dw, db of maps: a block keeps 512 columns and walks tiles of 16 points, a thread two columns and
+// half of the points; the next tile of x and dy is on its way while one is worked on. No sums over n are needed here, so
+// any n goes through the same tile.
 template <typename Tx, typename Ty>
 __global__ __launch_bounds__(kMapThreads) void k_norm_bwd_maps(NormArgs a) {
-    __shared__ float tile[kPts * kLd];
-    __shared__ float fold[2][kCols];
-    const int64_t k0 = static_cast<int64_t>(blockIdx.x) * kCols;
-    const int nk = static_cast<int>(a.n - k0 < kCols ? a.n - k0 : kCols);
-    const int k = threadIdx.x & (kCols - 1), half = threadIdx.x / kCols;
+    __shared__ float tile[kPts * kBLd];
+    __shared__ float fold[2][kBCols];
+    const int64_t k0 = static_cast<int64_t>(blockIdx.x) * kBCols;
+    const int nk = static_cast<int>(a.n - k0 < kBCols ? a.n - k0 : kBCols);
+    const int k = (threadIdx.x & 255) * 2, half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
     const int64_t tiles = (a.points + kPts - 1) / kPts, all = a.rows / a.points * tiles;
-    const float w = a.w && k < nk ? load_as(a.w, a.wdt, k0 + k) : 1.f;
-    float dw = 0.f, db = 0.f;
-    for (int64_t t = blockIdx.y; t < all; t += gridDim.y) {
+    const bool mine = k < nk, pair = k + 1 < nk;
+    const float w[2] = {a.w && mine ? load_as(a.w, a.wdt, k0 + k) : 1.f, a.w && pair ? load_as(a.w, a.wdt, k0 + k + 1) : 1.f};
+    float dw[2] = {0.f, 0.f}, db[2] = {0.f, 0.f};
+    // loading: a thread's four points q .. q + 3 of columns kq, kq + 128, ...
+    const int q = (threadIdx.x & 3) * 4, kq = threadIdx.x >> 2;
+    float xv[4][4];
+    Vec<Ty, 2> gv[kPts / 2];
+    auto fetch = [&](int64_t t) {
+        const int64_t b = t / tiles, p0 = (t - b * tiles) * kPts;
+        const int np = static_cast<int>(a.points - p0 < kPts ? a.points - p0 : kPts);
+        const Tx* x = static_cast<const Tx*>(a.x) + b * a.sb + p0 + q + (k0 + kq) * a.sn;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (q + 4 <= np && kq + 128 * i < nk) {
+                load<4>(x + 128 * i * a.sn, xv[i]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) xv[i][e] = q + e < np && kq + 128 * i < nk ? static_cast<float>(x[128 * i * a.sn + e]) : 0.f;
+            }
+        }
+        const Ty* dy = static_cast<const Ty*>(a.dy) + (b * a.points + p0) * a.n + k0 + k;
+#pragma unroll
+        for (int i = 0; i < kPts / 2; ++i) {
+            const int p = half * (kPts / 2) + i;
+            if (p < np && pair) __builtin_memcpy(&gv[i], dy + p * a.n, sizeof(gv[i]));
+            else gv[i] = Vec<Ty, 2>{{p < np && mine ? dy[p * a.n] : static_cast<Ty>(0.f), static_cast<Ty>(0.f)}};
+        }
+    };
+    int64_t t = blockIdx.y;
+    if (t < all) fetch(t);
+    for (; t < all; t += gridDim.y) {
         const int64_t b = t / tiles, p0 = (t - b * tiles) * kPts;
         const int np = static_cast<int>(a.points - p0 < kPts ? a.points - p0 : kPts);
         __syncthreads();
-        load_tile(static_cast<const Tx*>(a.x) + b * a.sb + p0, a.sn, kPts, np, k0, nk, tile, kLd);
-        __syncthreads();
-        const int64_t row0 = b * a.points + p0;
-        if (k < nk) {
-            const Ty* dy = static_cast<const Ty*>(a.dy) + row0 * a.n + k0 + k;
 #pragma unroll
-            for (int i = 0; i < kPts / 2; ++i) {
-                const int p = half * (kPts / 2) + i;
-                if (p < np) {
-                    const float r = a.rstd[row0 + p];
-                    const float h = (tile[p * kLd + k] - a.mean[row0 + p]) * r;
-                    const float g = static_cast<float>(dy[p * a.n]);
-                    dw += g * h;
-                    db += g;
-                    if (a.dx) tile[p * kLd + k] = r * (g * w - a.c[2 * (row0 + p)] - h * a.c[2 * (row0 + p) + 1]);
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) tile[(q + e) * kBLd + kq + 128 * i] = xv[i][e];
+        Vec<Ty, 2> now[kPts / 2];
+#pragma unroll
+        for (int i = 0; i < kPts / 2; ++i) now[i] = gv[i];
+        __syncthreads();
+        if (t + gridDim.y < all) fetch(t + gridDim.y);
+        const int64_t row0 = b * a.points + p0;
+#pragma unroll
+        for (int i = 0; i < kPts / 2; ++i) {
+            const int p = half * (kPts / 2) + i;
+            if (p < np) {          // uniform
+                const float r = a.rstd[row0 + p], mu = a.mean[row0 + p];
+                float* v = tile + p * kBLd + k;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float h = (v[e] - mu) * r, g = static_cast<float>(now[i].v[e]);
+                    dw[e] = fmaf(g, h, dw[e]);
+                    db[e] += g;
+                    if (a.dx) v[e] = r * (g * w[e] - a.c[2 * (row0 + p)] - h * a.c[2 * (row0 + p) + 1]);
                 }
             }
         }
@@ -563,20 +675,26 @@ __global__ __launch_bounds__(kMapThreads) void k_norm_bwd_maps(NormArgs a) {
             Tx* dx = static_cast<Tx*>(a.dx) + b * a.db_ + p0 * a.dp_;
             for (int i = threadIdx.x; i < kPts * nk; i += kMapThreads) {
                 const int p = i & (kPts - 1), kk = i / kPts;
-                if (p < np) dx[(k0 + kk) * a.dn_ + p * a.dp_] = static_cast<Tx>(tile[p * kLd + kk]);
+                if (p < np) dx[(k0 + kk) * a.dn_ + p * a.dp_] = static_cast<Tx>(tile[p * kBLd + kk]);
             }
         }
     }
     if (!a.part) return;
-    if (half) {
-        fold[0][k] = dw;
-        fold[1][k] = db;
+    if (half && mine) {
+        fold[0][k] = dw[0];
+        fold[1][k] = db[0];
+        fold[0][k + 1] = dw[1];
+        fold[1][k + 1] = db[1];
     }
     __syncthreads();
-    if (!half && k < nk) {
+    if (!half && mine) {
         float* part = a.part + static_cast<int64_t>(blockIdx.y) * 2 * a.n + k0 + k;
-        part[0] = dw + fold[0][k];
-        part[a.n] = db + fold[1][k];
+        part[0] = dw[0] + fold[0][k];
+        part[a.n] = db[0] + fold[1][k];
+        if (pair) {
+            part[1] = dw[1] + fold[0][k + 1];
+            part[a.n + 1] = db[1] + fold[1][k + 1];
+        }
     }
 }
 
@@ -630,13 +748,13 @@ constexpr int64_t kRegRows = 8192;          // longest rows whose backward pass 
 int norm_groups(const wst_norm_desc& d) {
     const int64_t rows = d.batch * d.points;
     if (as_maps(d)) {
-        const int64_t tiles = d.batch * ((d.points + kPts - 1) / kPts), cols = (d.n + kCols - 1) / kCols;
+        const int64_t tiles = d.batch * ((d.points + kPts - 1) / kPts), cols = (d.n + kBCols - 1) / kBCols;
         int64_t g = (1024 + cols - 1) / cols;                    // about four blocks a CU
         if (g > kGroups) g = kGroups;
         return static_cast<int>(g < tiles ? g : tiles);
     }
     if (d.n > kRegRows) return static_cast<int>(rows < 64 ? rows : 64);
-    const int64_t blocks = d.n <= 2048 ? (rows + 3) / 4 : rows;  // four rows a block up to 2048 values
+    const int64_t blocks = d.n <= 1024 ? (rows + 3) / 4 : rows;  // four rows a block up to 1024 values
     return static_cast<int>(blocks < kGroups ? blocks : kGroups);
 }
 
@@ -672,18 +790,21 @@ int norm_maps(const NormArgs& a, hipStream_t st) {
     const int64_t batch = a.rows / a.points;
     // Points a block takes: 32 make whole lines of 128 bytes; fewer when there are no more, or when the block's share of
     // the LDS would leave less than two to a CU.
-    auto map_ld = [&](int64_t tp) { return (a.n + 1 + 15 - 64 / tp) / 16 * 16 + 64 / tp; };   // n + 1 or more, 64 / tp modulo 16
+    // ld: n + 1 or more (a pair may end behind the last column), 64 / tp modulo 16
+    auto map_ld = [&](int64_t tp) { return (a.n + 1 + 15 - 64 / tp) / 16 * 16 + 64 / tp; };
     int tp = 32;
-    while (tp > 16 && (tp / 2 >= a.points || tp * map_ld(tp) * 4 > kLdsMax / 2)) tp >>= 1;
+    while (tp > 16 && (tp / 2 >= a.points || tp * map_ld(tp) * 4 > kLdsMax / 2 - 512)) tp >>= 1;
     const int64_t ld = map_ld(tp), bytes = tp * ld * 4, tiles = (a.points + tp - 1) / tp;
     const int threads = bytes > kLdsMax / 4 ? kMapBig : kMapThreads;      // two blocks of sixteen waves, or four of eight
-    if (bytes <= kLdsMax) {
+    if (bytes <= kLdsMax - 1024) {
         if (batch * tiles > 2147483647LL) return fail(WST_ERR_UNSUPPORTED, "layer norm: too many tiles");
-        if (bytes > 64 * 1024 &&
-            hipFuncSetAttribute(reinterpret_cast<const void*>(&k_norm_maps<Tx, Ty>), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                kLdsMax) != hipSuccess)
+        const bool plain = a.w && a.b && a.wdt == WST_F32;
+        const void* kernel = plain ? reinterpret_cast<const void*>(&k_norm_maps<Tx, Ty, true>) : reinterpret_cast<const void*>(&k_norm_maps<Tx, Ty, false>);
+        if (bytes > 64 * 1024 && hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsMax - 1024) != hipSuccess)
             return launched("layer norm");
-        k_norm_maps<Tx, Ty><<<dim3(static_cast<unsigned>(batch * tiles)), dim3(threads), bytes, st>>>(a, tp, static_cast<int>(ld));
+        const dim3 grid(static_cast<unsigned>(batch * tiles)), block(threads);
+        if (plain) k_norm_maps<Tx, Ty, true><<<grid, block, bytes, st>>>(a, tp, static_cast<int>(ld));
+        else k_norm_maps<Tx, Ty, false><<<grid, block, bytes, st>>>(a, tp, static_cast<int>(ld));
     } else {
         const int64_t all = batch * ((a.points + kPts - 1) / kPts);
         k_norm_maps_long<Tx, Ty><<<dim3(static_cast<unsigned>(all)), dim3(kMapThreads), 0, st>>>(a);
@@ -691,17 +812,23 @@ int norm_maps(const NormArgs& a, hipStream_t st) {
     return WST_OK;
 }
 
-template <typename Tx, typename Ty>
-void norm_bwd_rows(const NormArgs& a, hipStream_t st) {
+template <typename Tx, typename Ty, bool WHOLE>
+void norm_bwd_regs(const NormArgs& a, hipStream_t st) {
     const int chunks = static_cast<int>((a.n + 255) / 256);
     const dim3 g(static_cast<unsigned>(a.groups));
-    if (chunks <= 8) {
-        if (chunks <= 1) k_norm_bwd_rows<Tx, Ty, 4, 1, 64><<<g, dim3(256), 0, st>>>(a);
-        else if (chunks <= 2) k_norm_bwd_rows<Tx, Ty, 4, 2, 64><<<g, dim3(256), 0, st>>>(a);
-        else if (chunks <= 4) k_norm_bwd_rows<Tx, Ty, 4, 4, 64><<<g, dim3(256), 0, st>>>(a);
-        else k_norm_bwd_rows<Tx, Ty, 4, 8, 64><<<g, dim3(256), 0, st>>>(a);
-    } else if (a.n <= kRegRows) {
-        k_norm_bwd_rows<Tx, Ty, 4, 4, 512><<<g, dim3(512), 0, st>>>(a);
+    if (chunks <= 1) k_norm_bwd_rows<Tx, Ty, 4, 1, 64, WHOLE><<<g, dim3(256), 0, st>>>(a);
+    else if (chunks <= 2) k_norm_bwd_rows<Tx, Ty, 4, 2, 64, WHOLE><<<g, dim3(256), 0, st>>>(a);
+    else if (chunks <= 4) k_norm_bwd_rows<Tx, Ty, 4, 4, 64, WHOLE><<<g, dim3(256), 0, st>>>(a);
+    else if (chunks <= 8) k_norm_bwd_rows<Tx, Ty, 4, 1, 512, WHOLE><<<g, dim3(512), 0, st>>>(a);
+    else if (chunks <= 16) k_norm_bwd_rows<Tx, Ty, 4, 2, 512, WHOLE><<<g, dim3(512), 0, st>>>(a);
+    else k_norm_bwd_rows<Tx, Ty, 4, 4, 512, WHOLE><<<g, dim3(512), 0, st>>>(a);
+}
+
+template <typename Tx, typename Ty>
+void norm_bwd_rows(const NormArgs& a, hipStream_t st) {
+    if (a.n <= kRegRows) {
+        if (a.n % 4 == 0) norm_bwd_regs<Tx, Ty, true>(a, st);
+        else norm_bwd_regs<Tx, Ty, false>(a, st);
     } else {
         if (a.dx) k_norm_bwd_long_sums<Tx, Ty><<<dim3(static_cast<unsigned>(a.rows)), dim3(1024), 0, st>>>(a);
         k_norm_bwd_long_cols<Tx, Ty><<<dim3(static_cast<unsigned>((a.n + 255) / 256), a.groups), dim3(256), 0, st>>>(a);
@@ -712,7 +839,7 @@ template <typename Tx, typename Ty>
 void norm_bwd_maps(const NormArgs& a, hipStream_t st) {
     const int64_t tiles = a.rows / a.points * ((a.points + kPts - 1) / kPts);
     if (a.dx) k_norm_bwd_maps_sums<Tx, Ty><<<dim3(static_cast<unsigned>(tiles)), dim3(kMapThreads), 0, st>>>(a);
-    k_norm_bwd_maps<Tx, Ty><<<dim3(static_cast<unsigned>((a.n + kCols - 1) / kCols), a.groups), dim3(kMapThreads), 0, st>>>(a);
+    k_norm_bwd_maps<Tx, Ty><<<dim3(static_cast<unsigned>((a.n + kBCols - 1) / kBCols), a.groups), dim3(kMapThreads), 0, st>>>(a);
 }
 
 // ------------------------------------------------------------------------------------------ rotary
@@ -770,7 +897,13 @@ __global__ __launch_bounds__(256) void k_rotary(RotaryArgs a, RotaryTable tab) {
         T* y = static_cast<T*>(a.y[which]) + b * a.ys[which][0] + t * a.ys[which][1] + hh * a.ys[which][2];
         if (u >= turned) {
             const int d0 = 2 * a.pairs + (u - turned) * 8;
-            for (int d = d0; d < d0 + 8 && d < a.dim; ++d) y[d] = x[d];
+            if (d0 + 8 <= a.dim) {
+                Vec<T, 8> v;
+                __builtin_memcpy(&v, x + d0, sizeof(v));
+                __builtin_memcpy(y + d0, &v, sizeof(v));
+            } else {
+                for (int d = d0; d < a.dim; ++d) y[d] = x[d];
+            }
         } else if (p0 + kRotPairs <= a.pairs) {
             float x0[kRotPairs], x1[kRotPairs];
             if constexpr (INTER) {
