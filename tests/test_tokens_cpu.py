@@ -208,3 +208,36 @@ def test_packed_descriptors_match_the_structures():
         1, 3, 12, 19, 20, 29, 0.5, 31, 36)
     r = _lib.RotaryDesc.from_buffer_copy(_lib.ROTARY_PACK.pack(*range(1, 15), 0.25, *range(16, 28)))
     assert (r.tokens, r.k_out_strides[2], r.base, r.q_heads, r.sections[0], r.positions_shared) == (2, 14, 0.25, 16, 21, 27)
+
+
+def test_scattering_attention_refusals_and_parameters():
+    from wst_amd.torch import ScatteringAttention
+    m = ScatteringAttention(2, (32, 32), channels=3, heads=4, dim=32, key_heads=2)
+    assert {k: tuple(v.shape) for k, v in m.state_dict().items()} == {
+        "norm_weight": (243,), "norm_bias": (243,), "qkv.weight": (256, 243), "slopes": (4,), "pool_kv.weight": (128, 128),
+        "pool_query": (4, 32)}
+    assert m.sections == (5, 6, 5) and m.slopes.dtype == torch.float32
+    for kw, error in ((dict(heads=3, key_heads=2), RuntimeError), (dict(dim=0), RuntimeError), (dict(dim=257), RuntimeError),
+                      (dict(dtype=torch.float64), TypeError), (dict(dim=8, sections=(2, 2, 1)), RuntimeError),
+                      (dict(sections=(2, 2)), RuntimeError), (dict(J=6), RuntimeError), (dict(channels=0), RuntimeError)):
+        with pytest.raises(error):
+            ScatteringAttention(**{"J": 2, "shape": (32, 32), **kw})
+    x = torch.rand(2, 3, 32, 32)
+    with pytest.raises(TypeError):
+        m(x.numpy())
+    for bad in (x[0], x[:, :2], x[None, None]):
+        with pytest.raises(RuntimeError):
+            m(bad)
+    with pytest.raises(TypeError):
+        m(x, torch.zeros(2, 1))
+    with pytest.raises(RuntimeError):
+        m(x, torch.zeros(2, 3, dtype=torch.int32))
+    for count in (0, 2):
+        with pytest.raises(RuntimeError):
+            m.pooled(x, count=count)
+    if not torch.cuda.is_available():
+        with pytest.raises(RuntimeError, match="no ROCm GPU"):
+            m(x)
+        from wst_amd import features
+        with pytest.raises(RuntimeError, match="no ROCm GPU"):
+            features.extract_wst_tokens_batch(x)

@@ -79,6 +79,22 @@ def extract_wst_features(rgb_image, J: int = 2, L: int = 8):
     return extract_wst_features_batch(np.asarray(rgb_image)[None], J, L)[0]
 
 
+def extract_wst_tokens_batch(images, J: int = 2, L: int = 8, max_order: int = 2, weight=None, bias=None,
+                             eps: float = 1e-5, out_dtype=None):
+    """What a network behind the transform reads: (B, C, H, W) -> normalised tokens (B, Mo*No, C*K) on the GPU.
+
+    A token is one place of the maps with the coefficients of all channels, in the order of the training layout
+    (channel, then coefficient), brought to mean 0 and variance 1 over its values and then ``weight`` and ``bias``
+    ((C*K,), either may be None; gradients reach them, and stop before the transform).  The maps are read where the
+    transform wrote them.  ``out_dtype``: float32 (default), bfloat16 or float16."""
+    from . import tokens
+    x = _device_planes(images)
+    B, C, H, W = x.shape
+    S = scatter_device(x.reshape(B * C, H, W), H, W, J, L, max_order, False)
+    maps = S.reshape(B, C * S.shape[1], S.shape[2] * S.shape[3])
+    return tokens.layer_norm(maps.transpose(1, 2), weight, bias, eps=eps, out_dtype=out_dtype)
+
+
 def extract_wst_features_interleaved_batch(images, J: int = 2, L: int = 8, max_order: int = 2,
                                            as_numpy: bool = True):
     """Inference layout (inference.py:263-266): per channel [m_0, s_0, m_1, s_1, ...]."""

@@ -22,6 +22,7 @@ from . import _lib
 from .frontend import require_gpu
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+MAX_HEAD_DIM = _lib.MAX_HEAD_DIM
 
 
 def _dtype_id(t, name):
