@@ -1513,8 +1513,9 @@ __global__ __launch_bounds__((dkv_threads<T, DP>()), sizeof(T) == 2 ? 2 : 1) voi
     const wst_attention_desc& d = a.d;
     const int t = threadIdx.x, lane = t & 63, w = (t >> 6) & 3, half = t >> 8, hl = lane >> 5;
     const int group = d.q_heads / d.k_heads;
-    const uint32_t cells = static_cast<uint32_t>(d.batch) * d.k_heads, bh = blockIdx.x % cells, part = blockIdx.y;
-    const int j0 = static_cast<int>(blockIdx.x / cells) * kBQ;         // early keys are seen by most: first
+    const uint32_t cells = static_cast<uint32_t>(d.batch) * d.k_heads, slot = blockIdx.x % (cells * a.parts);
+    const uint32_t bh = slot % cells, part = slot / cells;
+    const int j0 = static_cast<int>(blockIdx.x / (cells * a.parts)) * kBQ;         // early keys are seen by most: first
     const int64_t b = bh / d.k_heads;
     const int kvh = static_cast<int>(bh % d.k_heads);
     const Scope sc(d, b);
@@ -1553,8 +1554,22 @@ __global__ __launch_bounds__((dkv_threads<T, DP>()), sizeof(T) == 2 ? 2 : 1) voi
     int full0 = tile0, full1 = keys == kBQ ? q_len / kRows : 0;
     if (sc.causal && j0 + kBQ > sc.prefix) full0 = max(tile0, (max(j0 + kBQ - 1 - sc.shift, 0) + kRows - 1) / kRows);
     const Walk walk{tile0, tiles, full0, max(full0, full1), marked};
-    // items of work: the full tiles of the first head, then of the next, ..., then the others; this part takes every
-    // a.parts-th
+    // Items of work: the full tiles of the first head, then of the next, ..., then the others. Parts take heads of their
+    // own where that comes out even, so that the blocks of an XCD (blocks 8 apart) read the same queries at a time (8192
+    // in order, 8 heads x 128 sharing 2: 560 -> 356 us; with cap and prefix 659 -> 442); what is left of the number of
+    // parts takes every so many-th item.
+    int g0 = 0, g1 = group, ahead = static_cast<int>(part), stride = a.parts;
+    if (a.parts % group == 0) {
+        g0 = ahead % group;
+        g1 = g0 + 1;
+        ahead /= group;
+        stride /= group;
+    } else if (group % a.parts == 0) {
+        g0 = ahead * (group / a.parts);
+        g1 = g0 + group / a.parts;
+        ahead = 0;
+        stride = 1;
+    }
     struct Item {
         Step s;
         int g;
@@ -1562,10 +1577,10 @@ __global__ __launch_bounds__((dkv_threads<T, DP>()), sizeof(T) == 2 ? 2 : 1) voi
     auto step = [&](Item x) {
         x.s.find(walk, marks);
         for (int k = 0; x.s.done(walk) && k < 2 * group; ++k) {       // bounded: there may be no tile at all
-            if (x.g + 1 < group) {
+            if (x.g + 1 < g1) {
                 ++x.g;
             } else if (!x.s.rest) {
-                x.g = 0;
+                x.g = g0;
                 x.s.rest = 1;
             } else {
                 break;
@@ -1616,10 +1631,10 @@ __global__ __launch_bounds__((dkv_threads<T, DP>()), sizeof(T) == 2 ? 2 : 1) voi
         dfetch.issue(at<T>(a.g.d_o, a.g.do_strides, b, i, h), whole, q_len - i, doc, dt + buf * kTile, t);
     };
     if (marked) __syncthreads();       // the marks
-    Item cur{{tile0 - 1, 0}, 0};
-    if (tile0 < tiles) cur = skip(step(cur), part);
+    Item cur{{tile0 - 1, 0}, g0};
+    if (tile0 < tiles) cur = skip(step(cur), ahead);
     else cur.s.tile = tiles;
-    Item nxt = skip(cur, a.parts);
+    Item nxt = skip(cur, stride);
     if (!cur.s.done(walk)) {
         load(cur);
         put(rows[0]);
@@ -1653,7 +1668,7 @@ __global__ __launch_bounds__((dkv_threads<T, DP>()), sizeof(T) == 2 ? 2 : 1) voi
         arrived();
         __syncthreads();
         if (!nxt.s.done(walk)) fetch(nxt, buf ^ 1, rows[turn1]);
-        const Item after = skip(nxt, a.parts);
+        const Item after = skip(nxt, stride);
         if (!after.s.done(walk)) load(after);
 #pragma unroll
         for (int n = 0; n < (kWide ? 1 : 2); ++n) {

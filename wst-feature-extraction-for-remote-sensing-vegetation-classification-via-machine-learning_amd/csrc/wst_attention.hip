@@ -94,7 +94,11 @@ AttnPlan plan_of(const wst_attention_desc& d, bool tiles) {
         const int64_t items = group * ((d.q_len + 63) / 64), keys = d.batch * d.k_heads * ((d.k_len + kBQ - 1) / kBQ);
         int64_t parts = keys ? (512 + keys - 1) / keys : 1;
         parts = parts < items / 2 ? parts : items / 2;
-        p.parts = static_cast<int>(parts < 1 ? 1 : parts > 64 ? 64 : parts);
+        parts = parts < 1 ? 1 : parts > 64 ? 64 : parts;
+        // whole heads a part, or whole parts a head, where that takes less than twice as many (k_attn_dkv)
+        int64_t even = parts;
+        while (even % group && group % even) ++even;
+        p.parts = static_cast<int>(even < 2 * parts ? even : parts);
         p.slots = static_cast<int>((d.q_len + kBQ - 1) / kBQ * 4);
         if (p.parts > 1) p.backward = static_cast<size_t>(p.parts) * d.batch * d.k_heads * d.k_len * 2 * d.dim;
     }

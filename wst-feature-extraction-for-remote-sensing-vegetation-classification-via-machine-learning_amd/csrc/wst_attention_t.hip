@@ -47,7 +47,7 @@ void attend_backward(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
         const int64_t q_blocks = d.batch * d.q_heads * ((d.q_len + kBQ - 1) / kBQ);
         const int64_t k_blocks = d.batch * d.k_heads * ((d.k_len + kBQ - 1) / kBQ);
         if (want_q) k_attn_dq<T, DP, CAP, BIAS><<<dim3(static_cast<unsigned>(q_blocks)), dim3(256), 0, st>>>(a);   // and delta
-        if (want_k) k_attn_dkv<T, DP, CAP, BIAS><<<dim3(static_cast<unsigned>(k_blocks), p.parts), dim3(dkv_threads<T, DP>()), 0, st>>>(a);
+        if (want_k) k_attn_dkv<T, DP, CAP, BIAS><<<dim3(static_cast<unsigned>(k_blocks * p.parts)), dim3(dkv_threads<T, DP>()), 0, st>>>(a);
     });
     if (p.parts > 1 && want_k) {
         const dim3 keys(static_cast<unsigned>((d.k_len + 3) / 4), d.k_heads, static_cast<unsigned>(d.batch));
