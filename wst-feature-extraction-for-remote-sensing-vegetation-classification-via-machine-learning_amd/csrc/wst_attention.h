@@ -879,15 +879,24 @@ constexpr int kBQ = 128, kBK = 64;
 // kSlack powers of two: larger weights cost neither sums nor roundings anything, and the output is not scaled. A wave
 // that meets such a score goes on in loops that move the maximum with every tile. (As a branch inside the loop the
 // scaling costs as much when it is not taken: where the ways meet, the compiler copies all sums between registers.)
-template <typename T, int DP, int CAP, int BIAS>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(AttnArgs a) {
+//
+// TEAMS: one or two teams of four waves. Two share the queries and take every other tile, each through its own part of
+// LDS, and join their maxima, sums and outputs at the end: the block with the longest rows of an order does not run on
+// alone at half the rate. Where all blocks are as long, two independent blocks are better than two teams that wait for
+// each other at every tile (8192 x 8 heads x 128: in order 238 -> 201 us, dq 283 -> 250; not in order 327 -> 379).
+template <typename T, int DP, int CAP, int BIAS, int TEAMS>
+__global__ __launch_bounds__(256 * TEAMS, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(AttnArgs a) {
     using L = Tile<T, DP>;
-    __shared__ __attribute__((aligned(256))) char kt[2][kBK * L::kRowBytes], vt[2][kBK * L::kRowBytes];
-    __shared__ Along al[3];
+    constexpr int kTile = kBK * L::kRowBytes;
+    __shared__ __attribute__((aligned(256))) char pool[TEAMS * 4 * kTile];
+    __shared__ Along alongs[TEAMS][3];
     __shared__ Marks marks;
     __shared__ float scratch[4][DP];
     const wst_attention_desc& d = a.d;
-    const int t = threadIdx.x, lane = t & 63, w = t >> 6, hl = lane >> 5;
+    const int team = TEAMS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0;
+    const int t = threadIdx.x & 255, lane = t & 63, w = t >> 6, hl = lane >> 5;
+    char *kt = pool + team * 4 * kTile, *vt = kt + 2 * kTile;
+    Along* al = alongs[team];
     const uint32_t cells = static_cast<uint32_t>(d.batch) * d.q_heads, bh = blockIdx.x % cells;
     const int nq = static_cast<int>((d.q_len + kBQ - 1) / kBQ), i0 = (nq - 1 - static_cast<int>(blockIdx.x / cells)) * kBQ;   // long rows first
     const int64_t b = bh / d.q_heads;
@@ -908,10 +917,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(AttnAr
     const int end = sc.limit(last), open = sc.limit(i0);
     const int tiles = end > 0 ? (end + kBK - 1) / kBK : 0;
     const bool marked = sc.q_doc != nullptr, along = sc.q_doc || sc.q_pos;
-    if (marked) scan_documents(marks, sc.q_doc, i0, kBQ, static_cast<int>(d.q_len), sc.k_doc, 0, tiles, sc.length);
+    if (marked) scan_documents(marks, sc.q_doc, i0, kBQ, static_cast<int>(d.q_len), sc.k_doc, 0, tiles, sc.length, 4 * TEAMS);
     if (marked || d.dim != DP || sc.length % kBK) {
-        clear<sizeof(kt)>(&kt[0][0], t);
-        clear<sizeof(vt)>(&vt[0][0], t);
+        clear<4 * kTile>(kt, t);
     }
     f32x16 o[DP / 32];
 #pragma unroll
@@ -929,16 +937,26 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(AttnAr
         const int* doc = marked ? with.doc : nullptr;
         const int left = sc.length - n * kBK;
         const bool whole = !marked && d.dim == DP && left >= kBK;
-        kf.issue(kb + static_cast<int64_t>(n) * kBK * ks, whole, left, doc, kt[buf], t);
-        vf.issue(vb + static_cast<int64_t>(n) * kBK * vs, whole, left, doc, vt[buf], t);
+        kf.issue(kb + static_cast<int64_t>(n) * kBK * ks, whole, left, doc, kt + buf * kTile, t);
+        vf.issue(vb + static_cast<int64_t>(n) * kBK * vs, whole, left, doc, vt + buf * kTile, t);
     };
     AlongStage as{};
     if (marked) __syncthreads();       // the marks
     const Walk walk{0, tiles, 0, open / kBK, marked};
+    bool behind = false;               // the first team has a tile after the second one's last
+    auto go = [&](Step& x) {           // over the other team's tile to the next of this one's
+        x.go(walk, marks);
+        if constexpr (TEAMS > 1) {
+            if (x.done(walk)) return;
+            x.go(walk, marks);
+            behind = x.done(walk);
+        }
+    };
     Step cur{-1, 0};
-    cur.go(walk, marks);
+    if (team) go(cur);
+    else cur.go(walk, marks);
     Step next = cur;
-    if (!cur.done(walk)) next.go(walk, marks);
+    if (!cur.done(walk)) go(next);
     if (along) {
         if (!cur.done(walk)) {
             as.load(sc.k_pos, sc.k_doc, sc.axes, cur.tile * kBK, sc.length, t);
@@ -963,7 +981,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(AttnAr
         after = next;
         if (!next.done(walk)) {
             fetch(next.tile, buf ^ 1, al[turn1]);
-            after.go(walk, marks);
+            go(after);
             if (along && !after.done(walk)) as.load(sc.k_pos, sc.k_doc, sc.axes, after.tile * kBK, sc.length, t);
         }
     };
@@ -976,7 +994,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(AttnAr
     };
     // x of a tile, and the query's largest
     auto look = [&](auto mask, f32x16 (&x)[2]) {
-        const typename L::Lane kc = lanes.at_tile(kt[buf]);
+        const typename L::Lane kc = lanes.at_tile(kt + buf * kTile);
         x[0] = x[1] = zero16();
 #pragma unroll
         for (int c = 0; c < DP / 16; ++c)
@@ -994,7 +1012,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(AttnAr
         return halves_max(top) * sh.mul;
     };
     auto add = [&](f32x16 (&x)[2]) {
-        const typename L::Lane vc = lanes.at_tile(vt[buf]);
+        const typename L::Lane vc = lanes.at_tile(vt + buf * kTile);
         const float base = fmaxf(m, -3.0e38f);         // nothing seen yet: exp2(-inf) = 0 either way
         Frag<T> p[2][2];
 #pragma unroll
@@ -1045,8 +1063,32 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(AttnAr
     entered = slow;
     while (!cur.done(walk) && !marked) careful(std::integral_constant<int, 1>{});
     while (!cur.done(walk)) careful(std::integral_constant<int, 2>{});
-    const AttnArgs& z = again();
     l = halves_sum(l);
+    if constexpr (TEAMS > 1) {         // a lane's registers go to the lane that has the same place in the first team
+        static_assert(sizeof(pool) >= 4 * (DP / 2 + 2) * 64 * sizeof(float), "room for the sums");
+        float* sums = reinterpret_cast<float*>(pool) + w * ((DP / 2 + 2) * 64) + lane;
+        if (team && behind) __syncthreads();           // as many waits as the first team's
+        __syncthreads();
+        if (team) {
+#pragma unroll
+            for (int k = 0; k < DP / 32; ++k)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sums[(16 * k + r) * 64] = o[k][r];
+            sums[(DP / 2) * 64] = m;
+            sums[(DP / 2 + 1) * 64] = l;
+        }
+        __syncthreads();
+        if (team) return;
+        const float m2 = sums[(DP / 2) * 64], top = fmaxf(m, m2), base = fmaxf(top, -3.0e38f);
+        const float f = __builtin_amdgcn_exp2f(m - base), f2 = __builtin_amdgcn_exp2f(m2 - base);
+        l = l * f + sums[(DP / 2 + 1) * 64] * f2;
+        m = top;
+#pragma unroll
+        for (int k = 0; k < DP / 32; ++k)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[k][r] = o[k][r] * f + sums[(16 * k + r) * 64] * f2;
+    }
+    const AttnArgs& z = again();
     const float inv = l == 0.f ? 0.f : 1.f / l;
     if (ok) {
         T* out = const_cast<T*>(at<T>(z.o, z.d.o_strides, b, i, h));
@@ -1294,15 +1336,19 @@ inline constexpr float kUp<f16> = 64.f;
 // dq, the slopes' shares and delta: walks the keys as the forward pass does. Scores come back as (keys x queries), so
 // their gradient is the operand of dq^T = k^T dz^T as it stands; keys are read from LDS both ways. delta goes in as the
 // product's starting value.
-template <typename T, int DP, int CAP, int BIAS>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(AttnArgs a) {
+template <typename T, int DP, int CAP, int BIAS, int TEAMS>
+__global__ __launch_bounds__(256 * TEAMS, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(AttnArgs a) {
     using L = Tile<T, DP>;
-    __shared__ __attribute__((aligned(256))) char kt[2][kBK * L::kRowBytes], vt[2][kBK * L::kRowBytes];
-    __shared__ Along al[3];
+    constexpr int kTile = kBK * L::kRowBytes;
+    __shared__ __attribute__((aligned(256))) char pool[TEAMS * 4 * kTile];
+    __shared__ Along alongs[TEAMS][3];
     __shared__ Marks marks;
     __shared__ float scratch[4][2][DP];
     const wst_attention_desc& d = a.d;
-    const int t = threadIdx.x, lane = t & 63, w = t >> 6, hl = lane >> 5;
+    const int team = TEAMS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0;
+    const int t = threadIdx.x & 255, lane = t & 63, w = t >> 6, hl = lane >> 5;
+    char *kt = pool + team * 4 * kTile, *vt = kt + 2 * kTile;
+    Along* al = alongs[team];
     const uint32_t cells = static_cast<uint32_t>(d.batch) * d.q_heads, bh = blockIdx.x % cells;
     const int nq = static_cast<int>((d.q_len + kBQ - 1) / kBQ), qt = nq - 1 - static_cast<int>(blockIdx.x / cells), i0 = qt * kBQ;
     const int64_t b = bh / d.q_heads;
@@ -1329,7 +1375,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(AttnArg
 #pragma unroll
             for (int e = 0; e < 8; ++e) delta += static_cast<float>(df[c][e]) * static_cast<float>(of[c][e]);
         delta = halves_sum(delta);
-        if (ok && hl == 0) a.delta[row] = delta;
+        if (ok && hl == 0 && !team) a.delta[row] = delta;
     }
     row_frags<T, DP>(at<T>(d.q, d.q_strides, b, ok ? i : 0, h), live, d.dim, qf);
     if (d.scale < 0.f) negate<T, DP>(qf);
@@ -1339,10 +1385,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(AttnArg
     const int end = sc.limit(last), open = sc.limit(i0);
     const int tiles = end > 0 ? (end + kBK - 1) / kBK : 0;
     const bool marked = sc.q_doc != nullptr, along = sc.q_doc || sc.q_pos;
-    if (marked) scan_documents(marks, sc.q_doc, i0, kBQ, static_cast<int>(d.q_len), sc.k_doc, 0, tiles, sc.length);
+    if (marked) scan_documents(marks, sc.q_doc, i0, kBQ, static_cast<int>(d.q_len), sc.k_doc, 0, tiles, sc.length, 4 * TEAMS);
     if (marked || d.dim != DP || sc.length % kBK) {
-        clear<sizeof(kt)>(&kt[0][0], t);
-        clear<sizeof(vt)>(&vt[0][0], t);
+        clear<4 * kTile>(kt, t);
     }
     f32x16 dq[DP / 32];
 #pragma unroll
@@ -1363,16 +1408,26 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(AttnArg
         const int* doc = marked ? with.doc : nullptr;
         const int left = sc.length - n * kBK;
         const bool whole = !marked && d.dim == DP && left >= kBK;
-        kf.issue(kb + static_cast<int64_t>(n) * kBK * ks, whole, left, doc, kt[buf], t);
-        vf.issue(vb + static_cast<int64_t>(n) * kBK * vs, whole, left, doc, vt[buf], t);
+        kf.issue(kb + static_cast<int64_t>(n) * kBK * ks, whole, left, doc, kt + buf * kTile, t);
+        vf.issue(vb + static_cast<int64_t>(n) * kBK * vs, whole, left, doc, vt + buf * kTile, t);
     };
     AlongStage as{};
     if (marked) __syncthreads();       // the marks
     const Walk walk{0, tiles, 0, open / kBK, marked};
+    bool behind = false;               // teams as in k_attn_fwd
+    auto go = [&](Step& x) {
+        x.go(walk, marks);
+        if constexpr (TEAMS > 1) {
+            if (x.done(walk)) return;
+            x.go(walk, marks);
+            behind = x.done(walk);
+        }
+    };
     Step cur{-1, 0};
-    cur.go(walk, marks);
+    if (team) go(cur);
+    else cur.go(walk, marks);
     Step next = cur;
-    if (!cur.done(walk)) next.go(walk, marks);
+    if (!cur.done(walk)) go(next);
     if (along) {
         if (!cur.done(walk)) {
             as.load(sc.k_pos, sc.k_doc, sc.axes, cur.tile * kBK, sc.length, t);
@@ -1396,10 +1451,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(AttnArg
         Step after = next;
         if (!next.done(walk)) {
             fetch(next.tile, buf ^ 1, al[turn1]);
-            after.go(walk, marks);
+            go(after);
             if (along && !after.done(walk)) as.load(sc.k_pos, sc.k_doc, sc.axes, after.tile * kBK, sc.length, t);
         }
-        const typename L::Lane kc = lanes.at_tile(kt[buf]), vc = lanes.at_tile(vt[buf]);
+        const typename L::Lane kc = lanes.at_tile(kt + buf * kTile), vc = lanes.at_tile(vt + buf * kTile);
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             f32x16 x = zero16(), dp, grad, far;
@@ -1456,6 +1511,30 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(AttnArg
     while (!cur.done(walk) && !cur.rest) work(std::integral_constant<int, 0>{});
     while (!cur.done(walk) && !marked) work(std::integral_constant<int, 1>{});
     while (!cur.done(walk)) work(std::integral_constant<int, 2>{});
+    if constexpr (TEAMS > 1) {
+        static_assert(sizeof(pool) >= 4 * (DP / 2 + 3) * 64 * sizeof(float), "room for the sums");
+        float* sums = reinterpret_cast<float*>(pool) + w * ((DP / 2 + 3) * 64) + lane;
+        if (team && behind) __syncthreads();
+        __syncthreads();
+        if (team) {
+#pragma unroll
+            for (int k = 0; k < DP / 32; ++k)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sums[(16 * k + r) * 64] = dq[k][r];
+            sums[(DP / 2) * 64] = pf;
+            sums[(DP / 2 + 1) * 64] = e0;
+            sums[(DP / 2 + 2) * 64] = e1;
+        }
+        __syncthreads();
+        if (team) return;
+#pragma unroll
+        for (int k = 0; k < DP / 32; ++k)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dq[k][r] += sums[(16 * k + r) * 64];
+        pf += sums[(DP / 2) * 64];
+        e0 += sums[(DP / 2 + 1) * 64];
+        e1 += sums[(DP / 2 + 2) * 64];
+    }
     const AttnArgs& z = again();
     const float mul = z.d.scale / kUp<T>;
     if (ok && z.g.dq) {

@@ -20,6 +20,15 @@ void with_kind(const wst_attention_desc& d, F f) {
     }
 }
 
+// Two teams a block where the rows are of many lengths; float32 has no room in LDS for two.
+template <typename T, typename F>
+void with_teams(const wst_attention_desc& d, F f) {
+    if constexpr (sizeof(T) == 2) {
+        if (d.causal && d.k_len > 2 * kBK) return f(std::integral_constant<int, 2>{});
+    }
+    f(std::integral_constant<int, 1>{});
+}
+
 template <typename T, int DP>
 void attend(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
     const wst_attention_desc& d = a.d;
@@ -30,7 +39,10 @@ void attend(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
             k_attn_split<T, DP, CAP, BIAS><<<dim3(static_cast<unsigned>(p.splits * row_tiles * d.batch * d.k_heads)), dim3(256), 0, st>>>(a);
         } else {
             const int64_t blocks = d.batch * d.q_heads * ((d.q_len + kBQ - 1) / kBQ);
-            k_attn_fwd<T, DP, CAP, BIAS><<<dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st>>>(a);
+            with_teams<T>(d, [&](auto teams) {
+                constexpr int TEAMS = decltype(teams)::value;
+                k_attn_fwd<T, DP, CAP, BIAS, TEAMS><<<dim3(static_cast<unsigned>(blocks)), dim3(256 * TEAMS), 0, st>>>(a);
+            });
         }
     });
     const int64_t rows = d.batch * d.q_heads * d.q_len;
@@ -46,7 +58,11 @@ void attend_backward(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
         constexpr int CAP = decltype(cap)::value, BIAS = decltype(bias)::value;
         const int64_t q_blocks = d.batch * d.q_heads * ((d.q_len + kBQ - 1) / kBQ);
         const int64_t k_blocks = d.batch * d.k_heads * ((d.k_len + kBQ - 1) / kBQ);
-        if (want_q) k_attn_dq<T, DP, CAP, BIAS><<<dim3(static_cast<unsigned>(q_blocks)), dim3(256), 0, st>>>(a);   // and delta
+        if (want_q)
+            with_teams<T>(d, [&](auto teams) {
+                constexpr int TEAMS = decltype(teams)::value;
+                k_attn_dq<T, DP, CAP, BIAS, TEAMS><<<dim3(static_cast<unsigned>(q_blocks)), dim3(256 * TEAMS), 0, st>>>(a);   // and delta
+            });
         if (want_k) k_attn_dkv<T, DP, CAP, BIAS><<<dim3(static_cast<unsigned>(k_blocks * p.parts)), dim3(dkv_threads<T, DP>()), 0, st>>>(a);
     });
     if (p.parts > 1 && want_k) {
