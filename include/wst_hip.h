@@ -354,6 +354,8 @@ typedef struct wst_attention_desc {
     const int32_t *q_doc, *k_doc;              /* (q_len), (k_len) or both NULL; negative: belongs to none */
     const int32_t* k_lengths;                  /* (batch) or NULL */
     const int32_t* prefix;                     /* (batch) or NULL; needs causal */
+    void* o_rest;                              /* o's type and strides, or NULL: what rounding took from o, which the
+                                                  forward call writes and the backward call reads for its sums over o */
     float scale, cap;
     int32_t q_heads, k_heads, dim, dtype, axes, causal;
 } wst_attention_desc;

@@ -504,3 +504,30 @@ def test_refusals_name_the_argument():
     y = tokens.layer_norm(x.requires_grad_())
     g, = torch.autograd.grad(y.sum(), x)
     assert g.shape == x.shape                                   # a refusal leaves nothing behind
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("D,Tq,causal", [(64, 200, False), (128, 200, True), (32, 20, False), (12, 40, False)])
+def test_attention_gradient_of_rows_with_one_large_weight(D, Tq, causal, dtype):
+    """Where one weight is nearly 1, every do.v_j - delta that counts is a small difference: delta taken from the rounded
+    output would miss it by |do| |o| half an eps, a multiple of the difference itself. With p_1 = 1 - t the exact
+    ds_1 = p_1 (do.v_1 - delta) is t do.(v_1 - mean of the rest), and |do| |o| eps / 2 against t |do| |v| sqrt(2) is a
+    relative error of eps / (2 sqrt 2 t) without, and eps^2 / (2 sqrt 2 t) with what the rounding took. Here t < eps / 2:
+    the first is over 0.7, the second under eps, beside the roundings of score gradients and dq (eps together). A tenth of
+    the first holds all of the second's (8 eps of bfloat16)."""
+    g = _gen(D + Tq)
+    eps = torch.finfo(dtype).eps
+    q, k, v, do = (torch.randn(1, Tq, 1, D, generator=g) for _ in range(4))
+    k = k / k.norm(dim=-1, keepdim=True)
+    k[:, 0] = k[:, 0] * 0 + D ** -0.5                    # key 0 stands out by -log(eps / 2 / Tq), from every query
+    far = -math.log(eps / 4 / Tq)
+    q = 0.01 * q + far
+    q, k, v, do = (t.to(dtype) for t in (q, k, v, do))
+    scale = D ** -0.5
+    want = ref.attention(q, k, v, causal=causal, scale=scale, do=do)["dq"][0]
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+    o = tokens.attention(*leaves, causal=causal, scale=scale)
+    dq = torch.autograd.grad(o, leaves[0], do.cuda())[0].cpu().to(torch.float64)
+    rows = slice(1, None)                                # query 0 in order sees key 0 alone: no gradient
+    off = (dq - want)[:, rows].norm() / want[:, rows].norm()
+    assert float(off) < 0.07, float(off)

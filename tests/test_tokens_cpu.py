@@ -203,9 +203,9 @@ def test_packed_descriptors_match_the_structures():
     for pack, kind in ((_lib.NORM_PACK, _lib.NormDesc), (_lib.ROTARY_PACK, _lib.RotaryDesc),
                        (_lib.ATTENTION_PACK, _lib.AttentionDesc), (_lib.GRADS_PACK, _lib.AttentionGrads)):
         assert pack.size == ctypes.sizeof(kind), kind
-    d = _lib.AttentionDesc.from_buffer_copy(_lib.ATTENTION_PACK.pack(*range(1, 30), 0.5, 2.0, *range(31, 37)))
-    assert (d.batch, d.k_len, d.v_strides[2], d.k_doc_stride, d.q, d.prefix, d.scale, d.q_heads, d.causal) == (
-        1, 3, 12, 19, 20, 29, 0.5, 31, 36)
+    d = _lib.AttentionDesc.from_buffer_copy(_lib.ATTENTION_PACK.pack(*range(1, 31), 0.5, 2.0, *range(32, 38)))
+    assert (d.batch, d.k_len, d.v_strides[2], d.k_doc_stride, d.q, d.prefix, d.o_rest, d.scale, d.q_heads, d.causal) == (
+        1, 3, 12, 19, 20, 29, 30, 0.5, 32, 37)
     r = _lib.RotaryDesc.from_buffer_copy(_lib.ROTARY_PACK.pack(*range(1, 15), 0.25, *range(16, 28)))
     assert (r.tokens, r.k_out_strides[2], r.base, r.q_heads, r.sections[0], r.positions_shared) == (2, 14, 0.25, 16, 21, 27)
 

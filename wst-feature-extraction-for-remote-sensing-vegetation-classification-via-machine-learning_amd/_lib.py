@@ -102,7 +102,7 @@ class AttentionDesc(ctypes.Structure):
                 ("q_pos_stride", _I64), ("k_pos_stride", _I64), ("q_doc_stride", _I64),
                 ("k_doc_stride", _I64)] + \
                [(n, _PTR) for n in ("q", "k", "v", "slopes", "q_pos", "k_pos", "q_doc", "k_doc", "k_lengths",
-                                    "prefix")] + \
+                                    "prefix", "o_rest")] + \
                [("scale", ctypes.c_float), ("cap", ctypes.c_float), ("q_heads", _I32), ("k_heads", _I32),
                 ("dim", _I32), ("dtype", _I32), ("axes", _I32), ("causal", _I32)]
 
@@ -116,7 +116,7 @@ class AttentionGrads(ctypes.Structure):
 # The descriptors as packed bytes: a call of a few microseconds should not spend as long on filling a Structure.
 NORM_PACK = struct.Struct("@9q3if")
 ROTARY_PACK = struct.Struct("@14qd12i")
-ATTENTION_PACK = struct.Struct("@19q10P2f6i")
+ATTENTION_PACK = struct.Struct("@19q11P2f6i")
 GRADS_PACK = struct.Struct("@7P12q")
 
 

@@ -92,6 +92,14 @@ __device__ __forceinline__ const T* at(const void* p, const int64_t (&s)[3], int
     return static_cast<const T*>(p) + b * s[0] + t * s[1] + h * s[2];
 }
 
+// What rounding v to T takes from it. The backward pass has it from the forward pass (o_rest): delta = sum do o taken
+// from the rounded output alone is off by its rounding, which a row with few large weights meets as a whole, since there
+// all of its do.v_j lie close to delta.
+template <typename T>
+__device__ __forceinline__ T lost(float v) {
+    return static_cast<T>(v - static_cast<float>(static_cast<T>(v)));
+}
+
 // dot of a row in LDS with a row in memory
 template <typename T>
 __device__ __forceinline__ float dot_row(const float* a, const T* b, int dim) {
@@ -157,7 +165,10 @@ __device__ void row_forward(const AttnArgs& a, const Scope& sc, int64_t b, int h
     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
     for (int c = 0; c < kPer; ++c)
-        if (lane + 64 * c < d.dim) o[lane + 64 * c] = static_cast<T>(acc[c] * inv);
+        if (lane + 64 * c < d.dim) {
+            o[lane + 64 * c] = static_cast<T>(acc[c] * inv);
+            if (d.o_rest) static_cast<T*>(d.o_rest)[o - static_cast<T*>(a.o) + lane + 64 * c] = lost<T>(acc[c] * inv);
+        }
     if (lane == 0 && a.lse) a.lse[(b * d.q_heads + h) * d.q_len + i] = l == 0.f ? -INFINITY : m + logf(l);
 }
 
@@ -274,7 +285,8 @@ __global__ __launch_bounds__(256) void k_attn_delta(AttnArgs a) {
     if (i >= d.q_len) return;
     const T *o = at<T>(a.g.o, d.o_strides, b, i, h), *dr = at<T>(a.g.d_o, a.g.do_strides, b, i, h);
     float s = 0.f;
-    for (int x = lane; x < d.dim; x += 64) s += static_cast<float>(o[x]) * static_cast<float>(dr[x]);
+    const T* rest = d.o_rest ? static_cast<const T*>(d.o_rest) + (o - static_cast<const T*>(a.g.o)) : nullptr;
+    for (int x = lane; x < d.dim; x += 64) s += (static_cast<float>(o[x]) + (rest ? static_cast<float>(rest[x]) : 0.f)) * static_cast<float>(dr[x]);
     s = wave_sum(s);
     if (lane == 0) a.delta[(b * d.q_heads + h) * d.q_len + i] = s;
 }
@@ -590,7 +602,8 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // product and mul = scale log2 e, so that scaling costs nothing beyond the subtraction of the maximum. Capped, with
 // e = exp(2 z / cap), tanh = 1 - 2 / (e + 1), x is -1 / (e + 1): the cap's slope is 1 - tanh^2 = -4 x (1 + x). Its error
 // of 2^-24 or two of the cap is below what 16-bit weights keep; float32 takes the library's tanh, good to an ulp. With a
-// bias x is the score itself, mul = 1. For a maximum over x mul must not be negative: there a negative
+// bias x is the score itself, mul = log2 e: slopes times log2 e, rounded, would be the slopes of a network a little way
+// off. For a maximum over x mul must not be negative: there a negative
 // scale turns q over instead (sign = false).
 struct Shape {
     float raw, mul, add;      // of the score before the bias
@@ -603,8 +616,8 @@ struct Shape {
         s.cap = d.cap > 0.f;
         s.twice = s.cap ? 2.f * scale * kLog2e / d.cap : 0.f;
         s.turn = s.cap ? scale / d.cap : 0.f;
-        s.raw = !s.cap ? scale * kLog2e : sizeof(T) == 4 ? d.cap * kLog2e : 2.f * d.cap * kLog2e;
-        s.mul = d.slopes ? 1.f : s.raw;
+        s.raw = !s.cap ? scale : sizeof(T) == 4 ? d.cap : 2.f * d.cap;
+        s.mul = d.slopes ? kLog2e : s.raw * kLog2e;
         s.add = s.cap && sizeof(T) != 4 ? d.cap * kLog2e : 0.f;
         return s;
     }
@@ -793,7 +806,7 @@ __device__ __forceinline__ Kind kind_of(const wst_attention_desc& d) {
 // Turns 32 x 32 dot products (rows: keys key0 + 32 sub .., column: the lane's query) into x of Shape, -inf where the
 // query does not see the key. GRAD: also the cap's slope and the distances.
 template <typename T, bool GRAD, int MASK>
-__device__ __forceinline__ void scores(f32x16& x, const Kind& kind, const Shape& sh, float slope2, const Query& q, const Along& al,
+__device__ __forceinline__ void scores(f32x16& x, const Kind& kind, const Shape& sh, float slope, const Query& q, const Along& al,
                                        int key0, int sub, f32x16& grad, f32x16& far) {
     const int h = (threadIdx.x & 63) >> 5;
     if (kind.cap) sh.bend<T, GRAD>(x, grad);
@@ -812,7 +825,7 @@ __device__ __forceinline__ void scores(f32x16& x, const Kind& kind, const Shape&
                 for (int e = 0; e < 4; ++e) {
                     const float f = static_cast<float>(sum[e]);
                     if constexpr (GRAD) far[4 * g + e] = f;
-                    x[4 * g + e] = fmaf(-slope2, f, x[4 * g + e] * sh.raw);
+                    x[4 * g + e] = fmaf(-slope, f, x[4 * g + e] * sh.raw);
                 }
             }
         } else {
@@ -821,7 +834,7 @@ __device__ __forceinline__ void scores(f32x16& x, const Kind& kind, const Shape&
             for (int r = 0; r < 16; ++r) {
                 const float f = fabsf(base - static_cast<float>(8 * (r >> 2) + (r & 3)));
                 if constexpr (GRAD) far[r] = f;
-                x[r] = fmaf(-slope2, f, x[r] * sh.raw);
+                x[r] = fmaf(-slope, f, x[r] * sh.raw);
             }
         }
     }
@@ -907,7 +920,7 @@ __global__ __launch_bounds__(256 * TEAMS, sizeof(T) == 2 ? 2 : 1) void k_attn_fw
     const int i = i0 + w * 32 + (lane & 31);
     const bool ok = i < d.q_len;
     const Query q = query_of(sc, i, ok);
-    const float slope2 = d.slopes ? d.slopes[h] * kLog2e : 0.f;
+    const float slope = d.slopes ? d.slopes[h] : 0.f;
     Frag<T> qf[DP / 16];
     row_frags<T, DP>(at<T>(d.q, d.q_strides, b, ok ? i : 0, h), ok && q.limit > 0, d.dim, qf);
     if (d.scale < 0.f) negate<T, DP>(qf);
@@ -1005,7 +1018,7 @@ __global__ __launch_bounds__(256 * TEAMS, sizeof(T) == 2 ? 2 : 1) void k_attn_fw
         float top = -INFINITY;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            scores<T, false, decltype(mask)::value>(x[n], kind, sh, slope2, q, al[turn], cur.tile * kBK, n, unused, unused);
+            scores<T, false, decltype(mask)::value>(x[n], kind, sh, slope, q, al[turn], cur.tile * kBK, n, unused, unused);
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = fmaxf(top, x[n][r]);
         }
@@ -1092,13 +1105,20 @@ __global__ __launch_bounds__(256 * TEAMS, sizeof(T) == 2 ? 2 : 1) void k_attn_fw
     const float inv = l == 0.f ? 0.f : 1.f / l;
     if (ok) {
         T* out = const_cast<T*>(at<T>(z.o, z.d.o_strides, b, i, h));
+        T* rest = z.d.o_rest ? static_cast<T*>(z.d.o_rest) + (out - static_cast<T*>(z.o)) : nullptr;
 #pragma unroll
         for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int c = 32 * db + 8 * g + 4 * hl;
-                const float v[4] = {o[db][4 * g] * inv, o[db][4 * g + 1] * inv, o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv};
-                if (c < z.d.dim) store<4>(out + c, v);
+                float v[4] = {o[db][4 * g] * inv, o[db][4 * g + 1] * inv, o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv};
+                if (c >= z.d.dim) continue;
+                store<4>(out + c, v);
+                if (rest) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = static_cast<float>(lost<T>(v[e]));
+                    store<4>(rest + c, v);
+                }
             }
         if (hl == 0 && z.lse) z.lse[(b * z.d.q_heads + h) * z.d.q_len + i] = l == 0.f ? -INFINITY : (m + sh.add) * kLn2 + logf(l);
     }
@@ -1138,7 +1158,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_split(Attn
     const Shape sh = Shape::of<T>(d);
     const Kind kind = kind_of<CAP, BIAS>(d);
     const Query q = query_of(sc, i, ok);
-    const float slope2 = d.slopes ? d.slopes[h] * kLog2e : 0.f;
+    const float slope = d.slopes ? d.slopes[h] : 0.f;
     Frag<T> qf[DP / 16];
     row_frags<T, DP>(at<T>(d.q, d.q_strides, b, i, h), ok && q.limit > 0, d.dim, qf);
 
@@ -1206,8 +1226,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_split(Attn
         f32x16 s = zero16(), unused;
 #pragma unroll
         for (int c = 0; c < DP / 16; ++c) s = Mma<T>::mul(L::row_frag(kc, 0, c), qf[c], s);
-        if (marked) scores<T, false, 2>(s, kind, sh, slope2, q, mine, key0 - 32 * sub, sub, unused, unused);
-        else scores<T, false, 1>(s, kind, sh, slope2, q, mine, key0 - 32 * sub, sub, unused, unused);
+        if (marked) scores<T, false, 2>(s, kind, sh, slope, q, mine, key0 - 32 * sub, sub, unused, unused);
+        else scores<T, false, 1>(s, kind, sh, slope, q, mine, key0 - 32 * sub, sub, unused, unused);
         float top = -INFINITY;
 #pragma unroll
         for (int x = 0; x < 16; ++x) top = fmaxf(top, s[x]);
@@ -1281,6 +1301,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_split(Attn
                 const float v = sum[y * kLd + e] * inv;
                 bad = bad || !(fabsf(v) < INFINITY);
                 out[e] = static_cast<T>(v);
+                if (d.o_rest) static_cast<T*>(d.o_rest)[out - static_cast<T*>(a.o) + e] = lost<T>(v);
             }
             if (lane == 0 && a.lse) a.lse[row] = ly == 0.f ? -INFINITY : (my + sh.add) * kLn2 + logf(ly);
             if (__ballot(bad)) row_forward<T>(a, sc, b, hh, ii, scratch[w]);   // see k_attn_fwd
@@ -1320,6 +1341,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
         if (lane + 64 * e < d.dim) {
             bad = bad || !(fabsf(v[e] * inv) < INFINITY);
             out[lane + 64 * e] = static_cast<T>(v[e] * inv);
+            if (d.o_rest) static_cast<T*>(d.o_rest)[out - static_cast<T*>(a.o) + lane + 64 * e] = lost<T>(v[e] * inv);
         }
     if (lane == 0 && a.lse) a.lse[row] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
     if (__ballot(bad)) row_forward<T>(a, Scope(d, b), b, h, i, scratch[w]);
@@ -1360,7 +1382,7 @@ __global__ __launch_bounds__(256 * TEAMS, sizeof(T) == 2 ? 2 : 1) void k_attn_dq
     const int64_t row = (b * d.q_heads + h) * d.q_len + i;
     const bool ok = i < d.q_len;
     const Query q = query_of(sc, i, ok);
-    const float slope2 = d.slopes ? d.slopes[h] * kLog2e : 0.f;
+    const float slope = d.slopes ? d.slopes[h] : 0.f;
     const float lse = ok ? a.g.lse[row] : -INFINITY;
     const bool live = ok && q.limit > 0 && lse != -INFINITY;
     const float base = live ? sh.add - lse * kLog2e : -INFINITY;         // of a query that sees nothing every weight is 0
@@ -1374,6 +1396,13 @@ __global__ __launch_bounds__(256 * TEAMS, sizeof(T) == 2 ? 2 : 1) void k_attn_dq
         for (int c = 0; c < DP / 16; ++c)
 #pragma unroll
             for (int e = 0; e < 8; ++e) delta += static_cast<float>(df[c][e]) * static_cast<float>(of[c][e]);
+        if (d.o_rest) {
+            row_frags<T, DP>(at<T>(d.o_rest, d.o_strides, b, ok ? i : 0, h), live, d.dim, of);
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) delta += static_cast<float>(df[c][e]) * static_cast<float>(of[c][e]);
+        }
         delta = halves_sum(delta);
         if (ok && hl == 0 && !team) a.delta[row] = delta;
     }
@@ -1467,7 +1496,7 @@ __global__ __launch_bounds__(256 * TEAMS, sizeof(T) == 2 ? 2 : 1) void k_attn_dq
                 dp = Mma<T>::mul(L::row_frag(vc, 32 * n, c), df[c], dp);
             }
             if constexpr (sizeof(T) == 2) paced<DP / 8, 1, 4>();
-            scores<T, true, MASK>(x, kind, sh, slope2, q, al[turn], key0, n, grad, far);
+            scores<T, true, MASK>(x, kind, sh, slope, q, al[turn], key0, n, grad, far);
             if constexpr (MASK != 0) {     // a weight of 0 may meet a value that is not finite
 #pragma unroll
                 for (int r = 0; r < 16; ++r) dp[r] = x[r] == -INFINITY ? 0.f : dp[r];
@@ -1478,12 +1507,16 @@ __global__ __launch_bounds__(256 * TEAMS, sizeof(T) == 2 ? 2 : 1) void k_attn_dq
                 dp[r] *= x[r];
             }
             if (kind.bias && slopes_too) {
+                float u = 0.f, v = 0.f, y = 0.f;       // sums of their own first: thousands of terms lose little so
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    pf = fmaf(x[r], far[r], pf);
-                    e0 += dp[r];
-                    e1 = fmaf(dp[r], far[r], e1);
+                    u = fmaf(x[r], far[r], u);
+                    v += dp[r];
+                    y = fmaf(dp[r], far[r], y);
                 }
+                pf += u;
+                e0 += v;
+                e1 += y;
             }
             if (kind.cap) {
 #pragma unroll
@@ -1740,7 +1773,7 @@ __global__ __launch_bounds__((dkv_threads<T, DP>()), sizeof(T) == 2 ? 2 : 1) voi
     auto work = [&](auto mask) {
         constexpr int MASK = decltype(mask)::value;
         const int turn1 = turn == 2 ? 0 : turn + 1, turn2 = turn1 == 2 ? 0 : turn1 + 1;
-        const float slope2 = kind.bias ? d.slopes[kvh * group + cur.g] * kLog2e : 0.f;
+        const float slope = kind.bias ? d.slopes[kvh * group + cur.g] : 0.f;
         const Rows& rw = rows[turn];
         const typename L::Lane qc = lanes.at_tile(qt + buf * kTile + row_half * L::kRowBytes);
         const typename L::Lane dc = lanes.at_tile(dt + buf * kTile + row_half * L::kRowBytes);
@@ -1809,7 +1842,7 @@ __global__ __launch_bounds__((dkv_threads<T, DP>()), sizeof(T) == 2 ? 2 : 1) voi
                         for (int e = 0; e < 4; ++e) f[e] = fabsf(static_cast<float>(v[e] - j));
                     }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[4 * c + e] = fmaf(-slope2, f[e], x[4 * c + e] * sh.raw);
+                    for (int e = 0; e < 4; ++e) x[4 * c + e] = fmaf(-slope, f[e], x[4 * c + e] * sh.raw);
                 }
             }
 #pragma unroll

@@ -301,7 +301,7 @@ class _Side:
         return (self.q_pos, self.k_pos, self.q_doc, self.k_doc, self.k_lengths, self.prefix)
 
 
-def _attention_desc(q, k, v, slopes, side, o):
+def _attention_desc(q, k, v, slopes, side, o, rest):
     B, Tq, H, D = q.shape
 
     def per_batch(t, dims):
@@ -311,7 +311,7 @@ def _attention_desc(q, k, v, slopes, side, o):
         B, Tq, k.shape[1], *_call_strides(q), *_call_strides(k), *_call_strides(v), *_strides(o), per_batch(side.q_pos, 3),
         per_batch(side.k_pos, 3), per_batch(side.q_doc, 2), per_batch(side.k_doc, 2), q.data_ptr(), k.data_ptr(),
         v.data_ptr(), *(0 if t is None else t.data_ptr() for t in (slopes, side.q_pos, side.k_pos, side.q_doc, side.k_doc,
-                                                                    side.k_lengths, side.prefix)),
+                                                                    side.k_lengths, side.prefix, rest)),
         side.scale, side.cap, H, k.shape[2], D, DTYPES[q.dtype], 0 if side.q_pos is None else side.q_pos.shape[-1],
         side.causal)
 
@@ -322,21 +322,23 @@ def _workspace(d, backward, device):
     return torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None, need.value
 
 
-def _attend(q, k, v, slopes, side, want_lse):
+def _attend(q, k, v, slopes, side, want_lse, want_rest):
+    """o, the scores' log-sum-exp, and for a backward pass what rounding o took from it (nothing in float32)."""
     B, Tq, H, _ = q.shape
     o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    rest = torch.empty_like(o) if want_rest and q.dtype != torch.float32 else None
     lse = torch.empty((B, H, Tq), dtype=torch.float32, device=q.device) if want_lse else None
-    d = _attention_desc(q, k, v, slopes, side, o)
+    d = _attention_desc(q, k, v, slopes, side, o, rest)
     ws, size = _workspace(d, 0, q.device)
     _call(q.get_device(), _lib.token_calls().attention_forward, d, o.data_ptr(), _ptr(lse), _ptr(ws), size)
-    return o, lse
+    return o, lse, rest
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, slopes, side):
-        o, lse = _attend(q, k, v, slopes, side, True)
-        ctx.save_for_backward(q, k, v, slopes, o, lse, *side.tensors())
+        o, lse, rest = _attend(q, k, v, slopes, side, True, True)
+        ctx.save_for_backward(q, k, v, slopes, o, lse, rest, *side.tensors())
         ctx.side = side
         ctx.mark_non_differentiable(lse)
         return o, lse
@@ -344,7 +346,7 @@ class _Attention(torch.autograd.Function):
     @staticmethod
     def backward(ctx, do, _):
         _first_order()
-        q, k, v, slopes, o, lse = ctx.saved_tensors[:6]
+        q, k, v, slopes, o, lse, rest = ctx.saved_tensors[:7]
         want = ctx.needs_input_grad
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if w else None
                       for t, w in zip((q, k, v), want))
@@ -352,7 +354,7 @@ class _Attention(torch.autograd.Function):
         if not q.numel() or not k.numel():
             return tuple(None if t is None else t.zero_() for t in (dq, dk, dv, dslopes)) + (None,)
         do = _lined_up(do)
-        d = _attention_desc(q, k, v, slopes, ctx.side, o)
+        d = _attention_desc(q, k, v, slopes, ctx.side, o, rest)
         none = (0, 0, 0)
         g = _lib.GRADS_PACK.pack(o.data_ptr(), do.data_ptr(), lse.data_ptr(),
                                  *(0 if t is None else t.data_ptr() for t in (dq, dk, dv, dslopes)), *_call_strides(do),
@@ -437,5 +439,5 @@ def attention(q, k, v, *, scale=None, cap=0.0, slopes=None, q_positions=None, k_
     if _wants_grad(q, k, v, slopes):
         o, lse = _Attention.apply(q, k, v, slopes, s)
     else:
-        o, lse = _attend(q, k, v, slopes, s, return_lse)
+        o, lse, _ = _attend(q, k, v, slopes, s, return_lse, False)
     return (o, lse) if return_lse else o
