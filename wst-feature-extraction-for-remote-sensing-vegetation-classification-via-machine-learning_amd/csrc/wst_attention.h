@@ -1161,8 +1161,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_split(Attn
     const float slope = d.slopes ? d.slopes[h] : 0.f;
     Frag<T> qf[DP / 16];
     row_frags<T, DP>(at<T>(d.q, d.q_strides, b, i, h), ok && q.limit > 0, d.dim, qf);
-
-    if (d.scale < 0.f) negate<T, DP>(qf);
     const int end = sc.limit(static_cast<int>(d.q_len) - 1);
     // this split's keys, in whole groups of 128: a wave has 32 of each
     const int groups = end > 0 ? (end + 127) / 128 : 0, per = (groups + a.splits - 1) / a.splits;
@@ -1208,6 +1206,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_split(Attn
     const typename L::Lane lanes = L::lane();
     int g = wanted(g0);
     if (g < g1) fetch(g * 128 + 32 * w);
+    if (d.scale < 0.f) negate<T, DP>(qf);      // after the keys' loads: it waits for the queries
     while (g < g1) {
         const int key0 = g * 128 + 32 * w;
         __builtin_amdgcn_wave_barrier();
@@ -1325,14 +1324,28 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
     m = wave_max(m);
     const float base = fmaxf(m, -3.0e38f);
     float l = 0.f, v[2] = {0.f, 0.f};
-    for (int s = 0; s < a.splits; ++s) {
-        const int64_t slot = s * all + row;
-        const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * slot] - base);
-        l += f * a.part_ml[2 * slot + 1];
+    for (int s0 = 0; s0 < a.splits; s0 += 64) {
+        const int count = min(a.splits - s0, 64);
+        float mine = 0.f;              // the lane's split's factor
+        if (lane < count) {
+            const int64_t slot = (s0 + lane) * all + row;
+            mine = __builtin_amdgcn_exp2f(a.part_ml[2 * slot] - base);
+            l = fmaf(mine, a.part_ml[2 * slot + 1], l);
+        }
+        for (int s = 0; s < count; s += 8) {           // eight splits' loads at a time
+            float x[8][2];
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-            if (lane + 64 * e < d.dim) v[e] += f * a.part[slot * d.dim + lane + 64 * e];
+            for (int u = 0; u < 8; ++u)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    x[u][e] = s + u < count && lane + 64 * e < d.dim ? a.part[((s0 + s + u) * all + row) * d.dim + lane + 64 * e] : 0.f;
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) v[e] = fmaf(__shfl(mine, (s + u) & 63), x[u][e], v[e]);
+        }
     }
+    l = wave_sum(l);
     const float inv = l == 0.f ? 0.f : 1.f / l;
     T* out = const_cast<T*>(at<T>(a.o, d.o_strides, b, i, h));
     bool bad = false;

@@ -86,7 +86,8 @@ AttnPlan plan_of(const wst_attention_desc& d, bool tiles) {
         const int64_t blocks = d.batch * d.q_heads * ((d.q_len + kBQ - 1) / kBQ);
         const int64_t row_tiles = (group * d.q_len + 31) / 32, cells = d.batch * d.k_heads * row_tiles;
         if (d.q_len <= 32 || (blocks < 128 && d.k_len >= 1024)) {
-            int64_t s = (1024 + cells - 1) / cells, most = (d.k_len + 255) / 256;
+            // two blocks a CU, all at once (64 queries over 4096 keys, 2 x 64: 512 blocks 29 us, 1024 34)
+            int64_t s = (512 + cells - 1) / cells, most = (d.k_len + 255) / 256;
             s = s < most ? s : most;
             p.splits = static_cast<int>(s < 1 ? 1 : s > 256 ? 256 : s);
             if (p.splits > 1) p.forward = static_cast<size_t>(p.splits) * rows * (d.dim + 2);
