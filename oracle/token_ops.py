@@ -163,21 +163,23 @@ def attention(q, k, v, *, scale=None, cap=0.0, slopes=None, q_positions=None, k_
             e_row = (e.max(1, keepdim=True)[0]) * 2 + (Tk + 24) * U32   # of p, relative: its own and the sum's
             out["lse"][1][b, h] = (e_row + 4 * U32 * (1 + torch.where(torch.isfinite(top), top, 0.0).abs()))[:, 0]
             o = p @ V
-            e_o = (u + e_row) * (p @ V.abs())
+            # a weight below float32's normal numbers may be taken for 0
+            least = torch.where(S, torch.finfo(torch.float32).tiny, 0.0).to(F64)
+            e_o = (u + e_row) * (p @ V.abs()) + least @ V.abs()
             out["o"][0][b, :, h] = o
             out["o"][1][b, :, h] = half(dtype) * o.abs() + e_o + tiny(dtype)
             if do is None:
                 continue
             G = torch.where(rows[:, None], do[b, :, h].to(F64), 0.0)
             out["dv"][0][b, :, c] += p.T @ G
-            out["dv"][1][b, :, c] += (p * (u + e_row + Tq * U32)).T @ G.abs()
+            out["dv"][1][b, :, c] += (p * (u + e_row + Tq * U32) + least).T @ G.abs()
             dp = G @ V.T
             delta = (p * dp).sum(1, keepdim=True)
             ds = p * (dp - delta)
-            # delta is taken from the rounded output
-            e_delta = (G.abs() * (out["o"][1][b, :, h] + (D + 4) * U32 * o.abs())).sum(1, keepdim=True)
+            # delta is taken from the output and what rounding took from it
+            e_delta = (G.abs() * (e_o + tiny(dtype) + (half(dtype) ** 2 + (2 * D + 8) * U32) * o.abs())).sum(1, keepdim=True)
             e_dp = (D + 4) * U32 * (G.abs() @ V.abs().T)
-            e_ds = p * (e_dp + e_delta) + ds.abs() * (e_row + 4 * U32) + 2 * U32 * p * (dp.abs() + delta.abs())
+            e_ds = least * (dp.abs() + delta.abs()) + p * (e_dp + e_delta) + ds.abs() * (e_row + 4 * U32) + 2 * U32 * p * (dp.abs() + delta.abs())
             if slopes is not None:
                 out["dslopes"][0][h] += -(ds * far).sum()
                 out["dslopes"][1][h] += ((e_ds + (Tk + Tq + B * Tq) * U32 * ds.abs()) * far).sum()

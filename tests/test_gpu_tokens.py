@@ -1,5 +1,6 @@
 """GPU tests of the token operators (wst_amd.tokens) against their float64 restatement (oracle/token_ops.py), whose
 bounds on rounding are the tolerances: every value must lie within its own."""
+import ctypes
 import math
 
 import pytest
@@ -531,3 +532,105 @@ def test_attention_gradient_of_rows_with_one_large_weight(D, Tq, causal, dtype):
     rows = slice(1, None)                                # query 0 in order sees key 0 alone: no gradient
     off = (dq - want)[:, rows].norm() / want[:, rows].norm()
     assert float(off) < 0.07, float(off)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("order", ["rising", "falling", "mixed"])
+def test_attention_scores_that_outgrow_the_first_maximum(D, order, dtype):
+    """Scores that grow by 58 powers of two from one tile of keys to the next: the running maximum has to move, for some
+    queries of a wave and not for others, in both directions of a walk and in order."""
+    T = 330
+    g = _gen(D)
+    step = torch.arange(T) // 64
+    step = {"rising": step, "falling": step.flip(0), "mixed": step[torch.randperm(T, generator=g)]}[order].float()
+    gain = torch.where(torch.arange(T) % 3 == 0, 40.0, torch.where(torch.arange(T) % 3 == 1, -7.0, 0.0))
+    q = (gain[:, None].expand(T, D) * D ** -0.5).reshape(1, T, 1, D).repeat(1, 1, 2, 1)
+    k = step[:, None].expand(T, D).reshape(1, T, 1, D).clone()
+    q, k = q + 0.01 * torch.randn(1, T, 2, D, generator=g), k + 0.01 * torch.randn(1, T, 1, D, generator=g)
+    v, do = torch.randn(1, T, 1, D, generator=g), torch.randn(1, T, 2, D, generator=g)
+    q, k, v, do = (t.to(dtype) for t in (q, k, v, do))
+    for kw in (dict(), dict(causal=True), dict(q_documents=_documents(g, 1, T, 2, 0.05), k_documents=_documents(g, 1, T, 2, 0.05))):
+        _check_attention(q, k, v, do, **kw)
+    _check_attention(q[:, 4:7], k, v, do[:, 4:7], train=False)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("scale", [-0.3, 0.0, -0.0])
+@pytest.mark.parametrize("Tq,D", [(150, 64), (150, 12), (2, 64), (140, 128)])
+def test_attention_scales_of_any_sign(Tq, D, scale, dtype):
+    q, k, v, do, g = _attention_inputs(1, Tq, 1100 if Tq == 2 else 150, 4, 2, D, dtype, 31)
+    slopes = torch.rand(4, generator=g)
+    for kw in (dict(), dict(cap=2.0), dict(slopes=slopes, causal=True), dict(cap=2.0, slopes=-slopes)):
+        _check_attention(q, k, v, do, scale=scale, **kw)
+
+
+@pytest.mark.parametrize("B,T,H,Hk,D", [(1, 700, 6, 1, 64), (1, 300, 5, 1, 128), (1, 64, 7, 1, 96), (60, 130, 10, 1, 32),
+                                        (1, 400, 12, 4, 128), (2, 129, 3, 1, 80), (1, 193, 1, 1, 64)])
+@pytest.mark.parametrize("how", ["plain", "causal", "documents"])
+def test_attention_heads_in_parts(B, T, H, Hk, D, how):
+    """Sums of dk and dv in parts: whole heads a part, whole parts a head, and neither."""
+    q, k, v, do, g = _attention_inputs(B, T, T, H, Hk, D, BF16, T + H)
+    docs = _documents(g, B, T, 3)
+    kw = {"plain": {}, "causal": dict(causal=True, slopes=torch.rand(H, generator=g) * 0.1),
+          "documents": dict(q_documents=docs, k_documents=docs, causal=True)}[how]
+    _check_attention(q, k, v, do, **kw)
+
+
+def _bare_call(q, k, v, do, lse, o, causal=True):
+    """The C entries on the tensors as they lie: forward, then backward; returns dq, dk, dv."""
+    lib = _lib.load()
+    B, T, H, D = q.shape
+    d = _lib.AttentionDesc(batch=B, q_len=T, k_len=k.shape[1], q_strides=q.stride()[:3], k_strides=k.stride()[:3],
+                           v_strides=v.stride()[:3], o_strides=o.stride()[:3], q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(),
+                           scale=D ** -0.5, q_heads=H, k_heads=k.shape[2], dim=D, dtype=tokens.DTYPES[q.dtype], causal=causal)
+    need, st = ctypes.c_size_t(), torch.cuda.current_stream().cuda_stream
+    for backward in (0, 1):
+        assert lib.wst_attention_workspace(d, backward, ctypes.byref(need)) == 0
+        ws = torch.empty(need.value + 1, dtype=torch.uint8, device="cuda")
+        if not backward:
+            assert lib.wst_attention_forward(d, o.data_ptr(), lse.data_ptr(), ws.data_ptr(), need.value, st) == 0
+    out = [torch.empty_like(t) for t in (q, k, v)]
+    g = _lib.AttentionGrads(o=o.data_ptr(), d_o=do.data_ptr(), lse=lse.data_ptr(), dq=out[0].data_ptr(), dk=out[1].data_ptr(),
+                            dv=out[2].data_ptr(), do_strides=do.stride()[:3], dq_strides=out[0].stride()[:3],
+                            dk_strides=out[1].stride()[:3], dv_strides=out[2].stride()[:3])
+    assert lib.wst_attention_backward(d, g, ws.data_ptr(), need.value, st) == 0
+    torch.cuda.synchronize()
+    return out
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("odd", ["q", "k", "do", "none"])
+def test_attention_c_entries_without_alignment(odd, dtype):
+    """Rows that do not begin on 16 bytes are taken value by value, each call by its own tensors. Without o_rest delta is
+    that of the rounded output, which the tolerance counts: |do| |o| half an eps for each ds."""
+    B, T, H, Hk, D = 1, 140, 2, 1, 64
+    q, k, v, do, _ = _attention_inputs(B, T, T, H, Hk, D, dtype, 77)
+    want = ref.attention(q, k, v, causal=True, do=do)
+
+    def place(t, name):
+        flat = torch.empty(t.numel() + 8, dtype=dtype, device="cuda")
+        out = flat[1 if name == odd else 0:][:t.numel()].view(t.shape)
+        return out.copy_(t)
+
+    qd, kd, vd, dod = place(q, "q"), place(k, "k"), place(v, "v"), place(do, "do")
+    o, lse = torch.empty_like(qd), torch.empty(B, H, T, device="cuda")
+    grads = _bare_call(qd, kd, vd, dod, lse, o)
+    _hold(o, want["o"], "o")
+    _hold(lse, want["lse"], "lse")
+    p, lost = torch.exp(-want["lse"][0]), torch.finfo(dtype).eps / 2 * (do.double().abs() * want["o"][0].abs()).sum(-1)
+    z = q.double().permute(0, 2, 1, 3) @ k.double().repeat_interleave(H // Hk, 2).permute(0, 2, 3, 1) * D ** -0.5
+    p = torch.where(torch.ones(T, T).tril().bool(), torch.exp(z) * p[..., None], 0.0) * lost.transpose(1, 2)[..., None] * D ** -0.5
+    kk, qq = k.double().abs().repeat_interleave(H // Hk, 2).transpose(1, 2), q.double().abs().transpose(1, 2)
+    extra = {"dq": (p @ kk).transpose(1, 2), "dk": (p.transpose(2, 3) @ qq).sum(1, keepdim=True).transpose(1, 2), "dv": 0.0}
+    for t, name in zip(grads, ("dq", "dk", "dv")):
+        _hold(t, (want[name][0], want[name][1] + extra[name]), name)
+
+
+def test_first_order_gradients_only():
+    x = torch.randn(3, 8, device="cuda", requires_grad=True)
+    q = torch.randn(1, 3, 1, 8, device="cuda", requires_grad=True)
+    pos = torch.arange(3, dtype=torch.int32, device="cuda")[:, None]
+    for y, leaf in ((tokens.layer_norm(x), x), (tokens.rotary(q, pos, (4,)), q), (tokens.attention(q, q, q), q)):
+        with pytest.raises(RuntimeError, match="first-order"):
+            torch.autograd.grad(y.sum(), leaf, create_graph=True)
