@@ -789,7 +789,8 @@ struct AlongStage {
 
 // The kinds of scores a kernel is compiled for: CAP 0 or 1; BIAS 0 none, 1 by place, 2 by coordinates; 2 and 3 stand for
 // "as the call says". Branches on these inside the loop over tiles cost more than the branch: the compiler moves whole
-// tiles of registers where the ways meet (measured at 8192 x 8 heads x 128, no cap, no bias: 318 us with such branches).
+// tiles of registers where the ways meet (forward, 8192 x 8 heads x 128, no cap, no bias: 318 us with such branches, 300
+// without, in one process).
 // float32, whose products take sixteen times as long, has the one general kernel.
 struct Kind {
     bool cap, bias, coordinates;
@@ -897,6 +898,9 @@ constexpr int kBQ = 128, kBK = 64;
 // LDS, and join their maxima, sums and outputs at the end: the block with the longest rows of an order does not run on
 // alone at half the rate. Where all blocks are as long, two independent blocks are better than two teams that wait for
 // each other at every tile (8192 x 8 heads x 128: in order 238 -> 201 us, dq 283 -> 250; not in order 327 -> 379).
+//
+// Bound by the matrix units and, with a cap or a bias, as much by what a score takes besides: 8192 x 8 heads of 128
+// 327 us, 840 TFLOP/s; in order 201 us; with cap 50 and a prefix 262 us.
 template <typename T, int DP, int CAP, int BIAS, int TEAMS>
 __global__ __launch_bounds__(256 * TEAMS, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(AttnArgs a) {
     using L = Tile<T, DP>;
@@ -1131,7 +1135,8 @@ __global__ __launch_bounds__(256 * TEAMS, sizeof(T) == 2 ? 2 : 1) void k_attn_fw
 
 // Few queries over many keys: the queries of all heads that share a key head make up to 32 rows, and the keys are split
 // over blocks, and in a block over its waves, each of which walks its own tiles of 32 keys through its own part of LDS
-// with nothing to wait for. The parts are joined by their maxima and sums, in the block and then by k_attn_join.
+// with nothing to wait for. The parts are joined by their maxima and sums, in the block and then by k_attn_join. Bound by
+// memory: 64 queries of 8 heads over 64 x 3/4 of 4096 keys of 2 x 64 in bfloat16, 100 MB: 29 us, 3.5 TB/s.
 template <typename T, int DP, int CAP, int BIAS>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_split(AttnArgs a) {
     using L = Tile<T, DP>;
@@ -1370,7 +1375,7 @@ inline constexpr float kUp<f16> = 64.f;
 
 // dq, the slopes' shares and delta: walks the keys as the forward pass does. Scores come back as (keys x queries), so
 // their gradient is the operand of dq^T = k^T dz^T as it stands; keys are read from LDS both ways. delta goes in as the
-// product's starting value.
+// product's starting value. 8192 x 8 heads of 128: 400 us, 1030 TFLOP/s; in order 250 us; with cap 50 and a prefix 327.
 template <typename T, int DP, int CAP, int BIAS, int TEAMS>
 __global__ __launch_bounds__(256 * TEAMS, sizeof(T) == 2 ? 2 : 1) void k_attn_dq(AttnArgs a) {
     using L = Tile<T, DP>;
@@ -1621,9 +1626,12 @@ constexpr int dkv_threads() { return sizeof(T) == 2 && DP > 64 ? 512 : 256; }
 // dk^T = q^T dz as they stand. With few key tiles the walk is split in parts whose sums k_attn_dkv_join adds in order.
 //
 // Heads up to 64 wide (and float32): four waves, keys and values held as operands in registers. Wider ones would then
-// leave room for one wave a SIMD, which waits for LDS most of its time (8192 x 8 heads x 128, cap and prefix: 870 us).
-// They take eight waves: keys and values stay in LDS, two waves share 32 keys and take half of each tile's queries, and
-// add their sums at the end.
+// leave room for one wave a SIMD, which waits for LDS most of its time (8192 x 8 heads x 128, cap and prefix: 870 us,
+// with eight waves 694). They take eight waves: keys and values stay in LDS, two waves share 32 keys and take half of
+// each tile's queries, and add their sums at the end.
+//
+// Bound by the matrix units and, with a cap or a bias, as much by what a score takes besides. 8192 x 8 heads of 128:
+// 670 us, 820 TFLOP/s, of 1137 that a library product of 8192^3 reaches here.
 template <typename T, int DP, int CAP, int BIAS>
 __global__ __launch_bounds__((dkv_threads<T, DP>()), sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnArgs a) {
     using L = Tile<T, DP>;

@@ -129,7 +129,8 @@ __device__ __forceinline__ void load_w(const void* w, int wdt, float none, I col
     }
 }
 
-// One row per TPR threads, its values in registers (CH chunks of VEC a thread): x is read once.
+// One row per TPR threads, its values in registers (CH chunks of VEC a thread): x is read once. 32768 rows of 1024 in
+// bfloat16: 30 us, 4.5 TB/s, of 4.9 that a large copy reaches.
 template <typename Tx, typename Ty, int VEC, int CH, int TPR>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_rows(NormArgs a) {
     __shared__ float slot[(TPR > 256 ? TPR : 256) / 64];
@@ -219,7 +220,9 @@ __global__ __launch_bounds__(1024) void k_norm_long(NormArgs a) {
 
 // Backward pass of rows: a block walks rows block, block + groups, ...; dx leaves at once, the thread's columns of dw
 // and db stay in its registers until the block has added its waves' up and writes one partial row of each. The
-// partials are added in a fixed order (k_norm_fold), so results repeat bit for bit.
+// partials are added in a fixed order (k_norm_fold), so results repeat bit for bit. A wave has the next row's loads under
+// way while it works on one; with a row in one piece of code for whole and for ragged chunks (not WHOLE) the compiler
+// waits for them at once. 32768 rows of 1024 in bfloat16: 53 us, 3.8 TB/s (70 without the loads ahead).
 template <typename Tx, typename Ty, int VEC, int CH, int TPR, bool WHOLE>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_bwd_rows(NormArgs a) {
     constexpr int kThreads = TPR > 256 ? TPR : 256, kRows = kThreads / TPR;
@@ -422,7 +425,9 @@ constexpr int kPack = sizeof(Ty) == 2 ? 2 : 1;
 // A block takes tp points of one batch entry with all n values into LDS, then a wave takes its points' mean and variance
 // out of LDS, and at last writes their rows whole, some columns at a time, with the weights of those columns in
 // registers: one read of x. For n * 16 values that fit the LDS. PLAIN: weight and bias are there, in float32 (a branch on
-// their type at every value took as many instructions as all else).
+// their type at every value took as many instructions as all else: 128 us then).
+// 160 x 1024 points of 243 in float32: 77 us, 4.1 TB/s. 1024 x 16 points of 1251, bfloat16 out: 39 us, 3.1 TB/s: there a
+// block's 80 KB of LDS leave room for two blocks a CU, which wait together for memory at their start.
 template <typename Tx, typename Ty, bool PLAIN>
 __global__ __launch_bounds__(kMapBig) void k_norm_maps(NormArgs a, int tp, int ld) {
     extern __shared__ float tile[];
@@ -505,7 +510,7 @@ __global__ __launch_bounds__(kMapBig) void k_norm_maps(NormArgs a, int tp, int l
 
 constexpr int kPts = 16, kCols = 256, kLd = 260;   // tile of the sweeps over longer maps: 260 = 4 modulo 16
 
-// Maps whose n * 16 values exceed the LDS (c5: 8932): mean, variance and output in three sweeps over tiles of 256
+// Maps whose n * 16 values exceed the LDS (four bands, J=6, L=12: 8932): mean, variance and output in three sweeps over tiles of 256
 // columns of 16 points, the later ones out of the caches.
 template <typename Tx, typename Ty>
 __global__ __launch_bounds__(kMapThreads) void k_norm_maps_long(NormArgs a) {
@@ -602,7 +607,7 @@ constexpr int kBCols = 512, kBLd = 516;      // 516 = 4 modulo 16
 
 // dx and the partial dw, db of maps: a block keeps 512 columns and walks tiles of 16 points, a thread two columns and
 // half of the points; the next tile of x and dy is on its way while one is worked on. No sums over n are needed here, so
-// any n goes through the same tile.
+// any n goes through the same tile. 1024 x 16 points of 1251, dy bfloat16, weight and bias alone: 40 us, 3.1 TB/s.
 template <typename Tx, typename Ty>
 __global__ __launch_bounds__(kMapThreads) void k_norm_bwd_maps(NormArgs a) {
     __shared__ float tile[kPts * kBLd];
