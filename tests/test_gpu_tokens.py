@@ -634,3 +634,15 @@ def test_first_order_gradients_only():
     for y, leaf in ((tokens.layer_norm(x), x), (tokens.rotary(q, pos, (4,)), q), (tokens.attention(q, q, q), q)):
         with pytest.raises(RuntimeError, match="first-order"):
             torch.autograd.grad(y.sum(), leaf, create_graph=True)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("Tq,Tk,H,Hk,D", [(100, 1500, 2, 1, 64), (1100, 1100, 1, 1, 32), (1030, 2000, 2, 2, 128), (33, 1024, 3, 1, 96)])
+def test_attention_few_blocks_over_many_keys(Tq, Tk, H, Hk, D, dtype):
+    """Too few queries to fill the chip: keys are split for these too, with documents, order and a length."""
+    q, k, v, do, g = _attention_inputs(1, Tq, Tk, H, Hk, D, dtype, Tq + D)
+    docs = {n: _documents(g, 1, t, 3) for n, t in (("q", Tq), ("k", Tk))}
+    slopes = torch.rand(H, generator=g) * 0.1
+    _check_attention(q, k, v, do, causal=True, slopes=slopes)
+    _check_attention(q, k, v, do, q_documents=docs["q"], k_documents=docs["k"], cap=4.0, causal=True,
+                     k_lengths=torch.tensor([Tk - 70], dtype=torch.int32))

@@ -9,8 +9,9 @@ learned counterpart, for training and inference:
 * ``attention``   -- scores capped by tanh, a bias that depends on distance, documents, order and a prefix.
 
 All run in the HIP library on the tensors' device and current stream, have gradients (torch autograd, first order), and
-can be captured into a graph.  float32, bfloat16 and float16; sums and statistics are held in float32.  There is no CPU
-execution: tensors must live on a ROCm GPU.
+can be captured into a graph (a backward pass: while no eager autograd graph of the same leaves is alive, since torch's
+engine would wait for that graph's stream inside the capture).  float32, bfloat16 and float16; sums and statistics are
+held in float32.  There is no CPU execution: tensors must live on a ROCm GPU.
 """
 from __future__ import annotations
 
@@ -102,24 +103,32 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _like(t):
+    """A new contiguous tensor of t's size and type; empty_like takes half the time of empty with its arguments."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _norm_forward(x, weight, bias, eps, out_dtype, stats):
     xs, view = _token_view(x)
-    y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
-    mean = rstd = None
-    if stats:
-        mean, rstd = torch.empty((2, view[0] * view[1]), dtype=torch.float32, device=x.device).unbind(0)
+    y = _like(x) if out_dtype == x.dtype else torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    rows = view[0] * view[1]
+    kept = mean = rstd = None
+    if stats:                                   # means, then 1 / deviations
+        kept = torch.empty(2 * rows, dtype=torch.float32, device=x.device)
+        mean = kept.data_ptr()
+        rstd = mean + 4 * rows
     if x.numel():
         d = _norm_desc(view, (0, 0, 0), x, out_dtype, weight, bias, eps)
         _call(x.get_device(), _lib.token_calls().layer_norm_forward, d, xs.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(),
-              _ptr(mean), _ptr(rstd))
-    return y, xs, mean, rstd
+              mean, rstd)
+    return y, xs, kept
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, out_dtype):
-        y, xs, mean, rstd = _norm_forward(x, weight, bias, eps, out_dtype, True)
-        ctx.save_for_backward(xs, weight, mean, rstd)
+        y, xs, kept = _norm_forward(x, weight, bias, eps, out_dtype, True)
+        ctx.save_for_backward(xs, weight, kept)
         ctx.bias_like = None if bias is None else (bias.shape, bias.dtype)
         ctx.eps, ctx.x_shape = eps, x.shape
         return y
@@ -127,14 +136,14 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         _first_order()
-        xs, weight, mean, rstd = ctx.saved_tensors
+        xs, weight, kept = ctx.saved_tensors
         want_x, want_w, want_b = ctx.needs_input_grad[:3]
         dx = dw = db = None
         dev = xs.device
         if want_w:
             dw = torch.empty_like(weight)
         if want_b:
-            db = torch.empty(ctx.bias_like[0], dtype=ctx.bias_like[1], device=dev)
+            db = torch.empty(ctx.bias_like[0], dtype=ctx.bias_like[1], device=dev) if weight is None else torch.empty_like(weight)
         if not xs.numel():
             return (torch.empty(ctx.x_shape, dtype=xs.dtype, device=dev) if want_x else None,
                     dw.zero_() if want_w else None, db.zero_() if want_b else None, None, None)
@@ -147,15 +156,15 @@ class _LayerNorm(torch.autograd.Function):
                 dview = (points * n, 1, points)
                 dx = dx.view(ctx.x_shape)
             else:
-                dx = torch.empty(ctx.x_shape, dtype=xs.dtype, device=dev)
+                dx = _like(xs)
         dy = dy.contiguous()
         d = _lib.NORM_PACK.pack(*view, *dview, DTYPES[xs.dtype], DTYPES[dy.dtype],
                                 DTYPES[weight.dtype] if weight is not None else DTYPES[db.dtype] if want_b else 0, ctx.eps)
         lib, need = _lib.token_calls(), ctypes.c_size_t()
         _lib.check_tokens(lib.layer_norm_workspace(d, ctypes.byref(need)))
         ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
-        _call(xs.get_device(), lib.layer_norm_backward, d, xs.data_ptr(), _ptr(weight), dy.data_ptr(), mean.data_ptr(),
-              rstd.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), ws.data_ptr(), need.value)
+        _call(xs.get_device(), lib.layer_norm_backward, d, xs.data_ptr(), _ptr(weight), dy.data_ptr(), kept.data_ptr(),
+              kept.data_ptr() + 4 * batch * points, _ptr(dx), _ptr(dw), _ptr(db), ws.data_ptr(), need.value)
         return dx, dw, db, None, None
 
 
@@ -227,11 +236,11 @@ def _call_strides(t):
 def _rotate(q, k, positions, sections, base, interleaved, inverse):
     q = _rows_of(q)
     B, T, H, D = q.shape
-    qo = torch.empty((B, T, H, D), dtype=q.dtype, device=q.device)
+    qo = _like(q)
     ko, ks, kos, Hk = None, (0, 0, 0), (0, 0, 0), 0
     if k is not None:
         k = _rows_of(k)
-        ko, Hk = torch.empty(k.shape, dtype=k.dtype, device=k.device), k.shape[2]
+        ko, Hk = _like(k), k.shape[2]
         ks, kos = _strides(k), _strides(ko)
     d = _lib.ROTARY_PACK.pack(B, T, *_strides(q), *ks, *_strides(qo), *kos, base, H, Hk, D, DTYPES[q.dtype], len(sections),
                               *sections, *(0,) * (_lib.MAX_AXES - len(sections)), interleaved, inverse, positions.dim() == 2)
@@ -294,26 +303,37 @@ def rotary(q, positions, sections, base=10000.0, interleaved=False, k=None):
 
 # ------------------------------------------------------------------------------------------ attention
 class _Side:
-    """The arguments of a call that have no gradient."""
-    __slots__ = ("scale", "cap", "q_pos", "k_pos", "q_doc", "k_doc", "k_lengths", "prefix", "causal")
+    """The arguments of a call that have no gradient, and their part of the descriptor."""
+    __slots__ = ("scale", "cap", "q_pos", "k_pos", "q_doc", "k_doc", "k_lengths", "prefix", "causal", "axes", "strides", "ptrs")
 
     def tensors(self):
         return (self.q_pos, self.k_pos, self.q_doc, self.k_doc, self.k_lengths, self.prefix)
 
+    def settle(self):
+        q_pos, k_pos, q_doc, k_doc, k_lengths, prefix = self.tensors()
+        self.axes = 0 if q_pos is None else q_pos.shape[-1]
+        self.strides = (_per_batch(q_pos, 3), _per_batch(k_pos, 3), _per_batch(q_doc, 2), _per_batch(k_doc, 2))
+        self.ptrs = (_ptr0(q_pos), _ptr0(k_pos), _ptr0(q_doc), _ptr0(k_doc), _ptr0(k_lengths), _ptr0(prefix))
+
+
+def _per_batch(t, dims):
+    return 0 if t is None or t.dim() < dims else t.stride(0)
+
+
+def _ptr0(t):
+    return 0 if t is None else t.data_ptr()
+
 
 def _attention_desc(q, k, v, slopes, side, o, rest):
     B, Tq, H, D = q.shape
-
-    def per_batch(t, dims):
-        return 0 if t is None or t.dim() < dims else t.stride(0)
-
     return _lib.ATTENTION_PACK.pack(
-        B, Tq, k.shape[1], *_call_strides(q), *_call_strides(k), *_call_strides(v), *_strides(o), per_batch(side.q_pos, 3),
-        per_batch(side.k_pos, 3), per_batch(side.q_doc, 2), per_batch(side.k_doc, 2), q.data_ptr(), k.data_ptr(),
-        v.data_ptr(), *(0 if t is None else t.data_ptr() for t in (slopes, side.q_pos, side.k_pos, side.q_doc, side.k_doc,
-                                                                    side.k_lengths, side.prefix, rest)),
-        side.scale, side.cap, H, k.shape[2], D, DTYPES[q.dtype], 0 if side.q_pos is None else side.q_pos.shape[-1],
-        side.causal)
+        B, Tq, k.shape[1], *_call_strides(q), *_call_strides(k), *_call_strides(v), *_strides(o), *side.strides, q.data_ptr(),
+        k.data_ptr(), v.data_ptr(), _ptr0(slopes), *side.ptrs, _ptr0(rest), side.scale, side.cap, H, k.shape[2], D,
+        DTYPES[q.dtype], side.axes, side.causal)
+
+
+def _grad_strides(t):
+    return (0, 0, 0) if t is None else t.stride()[:3]
 
 
 def _workspace(d, backward, device):
@@ -325,7 +345,7 @@ def _workspace(d, backward, device):
 def _attend(q, k, v, slopes, side, want_lse, want_rest):
     """o, the scores' log-sum-exp, and for a backward pass what rounding o took from it (nothing in float32)."""
     B, Tq, H, _ = q.shape
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    o = _like(q)
     rest = torch.empty_like(o) if want_rest and q.dtype != torch.float32 else None
     lse = torch.empty((B, H, Tq), dtype=torch.float32, device=q.device) if want_lse else None
     d = _attention_desc(q, k, v, slopes, side, o, rest)
@@ -348,17 +368,14 @@ class _Attention(torch.autograd.Function):
         _first_order()
         q, k, v, slopes, o, lse, rest = ctx.saved_tensors[:7]
         want = ctx.needs_input_grad
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if w else None
-                      for t, w in zip((q, k, v), want))
+        dq, dk, dv = _like(q) if want[0] else None, _like(k) if want[1] else None, _like(v) if want[2] else None
         dslopes = torch.empty_like(slopes) if want[3] else None
         if not q.numel() or not k.numel():
             return tuple(None if t is None else t.zero_() for t in (dq, dk, dv, dslopes)) + (None,)
         do = _lined_up(do)
         d = _attention_desc(q, k, v, slopes, ctx.side, o, rest)
-        none = (0, 0, 0)
-        g = _lib.GRADS_PACK.pack(o.data_ptr(), do.data_ptr(), lse.data_ptr(),
-                                 *(0 if t is None else t.data_ptr() for t in (dq, dk, dv, dslopes)), *_call_strides(do),
-                                 *(s for t in (dq, dk, dv) for s in (none if t is None else t.stride()[:3])))
+        g = _lib.GRADS_PACK.pack(o.data_ptr(), do.data_ptr(), lse.data_ptr(), _ptr0(dq), _ptr0(dk), _ptr0(dv), _ptr0(dslopes),
+                                 *_call_strides(do), *_grad_strides(dq), *_grad_strides(dk), *_grad_strides(dv))
         ws, size = _workspace(d, 1, q.device)
         _call(q.get_device(), _lib.token_calls().attention_backward, d, g, _ptr(ws), size)
         return dq, dk, dv, dslopes, None
@@ -435,6 +452,7 @@ def attention(q, k, v, *, scale=None, cap=0.0, slopes=None, q_positions=None, k_
         raise RuntimeError("cap must be finite and not negative")
     if not abs(s.scale) < float("inf"):
         raise RuntimeError("scale must be finite")
+    s.settle()
     q, k, v = _lined_up(q), _lined_up(k), _lined_up(v)
     if _wants_grad(q, k, v, slopes):
         o, lse = _Attention.apply(q, k, v, slopes, s)
