@@ -93,7 +93,11 @@ AttnPlan plan_of(const wst_attention_desc& d, bool tiles) {
             if (p.splits > 1) p.forward = static_cast<size_t>(p.splits) * rows * (d.dim + 2);
         }
         const int64_t items = group * ((d.q_len + 63) / 64), keys = d.batch * d.k_heads * ((d.k_len + kBQ - 1) / kBQ);
-        int64_t parts = keys ? (512 + keys - 1) / keys : 1;
+        // Blocks of dk and dv: two a CU, all at once; in order, where the first keys' walks are the longest, twice as many,
+        // so that short ones come in beside long ones (8192 x 8 heads x 64: 266 us, 193 and 22 for the join; wider heads
+        // have one block of eight waves a CU and are even as they are).
+        const int64_t want = d.causal && d.dim <= 64 && d.dtype != WST_F32 ? 1024 : 512;
+        int64_t parts = keys ? (want + keys - 1) / keys : 1;
         parts = parts < items / 2 ? parts : items / 2;
         parts = parts < 1 ? 1 : parts > 64 ? 64 : parts;
         // whole heads a part, or whole parts a head, where that takes less than twice as many (k_attn_dkv)
