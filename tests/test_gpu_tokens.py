@@ -646,3 +646,110 @@ def test_attention_few_blocks_over_many_keys(Tq, Tk, H, Hk, D, dtype):
     _check_attention(q, k, v, do, causal=True, slopes=slopes)
     _check_attention(q, k, v, do, q_documents=docs["q"], k_documents=docs["k"], cap=4.0, causal=True,
                      k_lengths=torch.tensor([Tk - 70], dtype=torch.int32))
+
+
+@pytest.mark.parametrize("layout,points,n", [("rows", 70000, 31000), ("maps", 9000000, 243), ("maps", 66000, 33000)])
+def test_layer_norm_offsets_past_32_bits(layout, points, n):
+    """More than 2^31 values: the last rows, whose gradient alone is not zero, are checked."""
+    last = 5
+    g = _gen(n)
+    x, w, b, dy = _norm_inputs(last, n, BF16, F32, n)
+    dy = dy.to(BF16)
+    want = ref.layer_norm(x, w, b, 1e-5, BF16, dy)
+    if layout == "rows":
+        xs = torch.zeros(points, n, dtype=BF16, device="cuda")
+    else:
+        xs = torch.zeros(n, points, dtype=BF16, device="cuda").t()
+    xs[-last:] = x.cuda()
+    xs.requires_grad_()
+    ws, bs = w.cuda().requires_grad_(), b.cuda().requires_grad_()
+    y = tokens.layer_norm(xs, ws, bs)
+    _hold(y[-last:], want["y"], "y")
+    assert torch.equal(y[0], b.cuda().to(BF16)) and torch.equal(y[points - last - 1], y[0])
+    dys = torch.zeros(points, n, dtype=BF16, device="cuda")
+    dys[-last:] = dy.cuda()
+    dx, dw, db = torch.autograd.grad(y, (xs, ws, bs), dys)
+    _hold(dx[-last:], want["dx"], "dx")
+    assert not bool(dx[0].any()) and not bool(dx[points - last - 1].any())
+    _hold(dw, want["dw"], "dw")
+    _hold(db, want["db"], "db")
+
+
+def test_rotary_offsets_past_32_bits():
+    T, H, D = 9000000, 4, 64
+    g = _gen(3)
+    x = torch.randn(1, 5, H, D, generator=g).to(BF16)
+    pos = torch.randint(-(1 << 20), 1 << 20, (5, 2), generator=g, dtype=torch.int32)
+    xs = torch.zeros(1, T, H, D, dtype=BF16, device="cuda")
+    ps = torch.zeros(T, 2, dtype=torch.int32, device="cuda")
+    xs[:, -5:], ps[-5:] = x.cuda(), pos.cuda()
+    y = tokens.rotary(xs, ps, (20, 12), base=100.0)
+    _hold(y[:, -5:], ref.rotary(x, pos, (20, 12), 100.0, False), "y")
+    assert not bool(y[:, :1000].any()) and not bool(y[:, T - 1000:T - 5].any())
+
+
+@pytest.mark.parametrize("Tq,Tk,D,how", [(300, 300, 128, "causal"), (300, 300, 64, "documents"), (1, 3000, 64, "few"), (70, 70, 12, "rows")])
+def test_captured_attention_variants(Tq, Tk, D, how):
+    """Each way through the kernels captured and replayed with new inputs, eager calls between."""
+    q, k, v, do, g = _attention_inputs(2, Tq, Tk, 4, 2, D, BF16, 5)
+    docs = _documents(g, 2, Tk, 3).cuda()
+    kw = {"causal": dict(causal=True, cap=3.0), "documents": dict(q_documents=docs, k_documents=docs), "rows": dict(causal=True),
+          "few": dict(k_lengths=torch.tensor([3000, 1234], dtype=torch.int32).cuda())}[how]
+    still = [t.cuda() for t in (q, k, v)]
+    do = do.cuda()
+
+    def step():
+        leaves = [t.detach().requires_grad_(how != "few") for t in still]
+        o = tokens.attention(*leaves, **kw)
+        return (o,) if how == "few" else (o.detach(), *torch.autograd.grad(o, leaves, do))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for n in range(4):
+        for t in still:
+            t.copy_(torch.randn(t.shape, generator=g).to(BF16))
+        want = [t.clone() for t in step()]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), n
+
+
+def test_calls_from_several_threads():
+    """Two threads, each on a stream of its own, training steps and refusals mixed: results and messages stay apart."""
+    import threading
+    q, k, v, do, _ = _attention_inputs(1, 200, 200, 2, 1, 64, BF16, 6)
+    leaves = [[t.cuda().requires_grad_() for t in (q, k, v)] for _ in range(2)]
+    do = do.cuda()
+    x = torch.randn(300, 700, device="cuda")
+    want = torch.autograd.grad(tokens.attention(*leaves[0], causal=True), leaves[0], do)
+    norm = tokens.layer_norm(x)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(n):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = torch.autograd.grad(tokens.attention(*leaves[n], causal=True), leaves[n], do)
+                y = tokens.layer_norm(x)
+                try:
+                    _lib.check_tokens(_lib.load().wst_layer_norm_workspace(None, None))
+                    wrong.append("no refusal")
+                except Exception as e:
+                    if "bytes is NULL" not in str(e):
+                        wrong.append(str(e))
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want)) or not torch.equal(y, norm):
+                    wrong.append(n)
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong[:3]
