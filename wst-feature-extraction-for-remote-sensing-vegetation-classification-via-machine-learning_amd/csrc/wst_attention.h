@@ -2024,15 +2024,35 @@ __global__ __launch_bounds__((dkv_threads<T, DP>()), sizeof(T) == 2 ? 2 : 1) voi
     }
 }
 
-// Adds the parts of a key's gradients, a wave a key.
+// dslopes[h] by one block: the partial sums of a head, added in a fixed order. s: a float a wave.
+__device__ __forceinline__ void add_slopes(const AttnArgs& a, int h, float* s) {
+    const int64_t count = a.d.batch * static_cast<int64_t>(a.slots);
+    const float* p = a.slope_part + h * count;
+    float v = 0.f;
+    for (int64_t i = threadIdx.x; i < count; i += blockDim.x) v += p[i];
+    v = wave_sum(v);
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (uint32_t k = 1; k < blockDim.x / 64; ++k) v += s[k];
+        a.g.dslopes[h] = v;
+    }
+}
+
+// Adds the parts of a key's gradients, a wave a key; blocks behind those of the keys, one a head that shares the key head,
+// add the slopes' partial sums, which saves a launch.
 template <typename T>
 __global__ __launch_bounds__(256) void k_attn_dkv_join(AttnArgs a) {
     __shared__ float scratch[4][2][kD];
     const wst_attention_desc& d = a.d;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int j = static_cast<int>(blockIdx.x) * 4 + w;
-    const int64_t b = blockIdx.z;
+    const int64_t b = blockIdx.z, behind = static_cast<int64_t>(blockIdx.x) - (d.k_len + 3) / 4;
     const int kvh = blockIdx.y;
+    if (behind >= 0) {
+        if (b == 0) add_slopes(a, kvh * (d.q_heads / d.k_heads) + static_cast<int>(behind), &scratch[0][0][0]);
+        return;
+    }
+    const int j = static_cast<int>(blockIdx.x) * 4 + w;
     if (j >= d.k_len) return;
     float v[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
     for (int p = 0; p < a.parts; ++p) {

@@ -7,19 +7,10 @@ namespace {
 
 using namespace wst_tok;
 
-// dslopes[h]: the partial sums of a head, added in a fixed order.
-__global__ __launch_bounds__(1024) void k_attn_slopes(const float* part, int64_t count, float* out) {
+// dslopes where no k_attn_dkv_join follows.
+__global__ __launch_bounds__(1024) void k_attn_slopes(AttnArgs a) {
     __shared__ float s[16];
-    const float* p = part + static_cast<int64_t>(blockIdx.x) * count;
-    float v = 0.f;
-    for (int64_t i = threadIdx.x; i < count; i += 1024) v += p[i];
-    v = wave_sum(v);
-    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int k = 1; k < 16; ++k) v += s[k];
-        out[blockIdx.x] = v;
-    }
+    add_slopes(a, blockIdx.x, s);
 }
 
 template <typename T>
@@ -56,7 +47,7 @@ int check(const wst_attention_desc* d) {
         return fail(WST_ERR_INVALID, "attention: 1 to %d axes", WST_MAX_DISTANCE_AXES);
     if (d->prefix && !d->causal) return fail(WST_ERR_INVALID, "attention: a prefix needs causal order");
     if (d->batch > 65535 || d->q_heads > 65535) return fail(WST_ERR_UNSUPPORTED, "attention: more than 65535 sequences or heads");
-    // blocks of every kernel are counted in 31 bits: a tile or row of each has at most eight splits or so in flight
+    // blocks of every kernel are counted in 31 bits; splits and parts are many only where rows are few
     if (static_cast<double>(d->batch) * d->q_heads * (static_cast<double>(d->q_len) / 4 + static_cast<double>(d->k_len) / 4 + 512) > 2147483647.0)
         return fail(WST_ERR_UNSUPPORTED, "attention: too many rows for one call");
     if (d->q_len > (1LL << 30) || d->k_len > (1LL << 30)) return fail(WST_ERR_UNSUPPORTED, "attention: more than 2^30 tokens");
@@ -191,7 +182,8 @@ int wst_attention_backward(const wst_attention_desc* d, const wst_attention_grad
         if (g->dk || g->dv)
             k_attn_dkv_rows<T><<<dim3(static_cast<unsigned>((d->k_len + 3) / 4), d->k_heads, static_cast<unsigned>(d->batch)), dim3(256), 0, st>>>(a);
     });
-    if (g->dslopes) k_attn_slopes<<<dim3(d->q_heads), dim3(1024), 0, st>>>(a.slope_part, d->batch * static_cast<int64_t>(a.slots), g->dslopes);
+    const bool joined = p.tiles && p.parts > 1 && (g->dk || g->dv);
+    if (g->dslopes && !joined) k_attn_slopes<<<dim3(d->q_heads), dim3(1024), 0, st>>>(a);
     return launched("attention backward");
 }
 

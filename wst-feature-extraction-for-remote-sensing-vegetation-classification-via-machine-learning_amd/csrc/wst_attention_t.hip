@@ -66,7 +66,8 @@ void attend_backward(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
         if (want_k) k_attn_dkv<T, DP, CAP, BIAS><<<dim3(static_cast<unsigned>(k_blocks * p.parts)), dim3(dkv_threads<T, DP>()), 0, st>>>(a);
     });
     if (p.parts > 1 && want_k) {
-        const dim3 keys(static_cast<unsigned>((d.k_len + 3) / 4), d.k_heads, static_cast<unsigned>(d.batch));
+        const int64_t behind = a.slope_part ? d.q_heads / d.k_heads : 0;
+        const dim3 keys(static_cast<unsigned>((d.k_len + 3) / 4 + behind), d.k_heads, static_cast<unsigned>(d.batch));
         k_attn_dkv_join<T><<<keys, dim3(256), 0, st>>>(a);
     }
 }
