@@ -610,25 +610,33 @@ struct Shape {
     float twice, turn;        // 2 |scale| log2 e / cap;  |scale| / cap
     bool cap;
     template <typename T>
-    static __device__ __forceinline__ Shape of(const wst_attention_desc& d, bool sign = false) {
+    static __device__ __forceinline__ Shape of(const wst_attention_desc& d, bool sign = false, bool fine = false) {
         Shape s;
         const float scale = sign ? d.scale : fabsf(d.scale);
         s.cap = d.cap > 0.f;
         s.twice = s.cap ? 2.f * scale * kLog2e / d.cap : 0.f;
         s.turn = s.cap ? scale / d.cap : 0.f;
-        s.raw = !s.cap ? scale : sizeof(T) == 4 ? d.cap : 2.f * d.cap;
+        s.raw = !s.cap ? scale : sizeof(T) == 4 || fine ? d.cap : 2.f * d.cap;
         s.mul = d.slopes ? kLog2e : s.raw * kLog2e;
-        s.add = s.cap && sizeof(T) != 4 ? d.cap * kLog2e : 0.f;
+        s.add = s.cap && sizeof(T) != 4 && !fine ? d.cap * kLog2e : 0.f;
         return s;
     }
     // dot products to x before the bias, and the cap's slope
-    template <typename T, bool GRAD>
+    // FINE: x is the tanh itself, for the slopes' gradient, a float32 sum that keeps what 16-bit weights do not. Its
+    // series to y^9 up to 1/4 (the next term is below 2^-26 of it there), beyond 1 - 2 / (e + 1).
+    template <typename T, bool GRAD, bool FINE = false>
     __device__ __forceinline__ void bend(f32x16& x, f32x16& grad) const {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             if constexpr (sizeof(T) == 4) {
                 x[r] = tanhf(x[r] * turn);
                 if constexpr (GRAD) grad[r] = 1.f - x[r] * x[r];
+            } else if constexpr (FINE) {
+                const float y = x[r] * turn, y2 = y * y;
+                const float series = fmaf(y * y2, fmaf(y2, fmaf(y2, fmaf(y2, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), y);
+                const float outer = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x[r] * twice)), 1.f);
+                x[r] = fabsf(y) < 0.25f ? series : outer;
+                if constexpr (GRAD) grad[r] = fmaf(-x[r], x[r], 1.f);
             } else {
                 x[r] = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(x[r] * twice));
                 if constexpr (GRAD) {
@@ -819,11 +827,11 @@ __device__ __forceinline__ Kind kind_of(const wst_attention_desc& d) {
 
 // Turns 32 x 32 dot products (rows: keys key0 + 32 sub .., column: the lane's query) into x of Shape, -inf where the
 // query does not see the key. GRAD: also the cap's slope and the distances.
-template <typename T, bool GRAD, int MASK>
+template <typename T, bool GRAD, int MASK, bool FINE = false>
 __device__ __forceinline__ void scores(f32x16& x, const Kind& kind, const Shape& sh, float slope, const Query& q, const Along& al,
                                        int key0, int sub, f32x16& grad, f32x16& far) {
     const int h = (threadIdx.x & 63) >> 5;
-    if (kind.cap) sh.bend<T, GRAD>(x, grad);
+    if (kind.cap) sh.bend<T, GRAD, FINE>(x, grad);
     if (kind.bias) {
         if (kind.coordinates) {
 #pragma unroll
@@ -1407,7 +1415,8 @@ __global__ __launch_bounds__(256 * TEAMS, sizeof(T) == 2 ? 2 : 1) void k_attn_dq
     const int64_t b = bh / d.q_heads;
     const int h = static_cast<int>(bh % d.q_heads), kvh = h / (d.q_heads / d.k_heads);
     const Scope sc(d, b);
-    const Shape sh = Shape::of<T>(d);
+    constexpr bool kFine = sizeof(T) == 2 && BIAS != 0;
+    const Shape sh = Shape::of<T>(d, false, kFine);
     const Kind kind = kind_of<CAP, BIAS>(d);
     const int i = i0 + w * 32 + (lane & 31);
     const int64_t row = (b * d.q_heads + h) * d.q_len + i;
@@ -1527,7 +1536,7 @@ __global__ __launch_bounds__(256 * TEAMS, sizeof(T) == 2 ? 2 : 1) void k_attn_dq
                 dp = Mma<T>::mul(L::row_frag(vc, 32 * n, c), df[c], dp);
             }
             if constexpr (sizeof(T) == 2) paced<DP / 8, 1, 4>();
-            scores<T, true, MASK>(x, kind, sh, slope, q, al[turn], key0, n, grad, far);
+            scores<T, true, MASK, kFine>(x, kind, sh, slope, q, al[turn], key0, n, grad, far);
             if constexpr (MASK != 0) {     // a weight of 0 may meet a value that is not finite
 #pragma unroll
                 for (int r = 0; r < 16; ++r) dp[r] = x[r] == -INFINITY ? 0.f : dp[r];
