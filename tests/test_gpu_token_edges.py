@@ -1,0 +1,52 @@
+"""GPU tests of the token operators at their edges, against the float64 restatement (oracle/token_ops.py)."""
+import pytest
+import torch
+
+import token_cases
+import wst_amd  # noqa: F401
+from oracle import token_ops as ref
+from test_gpu_tokens import BF16, F16, _attention_inputs, _hold
+from wst_amd import tokens
+
+pytestmark = pytest.mark.gpu
+
+
+def _out_of_the_caches():
+    """Writes more than the caches hold, so that what comes next is fetched from memory."""
+    torch.empty(1 << 29, dtype=torch.uint8, device="cuda").fill_(1)
+
+
+def _key_gradients(q, k, v, do, want, **kw):
+    """dk and dv alone, keys and values first read by the kernel that sums them, several times."""
+    leaves, dev = [t.cuda().requires_grad_() for t in (k, v)], {n: t.cuda() if torch.is_tensor(t) else t for n, t in kw.items()}
+    q, do, first = q.cuda(), do.cuda(), None
+    for _ in range(4):
+        o = tokens.attention(q, *leaves, **dev)
+        _out_of_the_caches()
+        got = torch.autograd.grad(o, leaves, do)
+        if first is None:
+            first = got
+            _hold(got[0], want["dk"], "dk")
+            _hold(got[1], want["dv"], "dv")
+        assert all(torch.equal(a, b) for a, b in zip(got, first))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("B,T,H,Hk,D", token_cases.PARTS_WITHOUT_TILES)
+def test_attention_parts_without_tiles(B, T, H, Hk, D, dtype):
+    """The last keys in order have fewer tiles of queries than there are parts: a part without one adds nothing."""
+    q, k, v, do, _ = _attention_inputs(B, T, T, H, Hk, D, dtype, T + D)
+    _key_gradients(q, k, v, do, ref.attention(q, k, v, do=do, causal=True), causal=True)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("D", [96, 128])
+def test_attention_documents_that_no_query_has(D, dtype):
+    q, k, v, do, _ = _attention_inputs(2, 300, 700, 4, 2, D, dtype, D)
+    docs = torch.zeros(2, 700, dtype=torch.int32)
+    docs[:, 128:384] = 5                                    # two blocks of keys whose document no query has
+    docs[1, 400:] = 9
+    kw = dict(q_documents=torch.zeros(2, 300, dtype=torch.int32), k_documents=docs)
+    want = ref.attention(q, k, v, do=do, **kw)
+    assert not bool(want["dv"][0][:, 128:384].any())
+    _key_gradients(q, k, v, do, want, **kw)

@@ -1801,7 +1801,9 @@ __global__ __launch_bounds__((dkv_threads<T, DP>()), sizeof(T) == 2 ? 2 : 1) voi
     __syncthreads();
     if (!cur.s.done(walk)) fetch(cur, 0, rows[0]);
     if constexpr (kWide) {
-        if (!half && tiles) {
+        // Only where a tile follows: its wait is the one for these loads too. A part without tiles (in order, the last
+        // keys; documents that no query has) reads no key, and the sums below lie where the keys would land.
+        if (!half && !cur.s.done(walk)) {
             Fetch<T, DP, kBQ> own;
             const bool whole = !marked && d.dim == DP && keys >= kBQ;
             own.init(d.k_strides[1], d.dim, t);
@@ -1962,6 +1964,7 @@ __global__ __launch_bounds__((dkv_threads<T, DP>()), sizeof(T) == 2 ? 2 : 1) voi
     if constexpr (kWide) {             // the second four waves hand their sums over, a lane its own registers
         float* sums = reinterpret_cast<float*>(pool) + w * (DP * 64) + lane;
         static_assert(sizeof(pool) >= 4 * DP * 64 * sizeof(float), "room for the sums");
+        arrived();                     // nothing may land in the pool any more
         __syncthreads();
         if (half) {
 #pragma unroll
