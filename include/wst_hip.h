@@ -342,7 +342,7 @@ int wst_rotary(const wst_rotary_desc* d, const void* q, void* q_out, const void*
  *   o_i = sum_j softmax(s_i)_j v_j over the keys seen; a query that sees none gets 0 (and lse = -inf, no gradient).
  * What is not seen has no influence, infinities and NaN included.  Scores, softmax and sums are float32; the weights
  * that multiply v, and the score gradients that multiply q and k, are rounded to the inputs' type.
- * Coordinates lie in [-2^29, 2^29).
+ * Coordinates lie in [-2^29, 2^29), cap is 0 or from 1e-30 to 1e30.
  */
 typedef struct wst_attention_desc {
     int64_t batch, q_len, k_len;

@@ -148,7 +148,11 @@ def attention(q, k, v, *, scale=None, cap=0.0, slopes=None, q_positions=None, k_
             if cap > 0:
                 t = torch.tanh(z / cap)
                 z = cap * t
-                e = e + 8 * U32 * cap              # tanh within a few ulp of one, times cap
+                # tanh within a few roundings of one, times cap; in float32, and for caps beyond 64, of itself: 24 where
+                # it is 1 - 2 / (e^2y + 1), so 8 of one from a third on and three times itself below, and fewer in its
+                # series (the argument's two, the polynomial's few)
+                near = u > 0 and cap <= 64
+                e = e + 8 * U32 * cap * (1.0 if near else torch.clamp(3 * t.abs(), max=1.0))
             if slopes is not None:
                 z = z - float(slopes[h]) * far
                 e = e + 4 * U32 * (float(slopes[h]) * far).abs()

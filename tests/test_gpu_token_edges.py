@@ -5,7 +5,7 @@ import torch
 import token_cases
 import wst_amd  # noqa: F401
 from oracle import token_ops as ref
-from test_gpu_tokens import BF16, F16, _attention_inputs, _hold
+from test_gpu_tokens import BF16, F16, F32, _attention_inputs, _check_attention, _documents, _hold
 from wst_amd import tokens
 
 pytestmark = pytest.mark.gpu
@@ -50,3 +50,32 @@ def test_attention_documents_that_no_query_has(D, dtype):
     want = ref.attention(q, k, v, do=do, **kw)
     assert not bool(want["dv"][0][:, 128:384].any())
     _key_gradients(q, k, v, do, want, **kw)
+
+
+CAPS = [1e-30, 1e-2, 50.0, 64.0, 65.0, 1e3, 1e6, 1e30]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("D", [64, 128, 12])
+@pytest.mark.parametrize("cap", CAPS)
+def test_attention_caps_of_any_size(cap, D, dtype):
+    """The cap's error is one of the score, not of the cap: a large cap is no cap, a small one takes the scores away."""
+    q, k, v, do, g = _attention_inputs(1, 200, 200, 4, 2, D, dtype, 41, gain=4.0)
+    slopes = torch.rand(4, generator=g) * 0.1
+    pos = torch.randint(-20, 20, (1, 200, 2), generator=g, dtype=torch.int32)
+    docs = _documents(g, 1, 200, 3)
+    for kw in (dict(), dict(slopes=slopes, causal=True), dict(scale=-0.2, slopes=slopes, q_positions=pos, k_positions=pos),
+               dict(q_documents=docs, k_documents=docs)):
+        o, _ = _check_attention(q, k, v, do, cap=cap, **kw)
+    if cap == 1e30:
+        want = ref.attention(q, k, v, **kw)
+        _hold(o, want["o"], "no cap")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("cap", CAPS)
+def test_attention_caps_of_any_size_few_queries(cap, dtype):
+    q, k, v, do, g = _attention_inputs(2, 2, 1500, 4, 2, 64, dtype, 42, gain=4.0)
+    lengths = torch.tensor([1500, 700], dtype=torch.int32)
+    for kw in (dict(), dict(k_lengths=lengths, slopes=torch.rand(4, generator=g) * 0.01)):
+        _check_attention(q, k, v, do, train=False, cap=cap, **kw)

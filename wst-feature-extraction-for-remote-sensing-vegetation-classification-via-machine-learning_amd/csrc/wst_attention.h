@@ -10,6 +10,7 @@
 #ifndef WST_ATTENTION_H
 #define WST_ATTENTION_H
 
+#include <cfloat>
 #include <type_traits>
 
 #include "wst_tokens.h"
@@ -598,10 +599,17 @@ __device__ __forceinline__ void to_frags(const f32x16& s, Frag<T> (&f)[2]) {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
+// Caps up to here, in 16-bit types, are taken as -1 / (e + 1) (Shape), which is off by about 2^-23 of the cap whatever the
+// score: a weight is off by 2^-17 of itself at most, a thirty-second of a rounding to float16 and less of one to bfloat16.
+// The error grows with the cap (at 1e6 a weight would be off by a tenth, from 1e8 on all scores be equal), so beyond the
+// tanh is taken to a relative error (bend, FINE), in a kernel for all kinds of biases. 8192 x 8 heads x 128 in order,
+// bfloat16, cap 64 and 65: forward 212 and 259 us, with its backward pass 811 and 1170; 64 wide 160 and 216, 599 and 829.
+constexpr float kNearCap = 64.f;
+
 // Scores in powers of two, as an affine function of what the tiles hold: score = mul * x + add. Plainly x is the dot
 // product and mul = scale log2 e, so that scaling costs nothing beyond the subtraction of the maximum. Capped, with
-// e = exp(2 z / cap), tanh = 1 - 2 / (e + 1), x is -1 / (e + 1): the cap's slope is 1 - tanh^2 = -4 x (1 + x). Its error
-// of 2^-24 or two of the cap is below what 16-bit weights keep; float32 takes the library's tanh, good to an ulp. With a
+// e = exp(2 z / cap), tanh = 1 - 2 / (e + 1), x is -1 / (e + 1): the cap's slope is 1 - tanh^2 = -4 x (1 + x); for caps
+// beyond kNearCap x is the tanh itself; float32 takes the library's tanh, good to an ulp. With a
 // bias x is the score itself, mul = log2 e: slopes times log2 e, rounded, would be the slopes of a network a little way
 // off. For a maximum over x mul must not be negative: there a negative
 // scale turns q over instead (sign = false).
@@ -614,16 +622,18 @@ struct Shape {
         Shape s;
         const float scale = sign ? d.scale : fabsf(d.scale);
         s.cap = d.cap > 0.f;
-        s.twice = s.cap ? 2.f * scale * kLog2e / d.cap : 0.f;
-        s.turn = s.cap ? scale / d.cap : 0.f;
+        // held to finite numbers: a dot product of 0 stays 0 under the smallest caps
+        s.twice = s.cap ? fminf(fmaxf(2.f * scale * kLog2e / d.cap, -FLT_MAX), FLT_MAX) : 0.f;
+        s.turn = s.cap ? fminf(fmaxf(scale / d.cap, -FLT_MAX), FLT_MAX) : 0.f;
         s.raw = !s.cap ? scale : sizeof(T) == 4 || fine ? d.cap : 2.f * d.cap;
         s.mul = d.slopes ? kLog2e : s.raw * kLog2e;
         s.add = s.cap && sizeof(T) != 4 && !fine ? d.cap * kLog2e : 0.f;
         return s;
     }
     // dot products to x before the bias, and the cap's slope
-    // FINE: x is the tanh itself, for the slopes' gradient, a float32 sum that keeps what 16-bit weights do not. Its
-    // series to y^9 up to 1/4 (the next term is below 2^-26 of it there), beyond 1 - 2 / (e + 1).
+    // FINE: x is the tanh itself, for caps beyond kNearCap and for the slopes' gradient, a float32 sum that keeps what
+    // 16-bit weights do not. Its series to y^9 up to 1/4 (the next term is below 2^-26 of it there), beyond
+    // 1 - 2 / (e + 1), off by 6 roundings of 1 and so by 24 of itself or fewer.
     template <typename T, bool GRAD, bool FINE = false>
     __device__ __forceinline__ void bend(f32x16& x, f32x16& grad) const {
 #pragma unroll
@@ -812,7 +822,8 @@ struct AlongStage {
 // "as the call says". Branches on these inside the loop over tiles cost more than the branch: the compiler moves whole
 // tiles of registers where the ways meet (forward, 8192 x 8 heads x 128, no cap, no bias: 318 us with such branches, 300
 // without, in one process).
-// float32, whose products take sixteen times as long, has the one general kernel.
+// float32, whose products take sixteen times as long, has the one general kernel, and 16-bit types one for caps beyond
+// kNearCap.
 struct Kind {
     bool cap, bias, coordinates;
 };
@@ -824,6 +835,10 @@ __device__ __forceinline__ Kind kind_of(const wst_attention_desc& d) {
     k.coordinates = BIAS == 3 ? d.q_pos != nullptr : BIAS == 2;
     return k;
 }
+
+// Whether scores are capped by the tanh itself (Shape::bend) in 16-bit types.
+template <typename T, int CAP>
+constexpr bool kFar = sizeof(T) == 2 && CAP == 2;
 
 // Turns 32 x 32 dot products (rows: keys key0 + 32 sub .., column: the lane's query) into x of Shape, -inf where the
 // query does not see the key. GRAD: also the cap's slope and the distances.
@@ -940,7 +955,7 @@ __global__ __launch_bounds__(256 * TEAMS, sizeof(T) == 2 ? 2 : 1) void k_attn_fw
     const int64_t b = bh / d.q_heads;
     const int h = static_cast<int>(bh % d.q_heads), kvh = h / (d.q_heads / d.k_heads);
     const Scope sc(d, b);
-    const Shape sh = Shape::of<T>(d);
+    const Shape sh = Shape::of<T>(d, false, kFar<T, CAP>);
     const Kind kind = kind_of<CAP, BIAS>(d);
     const int i = i0 + w * 32 + (lane & 31);
     const bool ok = i < d.q_len;
@@ -1043,7 +1058,7 @@ __global__ __launch_bounds__(256 * TEAMS, sizeof(T) == 2 ? 2 : 1) void k_attn_fw
         float top = -INFINITY;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            scores<T, false, decltype(mask)::value>(x[n], kind, sh, slope, q, al[turn], cur.tile * kBK, n, unused, unused);
+            scores<T, false, decltype(mask)::value, kFar<T, CAP>>(x[n], kind, sh, slope, q, al[turn], cur.tile * kBK, n, unused, unused);
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = fmaxf(top, x[n][r]);
         }
@@ -1181,7 +1196,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_split(Attn
     const int i = static_cast<int>(ok ? r % d.q_len : 0);
     const int h = kvh * group + static_cast<int>(ok ? r / d.q_len : 0);
     const Scope sc(d, b);
-    const Shape sh = Shape::of<T>(d);
+    const Shape sh = Shape::of<T>(d, false, kFar<T, CAP>);
     const Kind kind = kind_of<CAP, BIAS>(d);
     const Query q = query_of(sc, i, ok);
     const float slope = d.slopes ? d.slopes[h] : 0.f;
@@ -1251,8 +1266,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void k_attn_split(Attn
         f32x16 s = zero16(), unused;
 #pragma unroll
         for (int c = 0; c < DP / 16; ++c) s = Mma<T>::mul(L::row_frag(kc, 0, c), qf[c], s);
-        if (marked) scores<T, false, 2>(s, kind, sh, slope, q, mine, key0 - 32 * sub, sub, unused, unused);
-        else scores<T, false, 1>(s, kind, sh, slope, q, mine, key0 - 32 * sub, sub, unused, unused);
+        if (marked) scores<T, false, 2, kFar<T, CAP>>(s, kind, sh, slope, q, mine, key0 - 32 * sub, sub, unused, unused);
+        else scores<T, false, 1, kFar<T, CAP>>(s, kind, sh, slope, q, mine, key0 - 32 * sub, sub, unused, unused);
         float top = -INFINITY;
 #pragma unroll
         for (int x = 0; x < 16; ++x) top = fmaxf(top, s[x]);
@@ -1415,7 +1430,7 @@ __global__ __launch_bounds__(256 * TEAMS, sizeof(T) == 2 ? 2 : 1) void k_attn_dq
     const int64_t b = bh / d.q_heads;
     const int h = static_cast<int>(bh % d.q_heads), kvh = h / (d.q_heads / d.k_heads);
     const Scope sc(d, b);
-    constexpr bool kFine = sizeof(T) == 2 && BIAS != 0;
+    constexpr bool kFine = kFar<T, CAP> || (sizeof(T) == 2 && BIAS != 0);
     const Shape sh = Shape::of<T>(d, false, kFine);
     const Kind kind = kind_of<CAP, BIAS>(d);
     const int i = i0 + w * 32 + (lane & 31);
@@ -1674,7 +1689,7 @@ __global__ __launch_bounds__((dkv_threads<T, DP>()), sizeof(T) == 2 ? 2 : 1) voi
     const int64_t b = bh / d.k_heads;
     const int kvh = static_cast<int>(bh % d.k_heads);
     const Scope sc(d, b);
-    const Shape sh = Shape::of<T>(d, true);
+    const Shape sh = Shape::of<T>(d, true, kFar<T, CAP>);
     const Kind kind = kind_of<CAP, BIAS>(d);
     const int j = j0 + w * 32 + (lane & 31), q_len = static_cast<int>(d.q_len);
     const bool exists = j < d.k_len, ok = j < sc.length && (!sc.k_doc || sc.k_doc[j] >= 0);
@@ -1865,7 +1880,7 @@ __global__ __launch_bounds__((dkv_threads<T, DP>()), sizeof(T) == 2 ? 2 : 1) voi
                 }
                 if constexpr (sizeof(T) == 2) paced<DP / 8, 1, 6>();
             }
-            if (kind.cap) sh.bend<T, true>(x, grad);
+            if (kind.cap) sh.bend<T, true, kFar<T, CAP>>(x, grad);
             if (kind.bias) {
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {

@@ -40,7 +40,8 @@ int check(const wst_attention_desc* d) {
     if (d->dim > WST_MAX_HEAD_DIM) return fail(WST_ERR_UNSUPPORTED, "attention: heads wider than %d", WST_MAX_HEAD_DIM);
     if (d->dtype != WST_F32 && d->dtype != WST_BF16 && d->dtype != WST_F16) return fail(WST_ERR_INVALID, "attention: unknown type");
     if (!std::isfinite(d->scale)) return fail(WST_ERR_INVALID, "attention: scale must be finite");
-    if (!(d->cap >= 0.f) || !std::isfinite(d->cap)) return fail(WST_ERR_INVALID, "attention: cap must be finite and not negative");
+    if (d->cap != 0.f && !(d->cap >= 1e-30f && d->cap <= 1e30f))
+        return fail(WST_ERR_INVALID, "attention: cap must be 0 (none) or from 1e-30 to 1e30");
     if (!d->q_pos != !d->k_pos || !d->q_doc != !d->k_doc)
         return fail(WST_ERR_INVALID, "attention: positions and documents are given for queries and keys alike");
     if (d->q_pos && (d->axes < 1 || d->axes > WST_MAX_DISTANCE_AXES))

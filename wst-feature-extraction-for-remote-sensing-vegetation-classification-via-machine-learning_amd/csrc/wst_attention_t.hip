@@ -15,7 +15,8 @@ void with_kind(const wst_attention_desc& d, F f) {
             else if (!d.q_pos) f(cap, std::integral_constant<int, 1>{});
             else f(cap, std::integral_constant<int, 2>{});
         };
-        if (d.cap > 0.f) bias(std::integral_constant<int, 1>{});
+        if (d.cap > kNearCap) f(std::integral_constant<int, 2>{}, std::integral_constant<int, 3>{});
+        else if (d.cap > 0.f) bias(std::integral_constant<int, 1>{});
         else bias(std::integral_constant<int, 0>{});
     }
 }

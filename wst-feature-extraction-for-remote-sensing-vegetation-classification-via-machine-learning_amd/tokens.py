@@ -395,7 +395,7 @@ def attention(q, k, v, *, scale=None, cap=0.0, slopes=None, q_positions=None, k_
     """Softmax attention of q (B, Tq, H, D) over k, v (B, Tk, Hk, D); H a multiple of Hk, D <= 256.
 
     With ``L = k_lengths[b]`` (default Tk) and ``place(i) = i + L - Tq``, query i scores key j as
-    ``z = scale * q_i.k_j`` (scale defaults to ``D ** -0.5``), ``z = cap * tanh(z / cap)`` where ``cap > 0``, and
+    ``z = scale * q_i.k_j`` (scale defaults to ``D ** -0.5``), ``z = cap * tanh(z / cap)`` where ``cap > 0`` (1e-30 to 1e30), and
     ``z - slopes[h] * distance``: slopes float32 (H,); the distance is the sum over axes of
     ``|q_positions[i] - k_positions[j]|`` (int32 (T, A) or (B, T, A), A <= 3, within +-2**29), or ``|place(i) - j|``
     without positions.  Key j is seen iff
@@ -448,8 +448,8 @@ def attention(q, k, v, *, scale=None, cap=0.0, slopes=None, q_positions=None, k_
     s.causal = bool(causal) or prefix is not None
     s.scale = D ** -0.5 if scale is None else float(scale)
     s.cap = float(cap)
-    if not 0.0 <= s.cap < float("inf"):
-        raise RuntimeError("cap must be finite and not negative")
+    if s.cap != 0.0 and not 1e-30 <= s.cap <= 1e30:
+        raise RuntimeError("cap must be 0 (none) or from 1e-30 to 1e30")
     if not abs(s.scale) < float("inf"):
         raise RuntimeError("scale must be finite")
     s.settle()
