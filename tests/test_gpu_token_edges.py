@@ -1,6 +1,7 @@
 """GPU tests of the token operators at their edges, against the float64 restatement (oracle/token_ops.py)."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import token_cases
 import wst_amd  # noqa: F401
@@ -79,3 +80,34 @@ def test_attention_caps_of_any_size_few_queries(cap, dtype):
     lengths = torch.tensor([1500, 700], dtype=torch.int32)
     for kw in (dict(), dict(k_lengths=lengths, slopes=torch.rand(4, generator=g) * 0.01)):
         _check_attention(q, k, v, do, train=False, cap=cap, **kw)
+
+
+def _calls():
+    """Each operator on its differentiable arguments: (call, arguments)."""
+    x, w = torch.randn(2, 5, 2, 8, device="cuda"), torch.ones(8, device="cuda")
+    pos, slopes = torch.arange(5, dtype=torch.int32, device="cuda")[:, None], torch.ones(2, device="cuda")
+    return [(lambda x, w, b: tokens.layer_norm(x, w, b), (x, w, w.clone())),
+            (lambda q, k: torch.cat(tokens.rotary(q, pos, (4,), k=k)), (x, x.clone())),
+            (lambda q, k, v, s: tokens.attention(q, k, v, slopes=s), (x, x.clone(), x.clone(), slopes))]
+
+
+def test_forward_mode_is_refused():
+    """A tangent on any argument: without gradients too, and in either spelling."""
+    for call, args in _calls():
+        for n, t in enumerate(args):
+            for leaf in (t, t.clone().requires_grad_()):
+                with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+                    call(*args[:n], forward_ad.make_dual(leaf, torch.ones_like(t)), *args[n + 1:])
+            with pytest.raises(RuntimeError):
+                torch.func.jvp(lambda u: call(*args[:n], u, *args[n + 1:]), (t,), (torch.ones_like(t),))
+        with forward_ad.dual_level():
+            assert torch.equal(call(*args), call(*args))        # a level without tangents takes nothing away
+
+
+def test_tracing_is_refused():
+    for call, args in _calls():
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(call, args)
+        for transform in (torch.func.vmap(call, (0,) + (None,) * (len(args) - 1)), torch.func.grad(lambda *a: call(*a).sum())):
+            with pytest.raises(RuntimeError):
+                transform(*args)

@@ -10,14 +10,16 @@ learned counterpart, for training and inference:
 
 All run in the HIP library on the tensors' device and current stream, have gradients (torch autograd, first order), and
 can be captured into a graph (a backward pass: while no eager autograd graph of the same leaves is alive, since torch's
-engine would wait for that graph's stream inside the capture).  float32, bfloat16 and float16; sums and statistics are
-held in float32.  There is no CPU execution: tensors must live on a ROCm GPU.
+engine would wait for that graph's stream inside the capture).  Forward-mode derivatives and tracing
+(``torch.jit.trace``) are refused.  float32, bfloat16 and float16; sums and statistics are held in float32.  There is
+no CPU execution: tensors must live on a ROCm GPU.
 """
 from __future__ import annotations
 
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .frontend import require_gpu
@@ -68,6 +70,12 @@ def _first_order():
 
 
 def _wants_grad(*tensors):
+    # The library reads memory that neither of these follows: a tangent would be dropped, a trace would hold the result's
+    # allocation without the call.
+    if torch._C._is_tracing():
+        raise RuntimeError("the token operators cannot be traced")
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("the token operators have no forward-mode derivatives")
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
