@@ -111,3 +111,19 @@ def test_tracing_is_refused():
         for transform in (torch.func.vmap(call, (0,) + (None,) * (len(args) - 1)), torch.func.grad(lambda *a: call(*a).sum())):
             with pytest.raises(RuntimeError):
                 transform(*args)
+
+
+@pytest.mark.parametrize("B,Tq,Tk", [(2, 3, 0), (2, 70, 0), (2, 0, 5), (2, 0, 0), (0, 3, 5), (0, 3, 0)])
+@pytest.mark.parametrize("D", [8, 5])
+def test_attention_of_no_tokens_with_documents_and_positions(B, Tq, Tk, D):
+    """An empty store of keys, or an empty batch, takes the arguments that a full one takes."""
+    ints = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")   # noqa: E731
+    leaves = [torch.randn(B, t, h, D, device="cuda", requires_grad=True) for t, h in ((Tq, 2), (Tk, 1), (Tk, 1))]
+    slopes = torch.ones(2, device="cuda", requires_grad=True)
+    for batched in (True, False):
+        side = {f"{n}_{what}": ints(*((B, t) if batched or n == "q" else (t,)), *a)
+                for n, t in (("q", Tq), ("k", Tk)) for what, a in (("documents", ()), ("positions", (2,)))}
+        o, lse = tokens.attention(*leaves, slopes=slopes, k_lengths=ints(B), return_lse=True, causal=True, **side)
+        assert o.shape == (B, Tq, 2, D) and not bool(o.any()) and bool((lse == -torch.inf).all())
+        for t in torch.autograd.grad(o, [*leaves, slopes], torch.ones_like(o)):
+            assert not bool(t.any())

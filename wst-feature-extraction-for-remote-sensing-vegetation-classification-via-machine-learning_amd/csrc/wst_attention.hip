@@ -42,7 +42,8 @@ int check(const wst_attention_desc* d) {
     if (!std::isfinite(d->scale)) return fail(WST_ERR_INVALID, "attention: scale must be finite");
     if (d->cap != 0.f && !(d->cap >= 1e-30f && d->cap <= 1e30f))
         return fail(WST_ERR_INVALID, "attention: cap must be 0 (none) or from 1e-30 to 1e30");
-    if (!d->q_pos != !d->k_pos || !d->q_doc != !d->k_doc)
+    // (what has no elements may have no address)
+    if (d->batch && d->q_len && d->k_len && (!d->q_pos != !d->k_pos || !d->q_doc != !d->k_doc))
         return fail(WST_ERR_INVALID, "attention: positions and documents are given for queries and keys alike");
     if (d->q_pos && (d->axes < 1 || d->axes > WST_MAX_DISTANCE_AXES))
         return fail(WST_ERR_INVALID, "attention: 1 to %d axes", WST_MAX_DISTANCE_AXES);
