@@ -6,7 +6,7 @@ from torch.autograd import forward_ad
 import token_cases
 import wst_amd  # noqa: F401
 from oracle import token_ops as ref
-from test_gpu_tokens import BF16, F16, F32, _attention_inputs, _check_attention, _documents, _hold
+from test_gpu_tokens import BF16, F16, F32, _attention_inputs, _check_attention, _documents, _hold, _norm_inputs
 from wst_amd import tokens
 
 pytestmark = pytest.mark.gpu
@@ -127,3 +127,35 @@ def test_attention_of_no_tokens_with_documents_and_positions(B, Tq, Tk, D):
         assert o.shape == (B, Tq, 2, D) and not bool(o.any()) and bool((lse == -torch.inf).all())
         for t in torch.autograd.grad(o, [*leaves, slopes], torch.ones_like(o)):
             assert not bool(t.any())
+
+
+@pytest.mark.parametrize("rows,n,layout", [((1 << 26) + 7, 2, "rows"), ((1 << 23) + 5, 3, "maps"), ((1 << 22) + 3, 650, "maps")])
+def test_layer_norm_of_more_rows_than_a_launch_holds(rows, n, layout):
+    """A launch has fewer than 2^32 threads; these calls need more. Rows of the first and the last launch are checked, and
+    between them rows of zeros, whose result is the bias; the weight's gradient comes from the checked rows alone."""
+    points = 1 if layout == "rows" else 2                       # maps of two points
+    ends = 4 // points
+    x, w, b, dy = _norm_inputs(2 * ends * points, n, BF16, F32, n)
+    dy = dy.to(BF16)
+    want = ref.layer_norm(x, w, b, 1e-5, BF16, dy)
+    at = lambda t: torch.cat((t[:ends], t[-ends:])).reshape(-1, n)   # noqa: E731
+    if layout == "rows":
+        xs = torch.zeros(rows, n, dtype=BF16, device="cuda")
+    else:
+        xs = torch.zeros(rows, n, points, dtype=BF16, device="cuda").transpose(1, 2)
+    xs[:ends], xs[-ends:] = x.cuda().reshape(2 * ends, *xs.shape[1:]).split(ends)
+    xs.requires_grad_()
+    ws, bs = w.cuda().requires_grad_(), b.cuda().requires_grad_()
+    y = tokens.layer_norm(xs, ws, bs)
+    _hold(at(y), want["y"], "y")
+    plain = b.cuda().to(BF16)
+    for part in y.detach()[ends:-ends].split(1 << 20):
+        assert bool((part == plain).all())
+    dys = torch.zeros(y.shape, dtype=BF16, device="cuda")
+    dys[:ends], dys[-ends:] = dy.cuda().reshape(2 * ends, *xs.shape[1:]).split(ends)
+    dx, dw, db = torch.autograd.grad(y, (xs, ws, bs), dys)
+    _hold(at(dx), want["dx"], "dx")
+    _hold(dw, want["dw"], "dw")
+    _hold(db, want["db"], "db")
+    for part in dx[ends:-ends].split(1 << 20):
+        assert not bool(part.any())

@@ -29,3 +29,33 @@ def test_side_arguments_of_no_tokens_may_be_null(sizes):
     for side in (dict(q_doc=256), dict(k_doc=256), dict(q_pos=256), dict(k_pos=256)):
         assert lib.wst_attention_workspace(_lib.AttentionDesc(**{**d, **sizes, **side}), 0, ctypes.byref(need)) == 0
         assert lib.wst_attention_workspace(_lib.AttentionDesc(**{**d, **side}), 0, ctypes.byref(need)) == 1
+
+
+@pytest.mark.parametrize("kw", [dict(q_len=1 << 28, q_heads=8, k_heads=8), dict(q_len=1 << 27, dim=5), dict(q_len=1 << 27, dtype=1, causal=1)])
+def test_more_threads_than_a_launch_holds_are_refused(kw):
+    lib = _lib.load()
+    d = dict(batch=1, q_len=2, k_len=300, q=256, k=256, v=256, scale=1.0, q_heads=8, k_heads=8, dim=8)
+    d = _lib.AttentionDesc(**{**d, **kw})
+    need = ctypes.c_size_t()
+    assert lib.wst_attention_forward(d, 256, None, 256, 1 << 62, None) == 2
+    assert b"too many rows" in lib.wst_tokens_last_error()
+    assert lib.wst_attention_workspace(d, 1, ctypes.byref(need)) == 0
+    g = _lib.AttentionGrads(o=256, d_o=256, lse=256, dq=256)
+    assert lib.wst_attention_backward(d, g, 256, need.value, None) == 2
+    assert b"too many rows" in lib.wst_tokens_last_error()
+
+
+def test_backward_of_more_keys_than_a_launch_holds_is_refused():
+    lib, need = _lib.load(), ctypes.c_size_t()
+    d = _lib.AttentionDesc(batch=1, q_len=2, k_len=1 << 27, q=256, k=256, v=256, scale=1.0, q_heads=1, k_heads=1, dim=5)
+    assert lib.wst_attention_workspace(d, 1, ctypes.byref(need)) == 0
+    g = _lib.AttentionGrads(o=256, d_o=256, lse=256, dk=256)
+    assert lib.wst_attention_backward(d, g, 256, need.value, None) == 2
+    assert b"too many rows" in lib.wst_tokens_last_error()
+
+
+def test_rotary_of_more_tokens_than_a_launch_holds_is_refused():
+    lib = _lib.load()
+    d = _lib.RotaryDesc(batch=1, tokens=1 << 30, base=1e4, q_heads=1, dim=64, axes=1, sections=(ctypes.c_int32 * 4)(32, 0, 0, 0))
+    assert lib.wst_rotary(d, 256, 256, None, None, 256, None) == 2
+    assert b"too many tokens" in lib.wst_tokens_last_error()

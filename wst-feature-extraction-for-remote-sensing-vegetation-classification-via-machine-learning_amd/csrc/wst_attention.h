@@ -923,6 +923,9 @@ __device__ __forceinline__ void paced() {
 
 constexpr int kBQ = 128, kBK = 64;
 
+// Two teams a block (k_attn_fwd, k_attn_dq) where the rows are of many lengths; float32 has no room in LDS for two.
+inline bool two_teams(const wst_attention_desc& d) { return d.dtype != WST_F32 && d.causal && d.k_len > 2 * kBK; }
+
 // Forward pass: a block takes 128 queries of a head, 32 a wave, and walks the key tiles that any of them may see, keeping
 // the running maximum, sum and output of the softmax in registers; keys and values of a tile are shared through LDS.
 // The maximum is that of the first tile that shows the query anything, and stays as long as no score exceeds it by
@@ -1654,9 +1657,8 @@ struct Rows {
     uint32_t pos[kAxes][64];
 };
 
-// Threads of k_attn_dkv.
-template <typename T, int DP>
-constexpr int dkv_threads() { return sizeof(T) == 2 && DP > 64 ? 512 : 256; }
+// Threads of k_attn_dkv, by the width of a value and of a head.
+constexpr int dkv_threads(int size, int dim) { return size == 2 && dim > 64 ? 512 : 256; }
 
 // dk and dv: a block takes 128 keys of a key head, 32 a wave, and walks tiles of 64 queries of the heads that share it.
 // Scores come as (queries x keys), one key a lane, so weights and score gradients are the operands of dv^T = do^T p and
@@ -1670,9 +1672,9 @@ constexpr int dkv_threads() { return sizeof(T) == 2 && DP > 64 ? 512 : 256; }
 // Bound by the matrix units and, with a cap or a bias, as much by what a score takes besides. 8192 x 8 heads of 128:
 // 670 us, 820 TFLOP/s, of 1137 that a library product of 8192^3 reaches here.
 template <typename T, int DP, int CAP, int BIAS>
-__global__ __launch_bounds__((dkv_threads<T, DP>()), sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnArgs a) {
+__global__ __launch_bounds__(dkv_threads(sizeof(T), DP), sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnArgs a) {
     using L = Tile<T, DP>;
-    constexpr int kRows = 64, TH = dkv_threads<T, DP>(), kTile = kRows * L::kRowBytes;
+    constexpr int kRows = 64, TH = dkv_threads(sizeof(T), DP), kTile = kRows * L::kRowBytes;
     constexpr bool kWide = TH == 512;
     constexpr int kOwn = kBQ * L::kRowBytes;                          // the block's keys (or values)
     __shared__ __attribute__((aligned(256))) char pool[4 * kTile + (kWide ? 2 * kOwn : 0)];

@@ -105,6 +105,21 @@ AttnPlan plan_of(const wst_attention_desc& d, bool tiles) {
     return p;
 }
 
+// Whether every launch of a call has fewer than 2^32 threads along each axis: one that asks for more is cut to what is left
+// of them, without an error.
+bool launchable(const wst_attention_desc& d, const AttnPlan& p, bool backward) {
+    auto fits = [](double blocks, int threads) { return blocks * threads < 4294967296.0; };
+    const double q4 = std::ceil(d.q_len / 4.0), k4 = std::ceil(d.k_len / 4.0), seqs = d.batch;
+    if (!p.tiles) return fits(q4, 256) && (!backward || fits(k4, 256));
+    const double q_blocks = seqs * d.q_heads * std::ceil(d.q_len / static_cast<double>(kBQ));
+    if (!backward && p.splits)
+        return fits(p.splits * seqs * d.k_heads * std::ceil(static_cast<double>(d.q_heads / d.k_heads) * d.q_len / 32.0), 256);
+    if (!fits(q_blocks, two_teams(d) ? 512 : 256)) return false;
+    const double k_blocks = seqs * d.k_heads * std::ceil(d.k_len / static_cast<double>(kBQ));
+    return !backward || (fits(q4, 256) && fits(k_blocks * p.parts, dkv_threads(d.dtype == WST_F32 ? 4 : 2, d.dim)) &&
+                         (p.parts == 1 || fits(k4 + d.q_heads, 256)));
+}
+
 size_t bytes_of(const wst_attention_desc& d, int backward) {
     // either way of running: the gradient of the output, which decides with the rest, is not known here
     const AttnPlan p = plan_of(d, true), q = plan_of(d, false);
@@ -132,6 +147,7 @@ int wst_attention_forward(const wst_attention_desc* d, void* o, float* lse, void
     if (need && (!workspace || workspace_bytes < need)) return fail(WST_ERR_INVALID, "attention: workspace too small");
     AttnArgs a{};
     const AttnPlan p = plan_of(*d, can_tile(*d));
+    if (!launchable(*d, p, false)) return fail(WST_ERR_UNSUPPORTED, "attention: too many rows for one launch");
     a.d = *d;
     a.o = o;
     a.lse = lse;
@@ -162,6 +178,7 @@ int wst_attention_backward(const wst_attention_desc* d, const wst_attention_grad
     a.d = *d;
     a.g = *g;
     const AttnPlan p = plan_of(*d, can_tile(*d) && lined_up(*d, g->d_o, g->do_strides));
+    if (!launchable(*d, p, true)) return fail(WST_ERR_UNSUPPORTED, "attention: too many rows for one launch");
     a.delta = static_cast<float*>(workspace);
     a.slots = p.slots;
     a.parts = p.parts;

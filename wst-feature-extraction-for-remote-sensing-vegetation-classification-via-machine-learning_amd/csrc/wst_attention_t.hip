@@ -21,11 +21,10 @@ void with_kind(const wst_attention_desc& d, F f) {
     }
 }
 
-// Two teams a block where the rows are of many lengths; float32 has no room in LDS for two.
 template <typename T, typename F>
 void with_teams(const wst_attention_desc& d, F f) {
     if constexpr (sizeof(T) == 2) {
-        if (d.causal && d.k_len > 2 * kBK) return f(std::integral_constant<int, 2>{});
+        if (two_teams(d)) return f(std::integral_constant<int, 2>{});
     }
     f(std::integral_constant<int, 1>{});
 }
@@ -64,7 +63,7 @@ void attend_backward(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
                 constexpr int TEAMS = decltype(teams)::value;
                 k_attn_dq<T, DP, CAP, BIAS, TEAMS><<<dim3(static_cast<unsigned>(q_blocks)), dim3(256 * TEAMS), 0, st>>>(a);   // and delta
             });
-        if (want_k) k_attn_dkv<T, DP, CAP, BIAS><<<dim3(static_cast<unsigned>(k_blocks * p.parts)), dim3(dkv_threads<T, DP>()), 0, st>>>(a);
+        if (want_k) k_attn_dkv<T, DP, CAP, BIAS><<<dim3(static_cast<unsigned>(k_blocks * p.parts)), dim3(dkv_threads(sizeof(T), DP)), 0, st>>>(a);
     });
     if (p.parts > 1 && want_k) {
         const int64_t behind = a.slope_part ? d.q_heads / d.k_heads : 0;

@@ -75,6 +75,7 @@ struct NormArgs {
     float *part;                 // (groups, 2, n) partial dw, db
     float *c;                    // (rows, 2): mean(g), mean(g h)
     int groups;
+    int64_t first;               // this launch's first block (in_launches)
 };
 
 __device__ __forceinline__ int64_t row_at(const NormArgs& a, int64_t row, int64_t sb, int64_t sp) {
@@ -135,7 +136,7 @@ template <typename Tx, typename Ty, int VEC, int CH, int TPR>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_rows(NormArgs a) {
     __shared__ float slot[(TPR > 256 ? TPR : 256) / 64];
     const int t = threadIdx.x % TPR, n = static_cast<int>(a.n);
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x / TPR) + threadIdx.x / TPR;
+    const int64_t row = (a.first + blockIdx.x) * (blockDim.x / TPR) + threadIdx.x / TPR;
     if (row >= a.rows) return;   // whole waves; with TPR > 64 the block is one row
     const Tx* x = static_cast<const Tx*>(a.x) + row_at(a, row, a.sb, a.sp);
     float v[CH][VEC];
@@ -182,7 +183,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_rows(NormArgs a)
 template <typename Tx, typename Ty>
 __global__ __launch_bounds__(1024) void k_norm_long(NormArgs a) {
     __shared__ float slot[16];
-    const int64_t row = blockIdx.x;
+    const int64_t row = a.first + blockIdx.x;
     const Tx* x = static_cast<const Tx*>(a.x) + row_at(a, row, a.sb, a.sp);
     float s[1] = {0.f};
     for (int64_t col = threadIdx.x * 4L; col < a.n; col += 4096) {
@@ -324,7 +325,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_bwd_rows(NormArg
 template <typename Tx, typename Ty>
 __global__ __launch_bounds__(1024) void k_norm_bwd_long_sums(NormArgs a) {
     __shared__ float slot[32];
-    const int64_t row = blockIdx.x;
+    const int64_t row = a.first + blockIdx.x;
     const Tx* x = static_cast<const Tx*>(a.x) + row_at(a, row, a.sb, a.sp);
     const Ty* dy = static_cast<const Ty*>(a.dy) + row * a.n;
     const float mu = a.mean[row], r = a.rstd[row];
@@ -376,7 +377,7 @@ __global__ __launch_bounds__(256) void k_norm_bwd_long_cols(NormArgs a) {
 __global__ __launch_bounds__(1024) void k_norm_fold(NormArgs a) {
     __shared__ float s[32][33];
     const int c = threadIdx.x & 31, q = threadIdx.x >> 5;
-    const int64_t col = static_cast<int64_t>(blockIdx.x) * 32 + c;
+    const int64_t col = (a.first + blockIdx.x) * 32 + c;
     void* out = blockIdx.y ? a.dbias : a.dw;
     if (!out) return;
     float v = 0.f;
@@ -400,7 +401,7 @@ constexpr int kMapThreads = 512, kMapBig = 1024;
 // fours of points by 256 / tp consecutive columns, fall on different banks: ld = 64 / tp modulo 16 (map_ld).
 template <typename Tx>
 __device__ __forceinline__ void load_tile(const Tx* x, int64_t sn, int tp, int np, int64_t k0, int nk, float* tile, int ld) {
-    const int quads = tp >> 2;                      // 4, 8 or 16
+    const int quads = tp >> 2;                      // 4 or 8
     const int q = (threadIdx.x & (quads - 1)) * 4, step = blockDim.x / quads;
     for (int k = threadIdx.x / quads; k < nk; k += step) {
         const Tx* s = x + (k0 + k) * sn + q;
@@ -433,7 +434,7 @@ __global__ __launch_bounds__(kMapBig) void k_norm_maps(NormArgs a, int tp, int l
     extern __shared__ float tile[];
     __shared__ float stat[2][32];
     const int64_t tiles = (a.points + tp - 1) / tp;
-    const int64_t b = blockIdx.x / tiles, p0 = (blockIdx.x - b * tiles) * tp;
+    const int64_t id = a.first + blockIdx.x, b = id / tiles, p0 = (id - b * tiles) * tp;
     const int np = static_cast<int>(a.points - p0 < tp ? a.points - p0 : tp), n = static_cast<int>(a.n);
     load_tile(static_cast<const Tx*>(a.x) + b * a.sb + p0, a.sn, tp, np, 0, n, tile, ld);
     __syncthreads();
@@ -516,7 +517,7 @@ template <typename Tx, typename Ty>
 __global__ __launch_bounds__(kMapThreads) void k_norm_maps_long(NormArgs a) {
     __shared__ float tile[kPts * kLd];
     const int64_t tiles = (a.points + kPts - 1) / kPts;
-    const int64_t b = blockIdx.x / tiles, p0 = (blockIdx.x - b * tiles) * kPts;
+    const int64_t id = a.first + blockIdx.x, b = id / tiles, p0 = (id - b * tiles) * kPts;
     const int np = static_cast<int>(a.points - p0 < kPts ? a.points - p0 : kPts);
     const Tx* x = static_cast<const Tx*>(a.x) + b * a.sb + p0;
     const int lane = threadIdx.x & 63, w0 = threadIdx.x >> 6;   // a wave's points: w0 and w0 + 8
@@ -567,7 +568,7 @@ template <typename Tx, typename Ty>
 __global__ __launch_bounds__(kMapThreads) void k_norm_bwd_maps_sums(NormArgs a) {
     __shared__ float tile[kPts * kLd];
     const int64_t tiles = (a.points + kPts - 1) / kPts;
-    const int64_t b = blockIdx.x / tiles, p0 = (blockIdx.x - b * tiles) * kPts;
+    const int64_t id = a.first + blockIdx.x, b = id / tiles, p0 = (id - b * tiles) * kPts;
     const int np = static_cast<int>(a.points - p0 < kPts ? a.points - p0 : kPts);
     const Tx* x = static_cast<const Tx*>(a.x) + b * a.sb + p0;
     const int lane = threadIdx.x & 63, w0 = threadIdx.x >> 6;
@@ -768,51 +769,66 @@ size_t norm_bytes(const wst_norm_desc& d) {
     return (static_cast<size_t>(norm_groups(d)) * 2 * d.n + 2 * rows) * sizeof(float);
 }
 
+// A launch that asks for 2^32 threads or more is cut to what is left of them, without an error: calls with more blocks go in
+// several launches.
+template <typename F>
+void in_launches(NormArgs a, int64_t blocks, int threads, F launch) {
+    const int64_t most = (1LL << 31) / threads;
+    for (; a.first < blocks; a.first += most)
+        launch(a, static_cast<unsigned>(blocks - a.first < most ? blocks - a.first : most));
+}
+
 template <typename Tx, typename Ty>
-void norm_rows(const NormArgs& a, hipStream_t st) {
+void norm_rows(const NormArgs& args, hipStream_t st) {
     // one wave a row up to 2048 values, a block of 256 or 1024 threads up to 32768, three sweeps beyond
-    const int chunks = static_cast<int>((a.n + 255) / 256);
+    const int chunks = static_cast<int>((args.n + 255) / 256);
     if (chunks <= 8) {
-        const int per = a.rows >= 2048 ? 4 : 1;    // few rows: one to a block, so that they spread over the CUs
-        const dim3 g(static_cast<unsigned>((a.rows + per - 1) / per)), t(64 * per);
-        if (chunks <= 1) k_norm_rows<Tx, Ty, 4, 1, 64><<<g, t, 0, st>>>(a);
-        else if (chunks <= 2) k_norm_rows<Tx, Ty, 4, 2, 64><<<g, t, 0, st>>>(a);
-        else if (chunks <= 4) k_norm_rows<Tx, Ty, 4, 4, 64><<<g, t, 0, st>>>(a);
-        else k_norm_rows<Tx, Ty, 4, 8, 64><<<g, t, 0, st>>>(a);
-    } else if (a.n <= 8192) {
-        k_norm_rows<Tx, Ty, 4, 8, 256><<<dim3(static_cast<unsigned>(a.rows)), dim3(256), 0, st>>>(a);
-    } else if (a.n <= 32768) {
-        k_norm_rows<Tx, Ty, 4, 8, 1024><<<dim3(static_cast<unsigned>(a.rows)), dim3(1024), 0, st>>>(a);
+        const int per = args.rows >= 2048 ? 4 : 1;    // few rows: one to a block, so that they spread over the CUs
+        in_launches(args, (args.rows + per - 1) / per, 64 * per, [&](const NormArgs& a, unsigned blocks) {
+            const dim3 g(blocks), t(64 * per);
+            if (chunks <= 1) k_norm_rows<Tx, Ty, 4, 1, 64><<<g, t, 0, st>>>(a);
+            else if (chunks <= 2) k_norm_rows<Tx, Ty, 4, 2, 64><<<g, t, 0, st>>>(a);
+            else if (chunks <= 4) k_norm_rows<Tx, Ty, 4, 4, 64><<<g, t, 0, st>>>(a);
+            else k_norm_rows<Tx, Ty, 4, 8, 64><<<g, t, 0, st>>>(a);
+        });
+    } else if (args.n <= 8192) {
+        in_launches(args, args.rows, 256, [&](const NormArgs& a, unsigned blocks) {
+            k_norm_rows<Tx, Ty, 4, 8, 256><<<dim3(blocks), dim3(256), 0, st>>>(a);
+        });
     } else {
-        k_norm_long<Tx, Ty><<<dim3(static_cast<unsigned>(a.rows)), dim3(1024), 0, st>>>(a);
+        in_launches(args, args.rows, 1024, [&](const NormArgs& a, unsigned blocks) {
+            if (a.n <= 32768) k_norm_rows<Tx, Ty, 4, 8, 1024><<<dim3(blocks), dim3(1024), 0, st>>>(a);
+            else k_norm_long<Tx, Ty><<<dim3(blocks), dim3(1024), 0, st>>>(a);
+        });
     }
 }
 
 constexpr int kLdsMax = 160 * 1024;
 
 template <typename Tx, typename Ty>
-int norm_maps(const NormArgs& a, hipStream_t st) {
-    const int64_t batch = a.rows / a.points;
+int norm_maps(const NormArgs& args, hipStream_t st) {
+    const int64_t batch = args.rows / args.points;
     // Points a block takes: 32 make whole lines of 128 bytes; fewer when there are no more, or when the block's share of
     // the LDS would leave less than two to a CU.
     // ld: n + 1 or more (a pair may end behind the last column), 64 / tp modulo 16
-    auto map_ld = [&](int64_t tp) { return (a.n + 1 + 15 - 64 / tp) / 16 * 16 + 64 / tp; };
+    auto map_ld = [&](int64_t tp) { return (args.n + 1 + 15 - 64 / tp) / 16 * 16 + 64 / tp; };
     int tp = 32;
-    while (tp > 16 && (tp / 2 >= a.points || tp * map_ld(tp) * 4 > kLdsMax / 2 - 512)) tp >>= 1;
-    const int64_t ld = map_ld(tp), bytes = tp * ld * 4, tiles = (a.points + tp - 1) / tp;
+    while (tp > 16 && (tp / 2 >= args.points || tp * map_ld(tp) * 4 > kLdsMax / 2 - 512)) tp >>= 1;
+    const int64_t ld = map_ld(tp), bytes = tp * ld * 4, tiles = (args.points + tp - 1) / tp;
     const int threads = bytes > kLdsMax / 4 ? kMapBig : kMapThreads;      // two blocks of sixteen waves, or four of eight
     if (bytes <= kLdsMax - 1024) {
-        if (batch * tiles > 2147483647LL) return fail(WST_ERR_UNSUPPORTED, "layer norm: too many tiles");
-        const bool plain = a.w && a.b && a.wdt == WST_F32;
+        const bool plain = args.w && args.b && args.wdt == WST_F32;
         const void* kernel = plain ? reinterpret_cast<const void*>(&k_norm_maps<Tx, Ty, true>) : reinterpret_cast<const void*>(&k_norm_maps<Tx, Ty, false>);
         if (bytes > 64 * 1024 && hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsMax - 1024) != hipSuccess)
             return launched("layer norm");
-        const dim3 grid(static_cast<unsigned>(batch * tiles)), block(threads);
-        if (plain) k_norm_maps<Tx, Ty, true><<<grid, block, bytes, st>>>(a, tp, static_cast<int>(ld));
-        else k_norm_maps<Tx, Ty, false><<<grid, block, bytes, st>>>(a, tp, static_cast<int>(ld));
+        in_launches(args, batch * tiles, threads, [&](const NormArgs& a, unsigned blocks) {
+            if (plain) k_norm_maps<Tx, Ty, true><<<dim3(blocks), dim3(threads), bytes, st>>>(a, tp, static_cast<int>(ld));
+            else k_norm_maps<Tx, Ty, false><<<dim3(blocks), dim3(threads), bytes, st>>>(a, tp, static_cast<int>(ld));
+        });
     } else {
-        const int64_t all = batch * ((a.points + kPts - 1) / kPts);
-        k_norm_maps_long<Tx, Ty><<<dim3(static_cast<unsigned>(all)), dim3(kMapThreads), 0, st>>>(a);
+        in_launches(args, batch * ((args.points + kPts - 1) / kPts), kMapThreads, [&](const NormArgs& a, unsigned blocks) {
+            k_norm_maps_long<Tx, Ty><<<dim3(blocks), dim3(kMapThreads), 0, st>>>(a);
+        });
     }
     return WST_OK;
 }
@@ -835,7 +851,10 @@ void norm_bwd_rows(const NormArgs& a, hipStream_t st) {
         if (a.n % 4 == 0) norm_bwd_regs<Tx, Ty, true>(a, st);
         else norm_bwd_regs<Tx, Ty, false>(a, st);
     } else {
-        if (a.dx) k_norm_bwd_long_sums<Tx, Ty><<<dim3(static_cast<unsigned>(a.rows)), dim3(1024), 0, st>>>(a);
+        if (a.dx)
+            in_launches(a, a.rows, 1024, [&](const NormArgs& x, unsigned blocks) {
+                k_norm_bwd_long_sums<Tx, Ty><<<dim3(blocks), dim3(1024), 0, st>>>(x);
+            });
         k_norm_bwd_long_cols<Tx, Ty><<<dim3(static_cast<unsigned>((a.n + 255) / 256), a.groups), dim3(256), 0, st>>>(a);
     }
 }
@@ -843,7 +862,10 @@ void norm_bwd_rows(const NormArgs& a, hipStream_t st) {
 template <typename Tx, typename Ty>
 void norm_bwd_maps(const NormArgs& a, hipStream_t st) {
     const int64_t tiles = a.rows / a.points * ((a.points + kPts - 1) / kPts);
-    if (a.dx) k_norm_bwd_maps_sums<Tx, Ty><<<dim3(static_cast<unsigned>(tiles)), dim3(kMapThreads), 0, st>>>(a);
+    if (a.dx)
+        in_launches(a, tiles, kMapThreads, [&](const NormArgs& x, unsigned blocks) {
+            k_norm_bwd_maps_sums<Tx, Ty><<<dim3(blocks), dim3(kMapThreads), 0, st>>>(x);
+        });
     k_norm_bwd_maps<Tx, Ty><<<dim3(static_cast<unsigned>((a.n + kBCols - 1) / kBCols), a.groups), dim3(kMapThreads), 0, st>>>(a);
 }
 
@@ -1011,7 +1033,10 @@ int wst_layer_norm_backward(const wst_norm_desc* d, const void* x, const void* w
             return 0;
         });
     });
-    if (a.part) k_norm_fold<<<dim3(static_cast<unsigned>((d->n + 31) / 32), 2), dim3(1024), 0, st>>>(a);
+    if (a.part)
+        in_launches(a, (d->n + 31) / 32, 1024, [&](const NormArgs& x, unsigned blocks) {
+            k_norm_fold<<<dim3(blocks, 2), dim3(1024), 0, st>>>(x);
+        });
     return launched("layer norm backward");
 }
 
@@ -1054,7 +1079,7 @@ int wst_rotary(const wst_rotary_desc* d, const void* q, void* q_out, const void*
     a.sign = d->inverse ? -1.f : 1.f;
     const int units = (a.pairs + kRotPairs - 1) / kRotPairs + (a.dim - 2 * a.pairs + 7) / 8;
     const double blocks = std::ceil(static_cast<double>(a.rows) * units / 256.0);
-    if (blocks > 2147483647.0) return fail(WST_ERR_UNSUPPORTED, "rotary: too many tokens");
+    if (blocks * 256 >= 4294967296.0) return fail(WST_ERR_UNSUPPORTED, "rotary: too many tokens for one launch");
     // a thread walks all heads with one set of angles; few tokens: the heads are shared out over more blocks
     const int total = a.heads[0] + a.heads[1];
     int split = static_cast<int>(2048.0 / blocks);
