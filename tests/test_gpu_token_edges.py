@@ -159,3 +159,22 @@ def test_layer_norm_of_more_rows_than_a_launch_holds(rows, n, layout):
     _hold(db, want["db"], "db")
     for part in dx[ends:-ends].split(1 << 20):
         assert not bool(part.any())
+
+
+def test_views_that_negate_when_read():
+    """The imaginary part of a conjugate holds the number's own, and a flag; gradients may come as such views too."""
+    x = torch.randn(2, 6, 2, 8, device="cuda")
+    pos, slopes = torch.arange(6, dtype=torch.int32, device="cuda")[:, None], torch.ones(2, device="cuda")
+    calls = [lambda x: tokens.layer_norm(x), lambda x: tokens.layer_norm(x[0, 0, 0]),
+             lambda x: tokens.layer_norm(x, x[0, 0, 0], x[0, 0, 1]), lambda x: torch.cat(tokens.rotary(x, pos, (4,), k=x)),
+             lambda x: tokens.attention(x, x, x, slopes=x[0, 0, :, 0])]
+    imag = torch.complex(torch.zeros_like(x), x).conj().imag
+    for view, value in ((imag, -x), (torch._neg_view(x), -x)):
+        assert view.is_neg() and torch.equal(view, value)
+        for n, call in enumerate(calls):
+            assert torch.equal(call(view), call(value)), n
+            leaf = value.clone().requires_grad_()
+            y = call(leaf)
+            dy = torch.randn_like(y)
+            got, want = (torch.autograd.grad(y, leaf, d, retain_graph=True)[0] for d in (torch._neg_view(dy), -dy))
+            assert torch.equal(got, want), n

@@ -165,7 +165,7 @@ class _LayerNorm(torch.autograd.Function):
                 dx = dx.view(ctx.x_shape)
             else:
                 dx = _like(xs)
-        dy = dy.contiguous()
+        dy = dy.resolve_neg().contiguous()
         d = _lib.NORM_PACK.pack(*view, *dview, DTYPES[xs.dtype], DTYPES[dy.dtype],
                                 DTYPES[weight.dtype] if weight is not None else DTYPES[db.dtype] if want_b else 0, ctx.eps)
         lib, need = _lib.token_calls(), ctypes.c_size_t()
@@ -200,8 +200,9 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, out_dtype=None):
     eps = float(eps)
     if not eps >= 0.0:
         raise RuntimeError("eps must not be negative")
-    weight = None if weight is None else weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
+    x = x.resolve_neg()                         # a view that negates when it is read, which the library would not
+    weight = None if weight is None else weight.resolve_neg().contiguous()
+    bias = None if bias is None else bias.resolve_neg().contiguous()
     if _wants_grad(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, eps, out_dtype)
     return _norm_forward(x, weight, bias, eps, out_dtype, False)[0]
@@ -268,7 +269,7 @@ class _Rotary(torch.autograd.Function):
     def backward(ctx, dq, dk=None):
         _first_order()
         positions, = ctx.saved_tensors
-        gq, gk = _rotate(dq, dk, positions, *ctx.how, 1)
+        gq, gk = _rotate(dq.resolve_neg(), None if dk is None else dk.resolve_neg(), positions, *ctx.how, 1)
         return gq, gk, None, None, None, None
 
 
@@ -303,6 +304,7 @@ def rotary(q, positions, sections, base=10000.0, interleaved=False, k=None):
     if not 0.0 < base < float("inf"):
         raise RuntimeError("base must be positive")
     positions = positions.contiguous()
+    q, k = q.resolve_neg(), None if k is None else k.resolve_neg()
     if _wants_grad(q, k):
         return _Rotary.apply(q, k, positions, sections, base, bool(interleaved))
     qo, ko = _rotate(q, k, positions, sections, base, bool(interleaved), 0)
@@ -380,7 +382,7 @@ class _Attention(torch.autograd.Function):
         dslopes = torch.empty_like(slopes) if want[3] else None
         if not q.numel() or not k.numel():
             return tuple(None if t is None else t.zero_() for t in (dq, dk, dv, dslopes)) + (None,)
-        do = _lined_up(do)
+        do = _lined_up(do.resolve_neg())
         d = _attention_desc(q, k, v, slopes, ctx.side, o, rest)
         g = _lib.GRADS_PACK.pack(o.data_ptr(), do.data_ptr(), lse.data_ptr(), _ptr0(dq), _ptr0(dk), _ptr0(dv), _ptr0(dslopes),
                                  *_call_strides(do), *_grad_strides(dq), *_grad_strides(dk), *_grad_strides(dv))
@@ -436,7 +438,7 @@ def attention(q, k, v, *, scale=None, cap=0.0, slopes=None, q_positions=None, k_
             raise TypeError(f"slopes must be float32, not {slopes.dtype}")
         if slopes.shape != (H,):
             raise RuntimeError(f"slopes must be of shape ({H},), not {tuple(slopes.shape)}")
-        slopes = slopes.contiguous()
+        slopes = slopes.resolve_neg().contiguous()
     if (q_positions is None) != (k_positions is None) or (q_documents is None) != (k_documents is None):
         raise RuntimeError("positions and documents are given for queries and keys alike")
     if q_positions is not None and slopes is None:
@@ -461,7 +463,7 @@ def attention(q, k, v, *, scale=None, cap=0.0, slopes=None, q_positions=None, k_
     if not abs(s.scale) < float("inf"):
         raise RuntimeError("scale must be finite")
     s.settle()
-    q, k, v = _lined_up(q), _lined_up(k), _lined_up(v)
+    q, k, v = _lined_up(q.resolve_neg()), _lined_up(k.resolve_neg()), _lined_up(v.resolve_neg())
     if _wants_grad(q, k, v, slopes):
         o, lse = _Attention.apply(q, k, v, slopes, s)
     else:
