@@ -284,6 +284,7 @@ const char* wst_aux_last_error(void);
 enum wst_dtype { WST_F32 = 0, WST_BF16 = 1, WST_F16 = 2 };
 
 #define WST_MAX_AXES 4            /* of rotary positions */
+#define WST_MAX_PAIRS 128         /* that they turn, over all axes */
 #define WST_MAX_DISTANCE_AXES 3   /* of attention's distances */
 #define WST_MAX_HEAD_DIM 256
 

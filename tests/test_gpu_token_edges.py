@@ -178,3 +178,10 @@ def test_views_that_negate_when_read():
             dy = torch.randn_like(y)
             got, want = (torch.autograd.grad(y, leaf, d, retain_graph=True)[0] for d in (torch._neg_view(dy), -dy))
             assert torch.equal(got, want), n
+
+
+def test_rotary_of_more_pairs_than_it_has_is_refused():
+    q, pos = torch.zeros(1, 3, 1, 300, device="cuda"), torch.zeros(3, 2, dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="sections must turn at most 128 pairs, not 129"):
+        tokens.rotary(q, pos, (64, 65))
+    assert torch.equal(tokens.rotary(q, pos, (64, 64)), q)

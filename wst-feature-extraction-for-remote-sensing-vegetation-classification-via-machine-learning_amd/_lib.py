@@ -76,7 +76,7 @@ def _conv_ptr(convention):
 
 _I64, _I32, _PTR = ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p
 _STRIDES = _I64 * 3
-MAX_AXES, MAX_DISTANCE_AXES, MAX_HEAD_DIM = 4, 3, 256
+MAX_AXES, MAX_PAIRS, MAX_DISTANCE_AXES, MAX_HEAD_DIM = 4, 128, 3, 256
 
 
 class NormDesc(ctypes.Structure):

@@ -395,13 +395,14 @@ __global__ __launch_bounds__(1024) void k_norm_fold(NormArgs a) {
 
 // ------------------------------------------------------------------------------------------ layer norm, maps
 constexpr int kMapThreads = 512, kMapBig = 1024;
+constexpr int kMapPts = 32;      // points of a block at most
 
 // Copies columns [k0, k0 + nk) of the points [p0, p0 + np) of one batch entry into LDS, turned: tile[p][k], row
 // stride ld. Global memory is read along the points (four at a time), LDS written so that the lanes of a wave, tp / 4
 // fours of points by 256 / tp consecutive columns, fall on different banks: ld = 64 / tp modulo 16 (map_ld).
 template <typename Tx>
 __device__ __forceinline__ void load_tile(const Tx* x, int64_t sn, int tp, int np, int64_t k0, int nk, float* tile, int ld) {
-    const int quads = tp >> 2;                      // 4 or 8
+    const int quads = tp >> 2;                      // 4 or 8: tp is 16 or kMapPts
     const int q = (threadIdx.x & (quads - 1)) * 4, step = blockDim.x / quads;
     for (int k = threadIdx.x / quads; k < nk; k += step) {
         const Tx* s = x + (k0 + k) * sn + q;
@@ -432,7 +433,7 @@ constexpr int kPack = sizeof(Ty) == 2 ? 2 : 1;
 template <typename Tx, typename Ty, bool PLAIN>
 __global__ __launch_bounds__(kMapBig) void k_norm_maps(NormArgs a, int tp, int ld) {
     extern __shared__ float tile[];
-    __shared__ float stat[2][32];
+    __shared__ float stat[2][kMapPts];
     const int64_t tiles = (a.points + tp - 1) / tp;
     const int64_t id = a.first + blockIdx.x, b = id / tiles, p0 = (id - b * tiles) * tp;
     const int np = static_cast<int>(a.points - p0 < tp ? a.points - p0 : tp), n = static_cast<int>(a.n);
@@ -812,7 +813,7 @@ int norm_maps(const NormArgs& args, hipStream_t st) {
     // the LDS would leave less than two to a CU.
     // ld: n + 1 or more (a pair may end behind the last column), 64 / tp modulo 16
     auto map_ld = [&](int64_t tp) { return (args.n + 1 + 15 - 64 / tp) / 16 * 16 + 64 / tp; };
-    int tp = 32;
+    int tp = kMapPts;
     while (tp > 16 && (tp / 2 >= args.points || tp * map_ld(tp) * 4 > kLdsMax / 2 - 512)) tp >>= 1;
     const int64_t ld = map_ld(tp), bytes = tp * ld * 4, tiles = (args.points + tp - 1) / tp;
     const int threads = bytes > kLdsMax / 4 ? kMapBig : kMapThreads;      // two blocks of sixteen waves, or four of eight
@@ -874,7 +875,7 @@ void norm_bwd_maps(const NormArgs& a, hipStream_t st) {
 // a revolution: position * (frequency / 2 pi) in 64 bits less its whole part, so far positions lose nothing; the
 // sine and cosine of what is left are taken in 32 bits. The angle depends on token and pair alone, so a thread
 // computes it once and applies it to all its heads.
-constexpr int kMaxPairs = 128;
+constexpr int kMaxPairs = WST_MAX_PAIRS;
 
 struct RotaryTable {
     double rev[kMaxPairs];        // revolutions a step of position

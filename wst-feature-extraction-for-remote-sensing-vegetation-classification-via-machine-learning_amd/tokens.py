@@ -277,8 +277,8 @@ def rotary(q, positions, sections, base=10000.0, interleaved=False, k=None):
     """Rotary positions with several axes.
 
     q (B, T, H, D) and, in the same call, k (B, T, Hk, D); positions int32 (T, A) or (B, T, A), 1 <= A <= 4, such as
-    ``grid_positions``; sections: the pairs that each of the A axes turns.  The first 2 * sum(sections) values of a head
-    are turned, the rest copied.  Pair i of an axis with s pairs turns by ``position * base**(-i / s)``.  With P pairs in
+    ``grid_positions``; sections: the pairs that each of the A axes turns, 128 in all at most.  The first
+    2 * sum(sections) values of a head are turned, the rest copied.  Pair i of an axis with s pairs turns by ``position * base**(-i / s)``.  With P pairs in
     all, pair p is the values (p, p + P), or (2p, 2p + 1) when ``interleaved``.  Returns q turned, or (q, k)."""
     _check_tensor(q, "q")
     _dtype_id(q, "q")
@@ -296,6 +296,8 @@ def rotary(q, positions, sections, base=10000.0, interleaved=False, k=None):
         raise RuntimeError(f"sections must be 1 to {_lib.MAX_AXES} numbers of pairs")
     if 2 * sum(sections) > D:
         raise RuntimeError(f"{sum(sections)} pairs do not fit heads of {D} values")
+    if sum(sections) > _lib.MAX_PAIRS:
+        raise RuntimeError(f"sections must turn at most {_lib.MAX_PAIRS} pairs, not {sum(sections)}")
     _check_ints(positions, "positions", q)
     A = len(sections)
     if tuple(positions.shape) not in ((T, A), (B, T, A)):
@@ -402,7 +404,7 @@ def _check_side(t, name, like, shapes):
 
 def attention(q, k, v, *, scale=None, cap=0.0, slopes=None, q_positions=None, k_positions=None, q_documents=None,
               k_documents=None, causal=False, prefix=None, k_lengths=None, return_lse=False):
-    """Softmax attention of q (B, Tq, H, D) over k, v (B, Tk, Hk, D); H a multiple of Hk, D <= 256.
+    """Softmax attention of q (B, Tq, H, D) over k, v (B, Tk, Hk, D); H a multiple of Hk, D <= 256, B and H <= 65535.
 
     With ``L = k_lengths[b]`` (default Tk) and ``place(i) = i + L - Tq``, query i scores key j as
     ``z = scale * q_i.k_j`` (scale defaults to ``D ** -0.5``), ``z = cap * tanh(z / cap)`` where ``cap > 0`` (1e-30 to 1e30), and
