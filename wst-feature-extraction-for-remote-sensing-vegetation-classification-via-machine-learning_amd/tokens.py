@@ -417,7 +417,10 @@ def attention(q, k, v, *, scale=None, cap=0.0, slopes=None, q_positions=None, k_
     * ``q_documents[i] == k_documents[j] >= 0`` where given (int32 (T,) or (B, T); negative belongs to none).
 
     What is not seen has no influence, not even infinities or NaN.  A query that sees nothing gets 0, and no gradient.
-    Gradients reach q, k, v and slopes.  Returns o (B, Tq, H, D), and with ``return_lse`` the float32 (B, H, Tq)
+    Gradients reach q, k, v and slopes.  In float16 the backward pass does rows and keys whose score gradients exceed
+    2**10 over, one by one: right, but slow where a loss scale makes that most of them (1024 tokens, 8 heads of 64: 100 us,
+    with output gradients of 2**10 450 us and of 2**13 5.3 ms); bfloat16 has no such bound.  So it is in every type for
+    rows and keys that see a value that is not finite.  Returns o (B, Tq, H, D), and with ``return_lse`` the float32 (B, H, Tq)
     log-sum-exp of the scores (-inf where nothing is seen; it has no gradient)."""
     for t, name in ((q, "q"), (k, "k"), (v, "v")):
         _check_tensor(t, name, q if t is not q else None)
