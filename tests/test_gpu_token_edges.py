@@ -6,7 +6,7 @@ from torch.autograd import forward_ad
 import token_cases
 import wst_amd  # noqa: F401
 from oracle import token_ops as ref
-from test_gpu_tokens import BF16, F16, F32, _attention_inputs, _check_attention, _documents, _hold, _norm_inputs
+from test_gpu_tokens import BF16, F16, F32, _attention_inputs, _check_attention, _documents, _gen, _hold, _norm_inputs
 from wst_amd import tokens
 
 pytestmark = pytest.mark.gpu
@@ -198,3 +198,36 @@ def test_attention_float16_large_output_gradients(gain, D):
     slopes = torch.rand(4, generator=g) * 0.1
     for kw in (dict(causal=True), dict(cap=5.0, slopes=slopes)):
         _check_attention(q, k, v, do, **kw)
+
+
+@pytest.mark.parametrize("D", [32, 64, 12])
+@pytest.mark.parametrize("height", [0.0, 1000.0, 100000.0])
+def test_attention_float32_gradients_of_high_scores(height, D):
+    """Every score is a height plus small steps, all exact in float32. Weights rebuilt from a float32 log-sum-exp of that height
+    alone would be off by half an ulp of it, 2^-24 * 2^16 = 4e-3 of themselves at 1e5, and every gradient with them.
+    Normalised, what is left of a weight's error is its own exponent's (two roundings of numbers below 16, log2 e's times the
+    steps, 4 for exp2) and that of the sum over T weights; a result adds a sum over D, T or both: below (2 T + 64 + D) 2^-24 of
+    the magnitudes' sums, and twice for a score gradient of two parts."""
+    T, H = 96, 2
+    g = _gen(int(height) + D)
+    # q.k = height exactly: one column of q and k; the others hold eighths, whose products are exact
+    q, k = (torch.randint(-4, 5, (1, T, h, D), generator=g).float() / 8 for h in (H, H))
+    q[..., 4:], k[..., 4:] = 0, 0
+    q[..., 0], k[..., 0] = height, 1.0
+    v, do = torch.randn(1, T, H, D, generator=g), torch.randn(1, T, H, D, generator=g)
+    slopes = torch.full((H,), 2.0 ** -6)                        # distances below 96 times 2^-6: exact
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v, slopes)]
+    o = tokens.attention(*leaves[:3], scale=1.0, slopes=leaves[3])
+    grads = torch.autograd.grad(o, leaves, do.cuda())
+    Q, K, V, G = (t.double().transpose(1, 2) for t in (q, k, v, do))
+    far = (torch.arange(T)[:, None] - torch.arange(T)).abs().double()
+    p = (Q @ K.transpose(2, 3) - 2.0 ** -6 * far).softmax(-1)
+    dp = G @ V.transpose(2, 3)
+    delta = (p * dp).sum(-1, keepdim=True)
+    ds, size = p * (dp - delta), p * (G.abs() @ V.abs().transpose(2, 3) + (p * (G.abs() @ V.abs().transpose(2, 3))).sum(-1, keepdim=True))
+    tol = 2 * (2 * T + 64 + D) * 2.0 ** -24
+    for got, want, most in zip(grads, ((ds @ K), (ds.transpose(2, 3) @ Q), (p.transpose(2, 3) @ G), -(ds * far).sum((0, 2, 3))),
+                               ((size @ K.abs()), (size.transpose(2, 3) @ Q.abs()), (p.transpose(2, 3) @ G.abs()), (size * far).sum((0, 2, 3)))):
+        got = got.double().cpu()
+        got = got if got.dim() == 1 else got.transpose(1, 2)
+        assert bool(((got - want).abs() <= tol * most).all()), float(((got - want).abs() / most).max() / tol)

@@ -31,6 +31,7 @@ struct AttnArgs {
     void* o;
     float* lse;
     float* delta;        // (batch, heads, q_len)
+    float* unit;         // float32: (batch, heads, q_len), 1 / the sum of the weights that the backward pass rebuilds; else null
     float* slope_part;   // (heads, batch, slots)
     float *part, *part_ml;   // forward: (splits, rows, dim) and (splits, rows, 2); backward: (parts, keys, 2, dim)
     int slots, splits, parts;
@@ -173,6 +174,13 @@ __device__ void row_forward(const AttnArgs& a, const Scope& sc, int64_t b, int h
     if (lane == 0 && a.lse) a.lse[(b * d.q_heads + h) * d.q_len + i] = l == 0.f ? -INFINITY : m + logf(l);
 }
 
+// What makes a row's rebuilt weights add up to 1. They come as exp(s - lse), and lse is a float32 number: its rounding is
+// half an ulp of the largest score, the same for all weights of the row (and in powers of two once more). 16-bit weights lose
+// more when they are rounded; float32 gradients are the nearer to the exact ones so (256 keys: dq 3.9e-7 for 5.0e-7, dk 3.2
+// for 4.5, dv 3.0 for 4.5; 16 x 256, 4 heads x 32: dk/dv 23.5 us for 22.6, dq no slower), most of all where scores stand far
+// from 0 (at 1e5 a log-sum-exp of float32 is off by 4e-3).
+__device__ __forceinline__ float unit_of(float sum) { return sum > 0.f && sum < INFINITY ? 1.f / sum : 1.f; }
+
 // The gradient of one query, and its share of -sum ds distance. LDS: q and do of the row.
 template <typename T>
 __device__ float row_dq(const AttnArgs& a, const Scope& sc, int64_t b, int h, int i, float* q, float* dout) {
@@ -187,7 +195,7 @@ __device__ float row_dq(const AttnArgs& a, const Scope& sc, int64_t b, int h, in
     const float slope = d.slopes ? d.slopes[h] : 0.f;
     const int64_t row = (b * d.q_heads + h) * d.q_len + i;
     const float lse = a.g.lse[row], delta = a.delta[row];
-    float acc[kPer] = {}, share = 0.f;
+    float acc[kPer] = {}, share = 0.f, sum = 0.f;
     if (lse != -INFINITY)
         for (int j0 = 0; j0 < sc.length; j0 += 64) {
             const int j = j0 + lane;
@@ -198,7 +206,9 @@ __device__ float row_dq(const AttnArgs& a, const Scope& sc, int64_t b, int h, in
                 float s = capped(dot_row(q, at<T>(d.k, d.k_strides, b, j, kvh), d.dim) * d.scale, d.cap, grad);
                 const float far = d.slopes ? sc.distance(i, j) : 0.f;
                 s -= slope * far;
-                const float ds = expf(s - lse) * (dot_row(dout, at<T>(d.v, d.v_strides, b, j, kvh), d.dim) - delta);
+                const float p = expf(s - lse);
+                sum += p;
+                const float ds = p * (dot_row(dout, at<T>(d.v, d.v_strides, b, j, kvh), d.dim) - delta);
                 share -= ds * far;
                 dz = ds * grad * d.scale;
             }
@@ -211,13 +221,15 @@ __device__ float row_dq(const AttnArgs& a, const Scope& sc, int64_t b, int h, in
                     if (lane + 64 * c < d.dim) acc[c] += x * static_cast<float>(k[lane + 64 * c]);
             }
         }
+    const float unit = a.unit ? unit_of(wave_sum(sum)) : 1.f;
+    if (a.unit && lane == 0) a.unit[row] = unit;
     if (a.g.dq) {
         T* o = const_cast<T*>(at<T>(a.g.dq, a.g.dq_strides, b, i, h));
 #pragma unroll
         for (int c = 0; c < kPer; ++c)
-            if (lane + 64 * c < d.dim) o[lane + 64 * c] = static_cast<T>(acc[c]);
+            if (lane + 64 * c < d.dim) o[lane + 64 * c] = static_cast<T>(acc[c] * unit);
     }
-    return wave_sum(share);
+    return wave_sum(share) * unit;
 }
 
 // The gradients of one key and value, over all queries of the heads that share it. LDS: k and v of the row.
@@ -243,7 +255,7 @@ __device__ void row_dkv(const AttnArgs& a, const Scope& sc, int64_t b, int kvh, 
                 float grad;
                 float s = capped(dot_row(k, at<T>(d.q, d.q_strides, b, i, h), d.dim) * d.scale, d.cap, grad);
                 if (d.slopes) s -= slope * sc.distance(i, j);
-                p = expf(s - a.g.lse[row]);
+                p = expf(s - a.g.lse[row]) * (a.unit ? a.unit[row] : 1.f);
                 dz = p * (dot_row(v, at<T>(a.g.d_o, a.g.do_strides, b, i, h), d.dim) - a.delta[row]) * grad * d.scale;
             }
             for (uint64_t w = __ballot(see); w; w &= w - 1) {
@@ -1482,7 +1494,7 @@ __global__ __launch_bounds__(256 * TEAMS, sizeof(T) == 2 ? 2 : 1) void k_attn_dq
     for (int k = 0; k < DP / 32; ++k) dq[k] = zero16();
     // The slopes' share, -sum ds far. delta comes from the rounded output, and its error would meet a mean distance: with
     // e = sum ds (0, were delta exact) the share is -(sum ds far - e sum p far).
-    float pf = 0.f, e0 = 0.f, e1 = 0.f;
+    float pf = 0.f, e0 = 0.f, e1 = 0.f, whole_p = 0.f;      // whole_p: float32, the sum of the weights (unit_of)
     const bool slopes_too = a.slope_part != nullptr;
 
     const T *kb = at<T>(d.k, d.k_strides, b, 0, kvh), *vb = at<T>(d.v, d.v_strides, b, 0, kvh);
@@ -1565,6 +1577,7 @@ __global__ __launch_bounds__(256 * TEAMS, sizeof(T) == 2 ? 2 : 1) void k_attn_dq
                 x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], sh.mul, base));
                 dp[r] *= x[r];
             }
+            if constexpr (sizeof(T) == 4) whole_p += sum16(x);
             if (kind.bias && slopes_too) {
                 float u = 0.f, v = 0.f, y = 0.f;       // sums of their own first: thousands of terms lose little so
 #pragma unroll
@@ -1628,7 +1641,12 @@ __global__ __launch_bounds__(256 * TEAMS, sizeof(T) == 2 ? 2 : 1) void k_attn_dq
         e1 += sums[(DP / 2 + 2) * 64];
     }
     const AttnArgs& z = again();
-    const float mul = z.d.scale / kUp<T>;
+    float mul = z.d.scale / kUp<T>, unit = 1.f;
+    if constexpr (sizeof(T) == 4) {
+        unit = unit_of(halves_sum(whole_p));
+        mul *= unit;
+        if (ok && hl == 0) z.unit[row] = unit;
+    }
     if (ok && z.g.dq) {
         T* out = const_cast<T*>(at<T>(z.g.dq, z.g.dq_strides, b, i, h));
 #pragma unroll
@@ -1641,7 +1659,7 @@ __global__ __launch_bounds__(256 * TEAMS, sizeof(T) == 2 ? 2 : 1) void k_attn_dq
             }
     }
     if (z.slope_part) {
-        const float share = halves_sum(e0) * halves_sum(pf) - halves_sum(e1), sum = wave_sum(hl ? 0.f : share);
+        const float share = (halves_sum(e0) * (halves_sum(pf) * unit) - halves_sum(e1)) * unit, sum = wave_sum(hl ? 0.f : share);
         if (lane == 0) z.slope_part[(static_cast<int64_t>(h) * z.d.batch + b) * z.slots + qt * 4 + w] = sum;
     }
     uint64_t bad = __ballot(ok && not_finite<T, DP>(dq));      // see k_attn_fwd
@@ -1681,6 +1699,8 @@ __global__ __launch_bounds__(dkv_threads(sizeof(T), DP), sizeof(T) == 2 ? 2 : 1)
     __shared__ __attribute__((aligned(256))) char pool[4 * kTile + (kWide ? 2 * kOwn : 0)];
     char *qt = pool, *dt = pool + 2 * kTile, *kt = pool + 4 * kTile, *vt = kt + kOwn;
     __shared__ Rows rows[3];
+    constexpr bool kUnit = sizeof(T) == 4;
+    __shared__ __attribute__((aligned(16))) float units[3][kUnit ? 64 : 4];
     __shared__ Marks marks;
     __shared__ float scratch[TH / 64][2][DP];
     const wst_attention_desc& d = a.d;
@@ -1767,7 +1787,7 @@ __global__ __launch_bounds__(dkv_threads(sizeof(T), DP), sizeof(T) == 2 ? 2 : 1)
         for (int k = 0; k < n && !x.s.done(walk); ++k) x = step(x);
         return x;
     };
-    float r_base = -INFINITY, r_delta = 0.f;
+    float r_base = -INFINITY, r_delta = 0.f, r_unit = 1.f;
     int r_limit = 0, r_doc = -1, r_place = 0;
     uint32_t r_pos = 0;
     auto load = [&](Item x) {
@@ -1781,12 +1801,15 @@ __global__ __launch_bounds__(dkv_threads(sizeof(T), DP), sizeof(T) == 2 ? 2 : 1)
             if (sc.q_doc && r_doc < 0) r_limit = 0;
             r_base = lse == -INFINITY || r_limit <= 0 ? -INFINITY : sh.add - lse * kLog2e;
             r_delta = in ? -a.delta[row] : 0.f;
+            if constexpr (kUnit) r_unit = in ? a.unit[row] : 1.f;
             r_place = i + sc.shift;
         }
         if (sc.q_pos) r_pos = (t >> 6) < sc.axes && in ? static_cast<uint32_t>(sc.q_pos[static_cast<int64_t>(i) * sc.axes + (t >> 6)]) + kPosBias : 0u;
     };
-    auto put = [&](Rows& rw) {
+    auto put = [&](int n) {
+        Rows& rw = rows[n];
         if (t < 64) {
+            if constexpr (kUnit) units[n][t] = r_unit;
             rw.base[t] = r_base;
             rw.delta[t] = r_delta;
             rw.limit[t] = r_limit;
@@ -1810,11 +1833,11 @@ __global__ __launch_bounds__(dkv_threads(sizeof(T), DP), sizeof(T) == 2 ? 2 : 1)
     Item nxt = skip(cur, stride);
     if (!cur.s.done(walk)) {
         load(cur);
-        put(rows[0]);
+        put(0);
     }
     if (!nxt.s.done(walk)) {
         load(nxt);
-        put(rows[1]);
+        put(1);
     }
     __syncthreads();
     if (!cur.s.done(walk)) fetch(cur, 0, rows[0]);
@@ -1913,6 +1936,11 @@ __global__ __launch_bounds__(dkv_threads(sizeof(T), DP), sizeof(T) == 2 ? 2 : 1)
                 const f32x4 v = *reinterpret_cast<const f32x4*>(&rw.base[row_half + 32 * n + 8 * c + 4 * hl]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[4 * c + e] = __builtin_amdgcn_exp2f(fmaf(x[4 * c + e], sh.mul, v[e]));
+                if constexpr (kUnit) {
+                    const f32x4 u = *reinterpret_cast<const f32x4*>(&units[turn][row_half + 32 * n + 8 * c + 4 * hl]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[4 * c + e] *= u[e];
+                }
             }
             if constexpr (MASK != 0) {
 #pragma unroll
@@ -1970,7 +1998,7 @@ __global__ __launch_bounds__(dkv_threads(sizeof(T), DP), sizeof(T) == 2 ? 2 : 1)
                 if constexpr (sizeof(T) == 2) paced<DP / 8, 2, 4>();
             }
         }
-        if (!after.s.done(walk)) put(rows[turn2]);
+        if (!after.s.done(walk)) put(turn2);
         cur = nxt;
         nxt = after;
         buf ^= 1;

@@ -100,7 +100,7 @@ AttnPlan plan_of(const wst_attention_desc& d, bool tiles) {
         p.slots = static_cast<int>((d.q_len + kBQ - 1) / kBQ * 4);
         if (p.parts > 1) p.backward = static_cast<size_t>(p.parts) * d.batch * d.k_heads * d.k_len * 2 * d.dim;
     }
-    p.backward += rows;
+    p.backward += d.dtype == WST_F32 ? 2 * rows : rows;
     if (d.slopes) p.backward += static_cast<size_t>(d.q_heads) * d.batch * p.slots;
     return p;
 }
@@ -183,6 +183,10 @@ int wst_attention_backward(const wst_attention_desc* d, const wst_attention_grad
     a.slots = p.slots;
     a.parts = p.parts;
     float* rest = a.delta + rows_of(*d);
+    if (d->dtype == WST_F32) {
+        a.unit = rest;
+        rest += rows_of(*d);
+    }
     if (d->slopes) {
         if (g->dslopes) a.slope_part = rest;
         rest += static_cast<size_t>(d->q_heads) * d->batch * p.slots;
@@ -196,7 +200,7 @@ int wst_attention_backward(const wst_attention_desc* d, const wst_attention_grad
             return;
         }
         launch_delta<T>(a, st);
-        if (g->dq || g->dslopes)
+        if (g->dq || g->dslopes || a.unit)
             k_attn_dq_rows<T><<<dim3(static_cast<unsigned>((d->q_len + 3) / 4), d->q_heads, static_cast<unsigned>(d->batch)), dim3(256), 0, st>>>(a);
         if (g->dk || g->dv)
             k_attn_dkv_rows<T><<<dim3(static_cast<unsigned>((d->k_len + 3) / 4), d->k_heads, static_cast<unsigned>(d->batch)), dim3(256), 0, st>>>(a);

@@ -52,7 +52,8 @@ void attend(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
 template <typename T, int DP>
 void attend_backward(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
     const wst_attention_desc& d = a.d;
-    const bool want_q = a.g.dq || a.g.dslopes, want_k = a.g.dk || a.g.dv;
+    // float32: what makes the weights add up to 1 comes from the walk over the keys too
+    const bool want_q = a.g.dq || a.g.dslopes || a.unit, want_k = a.g.dk || a.g.dv;
     if (!want_q) launch_delta<T>(a, st);
     with_kind<T>(d, [&](auto cap, auto bias) {
         constexpr int CAP = decltype(cap)::value, BIAS = decltype(bias)::value;
