@@ -8,6 +8,7 @@ import wst_amd  # noqa: F401
 from oracle import token_ops as ref
 from test_gpu_tokens import BF16, F16, F32, _attention_inputs, _check_attention, _documents, _gen, _hold, _norm_inputs
 from wst_amd import tokens
+from wst_amd.torch import ScatteringAttention
 
 pytestmark = pytest.mark.gpu
 
@@ -231,3 +232,21 @@ def test_attention_float32_gradients_of_high_scores(height, D):
         got = got.double().cpu()
         got = got if got.dim() == 1 else got.transpose(1, 2)
         assert bool(((got - want).abs() <= tol * most).all()), float(((got - want).abs() / most).max() / tol)
+
+
+def test_scattering_attention_under_autocast():
+    """The projections come in the autocast's type, the other parameters are float32: the read-out takes both. Against the same
+    module without autocast: weights, projections, rotary, attention and read-out round to bfloat16 eight times in a row or
+    fewer, each by at most 2^-8 of a value, and a score's relative error comes out of the softmax at most cap = 4 times as
+    large."""
+    torch.manual_seed(5)
+    net = ScatteringAttention(2, (32, 32), channels=1, heads=2, dim=24, L=2, cap=4.0).cuda()
+    images, owner = torch.rand(2, 3, 1, 32, 32, device="cuda"), torch.tensor([[0, 0, 1], [1, -1, 0]], dtype=torch.int32)
+    want = [net(images, owner), net.pooled(images, owner, 2)]
+    with torch.autocast("cuda", dtype=BF16):
+        got = [net(images, owner), net.pooled(images, owner, 2)]
+    for a, b in zip(got, want):
+        assert a.dtype == BF16 and float(((a.float() - b).norm() / b.norm()).detach()) < 8 * 2 ** -8 * 4
+    got[1].float().square().sum().backward()
+    for name, t in net.named_parameters():
+        assert t.grad is not None and t.grad.dtype == F32 and bool(torch.isfinite(t.grad).all()) and bool(t.grad.any()), name

@@ -160,7 +160,7 @@ class ScatteringAttention(torch.nn.Module):
         x = self.forward(images, documents)
         B, T = x.shape[:2]
         k, v = self.pool_kv(x).view(B, T, 2 * self.key_heads, self.dim).split((self.key_heads, self.key_heads), 2)
-        q = self.pool_query.expand(B, count, -1, -1)
+        q = self.pool_query.to(k.dtype).expand(B, count, -1, -1)        # autocast gives k another type
         if documents is not None:
             documents = self._places(documents, x)
             series = torch.arange(count, dtype=torch.int32, device=x.device)
