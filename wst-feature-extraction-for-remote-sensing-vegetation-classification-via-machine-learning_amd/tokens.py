@@ -417,6 +417,7 @@ def attention(q, k, v, *, scale=None, cap=0.0, slopes=None, q_positions=None, k_
     * ``q_documents[i] == k_documents[j] >= 0`` where given (int32 (T,) or (B, T); negative belongs to none).
 
     What is not seen has no influence, not even infinities or NaN.  A query that sees nothing gets 0, and no gradient.
+    16-bit types round the weights that multiply v, and the score gradients that multiply q and k, to their own type.
     Gradients reach q, k, v and slopes.  In float16 the backward pass does rows and keys whose score gradients exceed
     2**10 over, one by one: right, but slow where a loss scale makes that most of them (1024 tokens, 8 heads of 64: 100 us,
     with output gradients of 2**10 450 us and of 2**13 5.3 ms); bfloat16 has no such bound.  So it is in every type for
