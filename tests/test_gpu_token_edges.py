@@ -250,3 +250,34 @@ def test_scattering_attention_under_autocast():
     got[1].float().square().sum().backward()
     for name, t in net.named_parameters():
         assert t.grad is not None and t.grad.dtype == F32 and bool(torch.isfinite(t.grad).all()) and bool(t.grad.any()), name
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("D", [32, 128, 12])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("height", [0.0, 2.0 ** 10, 2.0 ** 17])
+def test_attention_16_bit_slope_gradients_of_high_scores(height, causal, D, dtype):
+    """The slopes' gradient is a float32 sum in 16-bit calls too, and meets the log-sum-exp's rounding as float32 gradients do.
+    delta, taken from an output in two 16-bit parts, leaves the gradient where the weights add up to 1: sum ds (far - sum p far)
+    is the same for every delta. A pair's own error is at most (64 + D) 2^-24 of its magnitude (the exponent's and the sums'
+    roundings as above, a row's sum of weights being a tree of T / 16 steps and 4); pairs round independently, and a sum of
+    independent errors lies within 8 times the root of the sum of their squares."""
+    T, H = 160, 2
+    g = _gen(int(height) + D)
+    q, k = (torch.randint(-4, 5, (1, T, H, D), generator=g).float() / 8 for _ in range(2))
+    q[..., 4:], k[..., 4:] = 0, 0
+    q[..., 0], k[..., 0] = height / 4, 4.0
+    v, do = torch.randn(1, T, H, D, generator=g), torch.randn(1, T, H, D, generator=g)
+    q, k, v, do = (t.to(dtype) for t in (q, k, v, do))
+    slopes = torch.full((H,), 2.0 ** -6, device="cuda", requires_grad=True)
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+    o = tokens.attention(*leaves, scale=1.0, slopes=slopes, causal=causal)
+    got = torch.autograd.grad(o, slopes, do.cuda())[0].double().cpu()
+    Q, K, V, G = (t.double().transpose(1, 2) for t in (q, k, v, do))
+    far = (torch.arange(T)[:, None] - torch.arange(T)).abs().double()
+    z = Q @ K.transpose(2, 3) - 2.0 ** -6 * far
+    p = (z.masked_fill(~torch.ones(T, T).tril().bool(), -torch.inf) if causal else z).softmax(-1)
+    dp, most = G @ V.transpose(2, 3), G.abs() @ V.abs().transpose(2, 3)
+    ds, size = p * (dp - (p * dp).sum(-1, keepdim=True)), p * (most + (p * most).sum(-1, keepdim=True))
+    want, bound = -(ds * far).sum((0, 2, 3)), 8 * (64 + D) * 2.0 ** -24 * (size * far).square().sum((0, 2, 3)).sqrt()
+    assert bool(((got - want).abs() <= bound).all()), ((got - want).abs() / bound).tolist()

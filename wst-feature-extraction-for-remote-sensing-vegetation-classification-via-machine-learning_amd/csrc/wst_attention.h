@@ -176,7 +176,7 @@ __device__ void row_forward(const AttnArgs& a, const Scope& sc, int64_t b, int h
 
 // What makes a row's rebuilt weights add up to 1. They come as exp(s - lse), and lse is a float32 number: its rounding is
 // half an ulp of the largest score, the same for all weights of the row (and in powers of two once more). 16-bit weights lose
-// more when they are rounded; float32 gradients are the nearer to the exact ones so (256 keys: dq 3.9e-7 for 5.0e-7, dk 3.2
+// more when they are rounded, and only the slopes' gradients take it there; float32 gradients are the nearer to the exact ones so (256 keys: dq 3.9e-7 for 5.0e-7, dk 3.2
 // for 4.5, dv 3.0 for 4.5; 16 x 256, 4 heads x 32: dk/dv 23.5 us for 22.6, dq no slower), most of all where scores stand far
 // from 0 (at 1e5 a log-sum-exp of float32 is off by 4e-3).
 __device__ __forceinline__ float unit_of(float sum) { return sum > 0.f && sum < INFINITY ? 1.f / sum : 1.f; }
@@ -195,7 +195,7 @@ __device__ float row_dq(const AttnArgs& a, const Scope& sc, int64_t b, int h, in
     const float slope = d.slopes ? d.slopes[h] : 0.f;
     const int64_t row = (b * d.q_heads + h) * d.q_len + i;
     const float lse = a.g.lse[row], delta = a.delta[row];
-    float acc[kPer] = {}, share = 0.f, sum = 0.f;
+    float acc[kPer] = {}, sum = 0.f, pf = 0.f, e0 = 0.f, e1 = 0.f;      // as in k_attn_dq
     if (lse != -INFINITY)
         for (int j0 = 0; j0 < sc.length; j0 += 64) {
             const int j = j0 + lane;
@@ -209,7 +209,9 @@ __device__ float row_dq(const AttnArgs& a, const Scope& sc, int64_t b, int h, in
                 const float p = expf(s - lse);
                 sum += p;
                 const float ds = p * (dot_row(dout, at<T>(d.v, d.v_strides, b, j, kvh), d.dim) - delta);
-                share -= ds * far;
+                pf += p * far;
+                e0 += ds;
+                e1 += ds * far;
                 dz = ds * grad * d.scale;
             }
             for (uint64_t w = __ballot(see); w; w &= w - 1) {
@@ -221,7 +223,7 @@ __device__ float row_dq(const AttnArgs& a, const Scope& sc, int64_t b, int h, in
                     if (lane + 64 * c < d.dim) acc[c] += x * static_cast<float>(k[lane + 64 * c]);
             }
         }
-    const float unit = a.unit ? unit_of(wave_sum(sum)) : 1.f;
+    const float unit = unit_of(wave_sum(sum));
     if (a.unit && lane == 0) a.unit[row] = unit;
     if (a.g.dq) {
         T* o = const_cast<T*>(at<T>(a.g.dq, a.g.dq_strides, b, i, h));
@@ -229,7 +231,7 @@ __device__ float row_dq(const AttnArgs& a, const Scope& sc, int64_t b, int h, in
         for (int c = 0; c < kPer; ++c)
             if (lane + 64 * c < d.dim) o[lane + 64 * c] = static_cast<T>(acc[c] * unit);
     }
-    return wave_sum(share) * unit;
+    return (wave_sum(e0) * (wave_sum(pf) * unit) - wave_sum(e1)) * unit;
 }
 
 // The gradients of one key and value, over all queries of the heads that share it. LDS: k and v of the row.
@@ -1493,8 +1495,10 @@ __global__ __launch_bounds__(256 * TEAMS, sizeof(T) == 2 ? 2 : 1) void k_attn_dq
 #pragma unroll
     for (int k = 0; k < DP / 32; ++k) dq[k] = zero16();
     // The slopes' share, -sum ds far. delta comes from the rounded output, and its error would meet a mean distance: with
-    // e = sum ds (0, were delta exact) the share is -(sum ds far - e sum p far).
-    float pf = 0.f, e0 = 0.f, e1 = 0.f, whole_p = 0.f;      // whole_p: float32, the sum of the weights (unit_of)
+    // e = sum ds (0, were delta exact) the share is -(sum ds far - e sum p far), the weights made to add up to 1 in every
+    // type: it is a float32 sum that stays (bfloat16, 25 x 4001 in order: 8.9e-7 from the exact one before, 0.9e-7 so; dq
+    // 86 us and 87.5).
+    float pf = 0.f, e0 = 0.f, e1 = 0.f, whole_p = 0.f;      // whole_p: the sum of the weights (unit_of)
     const bool slopes_too = a.slope_part != nullptr;
 
     const T *kb = at<T>(d.k, d.k_strides, b, 0, kvh), *vb = at<T>(d.v, d.v_strides, b, 0, kvh);
@@ -1580,6 +1584,7 @@ __global__ __launch_bounds__(256 * TEAMS, sizeof(T) == 2 ? 2 : 1) void k_attn_dq
             if constexpr (sizeof(T) == 4) whole_p += sum16(x);
             if (kind.bias && slopes_too) {
                 float u = 0.f, v = 0.f, y = 0.f;       // sums of their own first: thousands of terms lose little so
+                if constexpr (sizeof(T) == 2) whole_p += sum16(x);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     u = fmaf(x[r], far[r], u);
@@ -1617,8 +1622,8 @@ __global__ __launch_bounds__(256 * TEAMS, sizeof(T) == 2 ? 2 : 1) void k_attn_dq
     while (!cur.done(walk) && !marked) work(std::integral_constant<int, 1>{});
     while (!cur.done(walk)) work(std::integral_constant<int, 2>{});
     if constexpr (TEAMS > 1) {
-        static_assert(sizeof(pool) >= 4 * (DP / 2 + 3) * 64 * sizeof(float), "room for the sums");
-        float* sums = reinterpret_cast<float*>(pool) + w * ((DP / 2 + 3) * 64) + lane;
+        static_assert(sizeof(pool) >= 4 * (DP / 2 + 4) * 64 * sizeof(float), "room for the sums");
+        float* sums = reinterpret_cast<float*>(pool) + w * ((DP / 2 + 4) * 64) + lane;
         if (team && behind) __syncthreads();
         __syncthreads();
         if (team) {
@@ -1629,6 +1634,7 @@ __global__ __launch_bounds__(256 * TEAMS, sizeof(T) == 2 ? 2 : 1) void k_attn_dq
             sums[(DP / 2) * 64] = pf;
             sums[(DP / 2 + 1) * 64] = e0;
             sums[(DP / 2 + 2) * 64] = e1;
+            sums[(DP / 2 + 3) * 64] = whole_p;
         }
         __syncthreads();
         if (team) return;
@@ -1639,11 +1645,12 @@ __global__ __launch_bounds__(256 * TEAMS, sizeof(T) == 2 ? 2 : 1) void k_attn_dq
         pf += sums[(DP / 2) * 64];
         e0 += sums[(DP / 2 + 1) * 64];
         e1 += sums[(DP / 2 + 2) * 64];
+        whole_p += sums[(DP / 2 + 3) * 64];
     }
     const AttnArgs& z = again();
-    float mul = z.d.scale / kUp<T>, unit = 1.f;
+    float mul = z.d.scale / kUp<T>;
+    const float unit = unit_of(halves_sum(whole_p));
     if constexpr (sizeof(T) == 4) {
-        unit = unit_of(halves_sum(whole_p));
         mul *= unit;
         if (ok && hl == 0) z.unit[row] = unit;
     }
